@@ -263,8 +263,9 @@ def prepare(case, seed):
         cache = _own_cache(case, 1, state["pages"], device)
         for name, (idx, absmax) in rows.items():
             packed = idx[..., 0::2] | (idx[..., 1::2] << 4)
-            getattr(cache, name + "_codes")[0].copy_(packed.view(-1, page, heads, d // 2).transpose(1, 2))
-            getattr(cache, name + "_absmax")[0].copy_(absmax.view(-1, page, heads, nb).transpose(1, 2))
+            # the cache's views: pages, heads, groups of 16 tokens, tokens, bytes or blocks
+            for view, rows_ in ((getattr(cache, name + "_codes")[0], packed), (getattr(cache, name + "_absmax")[0], absmax)):
+                view.copy_(rows_.view(-1, page // 16, 16, heads, rows_.shape[-1]).permute(0, 3, 1, 2, 4))
         state["cache"] = cache
     else:
         for name, (idx, absmax) in rows.items():
