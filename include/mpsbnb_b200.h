@@ -425,6 +425,76 @@ int mpsbnb_linear_fp8_e4m3(const void *x, int x_dtype, int64_t M, const uint8_t 
                            const float *scales, int64_t N, int64_t K, const void *bias, void *y,
                            int y_dtype, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged key/value cache in 4 bits, and the attention that reads it
+ *
+ * No reference counterpart (the reference quantises weights and embeddings only); codes, absmax and
+ * rounding are those of quantize_4bit (functional.py:216-255) with block sizes of 32 or 64 inside a row.
+ *
+ *   data   uint8 [num_layers][num_pages][kv_heads][page_size / 16][group bytes], 16-byte aligned.  A group is
+ *          16 tokens of one head: K codes [16][head_dim / 2], K absmax [16][head_dim / blocksize] in `dtype`,
+ *          V codes, V absmax - so a kernel fetches 16 tokens' keys and values with one bulk copy.
+ *          A byte holds two codes, low nibble = even element.
+ * head_dim 64, 128 or 256; blocksize 32 or 64; page_size a power of two from 16 to 1024; dtype F16 or BF16.
+ * A block's absmax is kept in `dtype`: max(|x|, 1e-8) of a 16-bit block is a 16-bit number except for the 1e-8
+ * itself, whose blocks stand for zeros (F16) or magnitudes below 1e-8 (BF16).  A block with an infinity or a NaN
+ * reads back as NaN.
+ * ------------------------------------------------------------------------------------- */
+typedef struct mpsbnb_kv4_cache {
+    void *data;
+    int64_t num_pages;
+    int num_layers, kv_heads, head_dim, page_size, blocksize, quant_type, dtype;
+} mpsbnb_kv4_cache;
+
+/* The sequences of a call.  Sequence b holds seq_lens[b] tokens (the call's new ones included; clamped to what its
+ * row of the page table can hold) in the pages page_table[b * table_ld + 0 ...].  Its new tokens are rows
+ * cu_seqlens[b] ... cu_seqlens[b + 1] - 1 of the call's [tokens, ...] tensors, or rows b * new_tokens ... with
+ * cu_seqlens NULL; they take the last places of the sequence.  new_tokens is the largest number of new tokens of a
+ * sequence (more are not looked at).  All tables are int32 on the device. */
+typedef struct mpsbnb_kv4_seqs {
+    const int32_t *page_table;
+    int64_t table_ld;
+    const int32_t *seq_lens;
+    const int32_t *cu_seqlens;
+    int64_t tokens;
+    int table_width, batch, new_tokens;
+} mpsbnb_kv4_seqs;
+
+size_t mpsbnb_kv4_group_bytes(int head_dim, int blocksize);
+size_t mpsbnb_kv4_cache_bytes(const mpsbnb_kv4_cache *cache);
+
+/* Quantises the new tokens' rows into their places.  k, v: [tokens, kv_heads, head_dim] in the cache's dtype with
+ * strides (in elements) between tokens and heads, head_dim contiguous.  Rows past cu_seqlens[batch], and tokens
+ * whose place is negative (a sequence shorter than its new tokens), are skipped; so are tokens whose page number is
+ * outside the cache, which raise device status 401.  Pages that are written belong to one sequence only. */
+int mpsbnb_kv4_append(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *k,
+                      int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                      int64_t v_head_stride, void *stream);
+
+/* The cached rows as they stand: k, v [batch, max_len, kv_heads, head_dim] in the cache's dtype (16-byte aligned,
+ * contiguous), fl(code * absmax) with the product in fp32; places at or past seq_lens[b] are zeros, places in a page
+ * outside the cache NaN (device status 401).  seqs: cu_seqlens, tokens and new_tokens are not looked at. */
+int mpsbnb_kv4_dequantize(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, int64_t max_len,
+                          void *k, void *v, void *stream);
+
+/* Copies whole pages src[i] -> dst[i] in all layers.  src, dst: HOST arrays; page numbers inside the cache, every
+ * destination once, no page both source and destination (INVALID_ARG otherwise, nothing copied). */
+int mpsbnb_kv4_copy_pages(const mpsbnb_kv4_cache *cache, const int32_t *src, const int32_t *dst, int64_t n, void *stream);
+
+/* out = softmax(scale * q K^T) V over the cached keys and values of each row's sequence; heads / kv_heads
+ * consecutive query heads share a key/value head.  The query of place p (its token's place in the sequence) sees the
+ * keys at places max(0, p - window + 1) ... p when causal (window 0: no lower limit), all of the sequence otherwise
+ * (window must then be 0).  A row that sees no key gives zeros and lse = -inf.  Rows past cu_seqlens[batch] are left
+ * as they were.  A row that sees a page outside the cache gives NaN (device status 401).
+ *   q    [tokens, heads, head_dim] in the cache's dtype, strides in elements, head_dim contiguous
+ *   out  [tokens, heads, head_dim] contiguous, in the cache's dtype;  lse  NULL or fp32 [tokens, heads], natural log
+ * Scores, softmax statistics and sums are fp32; probabilities and codes enter the products as fp16.
+ * workspace: mpsbnb_attention_4bit_workspace_bytes() bytes, 16-byte aligned, used by this call only while it runs. */
+size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads);
+int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
+                          int64_t q_token_stride, int64_t q_head_stride, int heads, int causal, int window, float scale,
+                          void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

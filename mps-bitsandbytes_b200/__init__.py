@@ -14,6 +14,8 @@ from .functional import (  # noqa: F401
     dequantize_nf4, dequantize_rowwise, double_quant, matmul_4bit, matmul_colrow, matmul_fp4,
     matmul_fp8_e4m3, matmul_int8, matmul_nf4, quantize_4bit, quantize_blockwise, quantize_colrow,
     quantize_fp4, quantize_fp8_e4m3, quantize_nf4, quantize_rowwise)
+from .kv_cache import (  # noqa: F401
+    KVCache4bit, append_kv_4bit, attention_4bit, copy_kv_pages_4bit, dequantize_kv_4bit)
 from .nn import (  # noqa: F401
     Embedding4bit, Embedding8bit, EmbeddingFP4, EmbeddingNF4, Linear4bit, Linear8bit, LinearFP8,
     OutlierAwareLinear, Params4bit)

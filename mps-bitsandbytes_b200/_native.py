@@ -48,6 +48,18 @@ class GroupPlan(C.Structure):
                 ("wait_add", C.c_int), ("acc_parts", C.c_int), ("n_segments", C.c_int), ("wait_seg_mul", C.c_int), ("ep", GroupEpilogue)]
 
 
+class Kv4Cache(C.Structure):
+    """mpsbnb_kv4_cache of include/mpsbnb_b200.h."""
+    _fields_ = [("data", C.c_void_p), ("num_pages", C.c_int64), ("num_layers", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("page_size", C.c_int), ("blocksize", C.c_int), ("quant_type", C.c_int), ("dtype", C.c_int)]
+
+
+class Kv4Seqs(C.Structure):
+    """mpsbnb_kv4_seqs of include/mpsbnb_b200.h."""
+    _fields_ = [("page_table", C.c_void_p), ("table_ld", C.c_int64), ("seq_lens", C.c_void_p), ("cu_seqlens", C.c_void_p),
+                ("tokens", C.c_int64), ("table_width", C.c_int), ("batch", C.c_int), ("new_tokens", C.c_int)]
+
+
 class NativeLibraryError(RuntimeError):
     pass
 
@@ -65,9 +77,18 @@ def lib():
         l.mpsbnb_last_cuda_error_string.restype = C.c_char_p
         for name in ("mpsbnb_gemv_4bit_group_plan_bytes", "mpsbnb_gemm_4bit_workspace_bytes", "mpsbnb_matmul_int8_workspace_bytes",
                      "mpsbnb_linear_int8_workspace_bytes", "mpsbnb_linear_fp8_workspace_bytes",
-                     "mpsbnb_outlier_linear_workspace_bytes", "mpsbnb_gemm_4bit_static_max_bytes", "mpsbnb_gemm_4bit_static_bytes"):
+                     "mpsbnb_outlier_linear_workspace_bytes", "mpsbnb_gemm_4bit_static_max_bytes", "mpsbnb_gemm_4bit_static_bytes",
+                     "mpsbnb_kv4_group_bytes", "mpsbnb_kv4_cache_bytes", "mpsbnb_attention_4bit_workspace_bytes"):
             if hasattr(l, name):
                 getattr(l, name).restype = C.c_size_t
+        # the cache's entry points take plain Python numbers (a call per layer and token: conversions count)
+        ptr_, i64_, int_ = C.c_void_p, C.c_int64, C.c_int
+        kv, sq = C.POINTER(Kv4Cache), C.POINTER(Kv4Seqs)
+        l.mpsbnb_kv4_append.argtypes = [kv, int_, sq, ptr_, i64_, i64_, ptr_, i64_, i64_, ptr_]
+        l.mpsbnb_kv4_dequantize.argtypes = [kv, int_, sq, i64_, ptr_, ptr_, ptr_]
+        l.mpsbnb_kv4_copy_pages.argtypes = [kv, C.POINTER(C.c_int32), C.POINTER(C.c_int32), i64_, ptr_]
+        l.mpsbnb_attention_4bit_workspace_bytes.argtypes = [kv, sq, int_]
+        l.mpsbnb_attention_4bit.argtypes = [kv, int_, sq, ptr_, i64_, i64_, int_, int_, int_, C.c_float, ptr_, ptr_, ptr_, C.c_size_t, ptr_]
         _lib = l
     return _lib
 

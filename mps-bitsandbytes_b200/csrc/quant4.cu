@@ -13,6 +13,7 @@
 // oracle/oracle.c:o_prove_quantizer with block maxima in [1e-30, 1e30]; fp32 input and maxima
 // outside that range use IEEE division.
 #include "common.cuh"
+#include "kv4.cuh"
 
 namespace mpsbnb {
 
@@ -324,6 +325,108 @@ quantize4_stream_kernel(const T *__restrict__ A, IDX total, uint8_t *__restrict_
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// ------------------------------------------------------------------------------------------
+// Rows of keys and values into their places in the paged cache (kv4.cuh): the quantiser above with a scattered
+// destination.  A thread owns 8 elements (one 16-byte load where the rows allow it, one 32-bit store), bs / 8 lanes a
+// block; K and V are the two halves of the index range, so one launch stores a layer's new tokens.
+// ------------------------------------------------------------------------------------------
+static __device__ int g_kv4_append_status = 0;
+
+template <typename T, int QT, int LPB>
+__global__ void __launch_bounds__(256)
+kv4_append_kernel(const Kv4Layer kv, const Kv4Seqs sq, const T *__restrict__ k, int64_t k_ts, int64_t k_hs,
+                  const T *__restrict__ v, int64_t v_ts, int64_t v_hs, int head_dim, int vec) {
+    __shared__ float2 nf4_tab[16];
+    if (QT == MPSBNB_NF4) {
+        if (threadIdx.x < 16) nf4_bucket_table_fill(nf4_tab, threadIdx.x);
+        __syncthreads();
+    }
+    const int cpr = head_dim / 8;                                  // chunks of a row: 8, 16 or 32, all in one warp
+    const int64_t rows = (int64_t)sq.tokens * kv.kv_heads, total = 2 * rows * cpr;
+    const int lane = threadIdx.x & 31;
+    const int64_t stride = (int64_t)gridDim.x * 256;
+    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c - lane < total; c += stride) {
+        const int64_t r = c / cpr;
+        const int kc = (int)(c - r * cpr);
+        const bool is_v = r >= rows;
+        const int64_t rr = is_v ? r - rows : r;
+        const int t = (int)(rr / kv.kv_heads), h = (int)(rr - (int64_t)t * kv.kv_heads);
+        bool live = c < total;
+        int place = 0, page = 0;
+        if (live) {                                                // where the token goes
+            int b, i, row, n, len;
+            if (sq.cu == nullptr) {
+                b = t / sq.new_tokens;
+            } else {
+                int lo = 0, hi = sq.batch;                         // last sequence that starts at or before t
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (__ldg(sq.cu + mid) <= t) lo = mid; else hi = mid;
+                }
+                b = lo;
+            }
+            sq.get(b, row, n, len);
+            i = t - row;
+            place = len - n + i;
+            live = i >= 0 && i < n && place >= 0;
+            if (live) {
+                page = __ldg(sq.table + (int64_t)b * sq.table_ld + (place >> kv.page_shift));
+                if (page < 0 || page >= kv.num_pages) {
+                    if (kc == 0) atomicExch(&g_kv4_append_status, KV4_BAD_PAGE);
+                    live = false;
+                }
+            }
+        }
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        if (live) {
+            const T *src = (is_v ? v + (int64_t)t * v_ts + (int64_t)h * v_hs : k + (int64_t)t * k_ts + (int64_t)h * k_hs) + kc * 8;
+            if (vec) {
+                raw = __ldg(reinterpret_cast<const uint4 *>(src));
+            } else {
+                const uint16_t *s16 = reinterpret_cast<const uint16_t *>(src);
+                raw = make_uint4(s16[0] | (uint32_t)s16[1] << 16, s16[2] | (uint32_t)s16[3] << 16,
+                                 s16[4] | (uint32_t)s16[5] << 16, s16[6] | (uint32_t)s16[7] << 16);
+            }
+        }
+        float x[8];
+        {
+            const T *hv = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(hv[j]);
+        }
+        // largest magnitude by its bits: a NaN orders above infinity and is not lost
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < LPB; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!live) continue;
+        const float a = m >= 0x7f800000u ? __int_as_float(0x7fc00000) : fmaxf(__uint_as_float(m), 1e-8f);
+        uint32_t word = 0;
+        if (a > 1e-8f && a <= 1e30f) {                             // a 16-bit input's magnitude: the shortcut is proven exact
+            const float ri = __frcp_rn(a);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) word |= code_fast<QT>(block_div<true>(x[j], a, ri), nf4_tab) << (4 * j);
+        } else {                                                   // (a NaN block: any codes will do)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) word |= code_fast<QT>(block_div<false>(x[j], a, 0.f), nf4_tab) << (4 * j);
+        }
+        uint8_t *g = kv.group(page, h, place) + (is_v ? kv.half_bytes : 0);
+        const int slot = place & (KV4_GROUP - 1);
+        reinterpret_cast<uint32_t *>(g + slot * (head_dim / 2))[kc] = word;
+        if ((kc & (LPB - 1)) == 0) reinterpret_cast<T *>(g + kv.scale_off)[slot * (cpr / LPB) + kc / LPB] = from_f32<T>(a);
+    }
+}
+
+int kv4_append_status_fetch(int *out, bool reset) {
+    MPSBNB_CUDA_TRY(cudaMemcpyFromSymbol(out, g_kv4_append_status, sizeof(int)));
+    if (reset) {
+        const int zero = 0;
+        MPSBNB_CUDA_TRY(cudaMemcpyToSymbol(g_kv4_append_status, &zero, sizeof(int)));
+    }
+    return MPSBNB_OK;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -748,5 +851,40 @@ extern "C" int mpsbnb_dequantize_blockwise(const int8_t *q, const float *absmax,
     const int grid = grid_for(n, 256, 16);
     MPSBNB_DISPATCH_DTYPE(out_dtype, T, (dequantize_blockwise_kernel<T><<<grid, 256, 0, (cudaStream_t)stream>>>(
                                             q, absmax, n, blocksize, (T *)out)));
+    return check_launch();
+}
+
+extern "C" int mpsbnb_kv4_append(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *k,
+                                 int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                                 int64_t v_head_stride, void *stream) {
+    int rc = kv4_check_cache(cache, layer);
+    if (rc == MPSBNB_OK) rc = kv4_check_seqs(seqs, cache);
+    if (rc != MPSBNB_OK) return rc;
+    if (seqs->tokens == 0 || seqs->batch == 0 || seqs->new_tokens == 0) return MPSBNB_OK;
+    if (k == nullptr || v == nullptr || k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0) return MPSBNB_ERR_INVALID_ARG;
+    const Kv4Layer kv = kv4_layer(cache, layer);
+    const Kv4Seqs sq = kv4_seqs(seqs, cache);
+    const int vec = aligned16(k) && aligned16(v) && ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
+    const int64_t total = 2 * seqs->tokens * cache->kv_heads * (cache->head_dim / 8);
+    const int grid = grid_for(total, 256, 16);
+    cudaStream_t st = (cudaStream_t)stream;
+#define LAUNCH_APPEND(T, QT, LPB)                                                                                   \
+    kv4_append_kernel<T, QT, LPB><<<grid, 256, 0, st>>>(kv, sq, (const T *)k, k_token_stride, k_head_stride, (const T *)v, \
+                                                        v_token_stride, v_head_stride, cache->head_dim, vec)
+#define LAUNCH_APPEND_LPB(T, QT)                                                                                    \
+    do {                                                                                                            \
+        if (cache->blocksize == 32) LAUNCH_APPEND(T, QT, 4);                                                        \
+        else LAUNCH_APPEND(T, QT, 8);                                                                               \
+    } while (0)
+#define LAUNCH_APPEND_QT(T)                                                                                         \
+    do {                                                                                                            \
+        if (cache->quant_type == MPSBNB_NF4) LAUNCH_APPEND_LPB(T, MPSBNB_NF4);                                      \
+        else LAUNCH_APPEND_LPB(T, MPSBNB_FP4);                                                                      \
+    } while (0)
+    if (cache->dtype == MPSBNB_F16) LAUNCH_APPEND_QT(__half);
+    else LAUNCH_APPEND_QT(__nv_bfloat16);
+#undef LAUNCH_APPEND_QT
+#undef LAUNCH_APPEND_LPB
+#undef LAUNCH_APPEND
     return check_launch();
 }
