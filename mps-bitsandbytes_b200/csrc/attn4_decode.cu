@@ -16,10 +16,10 @@
 //    of byte -> (low nibble's value, high nibble's), held once per lane so that 32 look-ups never meet in a bank.
 //    For V the pair has to run along tokens: the nibbles of two tokens' words are first brought into one byte.
 //  * A block's absmax multiplies the fp32 score (K) or the probability (V), never a code: K enters the product
-//    with the rounding of the 16 code values to fp16 only (2^-12 of the value).
+//    with the rounding of the 16 code values to fp16 only.
 //  * Softmax: probabilities are 2^(x - m) with a reference m that follows the running maximum only when a score
 //    exceeds it by 2^8: one vote per tile instead of a reduction, and fp32 sums lose nothing by it.  The weight
-//    p * absmax goes to fp16 under a power-of-two factor per row that is raised the same way (above 2^12).
+//    p * absmax goes to fp16 under a power-of-two factor per row that is raised the same way (above 2^15).
 //    bf16 queries are brought to fp16 by a power of two per row: exact, but for parts below 2^-24 of the row's largest.
 #include <type_traits>
 
@@ -171,7 +171,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
 
     // ------------------------------------------------------------ table, barriers
     {
-        const float mine = kCode[A.quant_type][lane & 15];
+        const float mine = kCode[A.quant_type][lane & 15] * attn4_code_scale(A.quant_type);
         for (int b = warp; b < 256; b += AD_WARPS) {
             const float lo = __shfl_sync(0xffffffffu, mine, b & 15), hi = __shfl_sync(0xffffffffu, mine, b >> 4);
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(sb + (uint32_t)(S::LUT + b * 128 + lane * 4)), "r"(ad_half2(lo, hi)) : "memory");
@@ -248,7 +248,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 raw[k] = make_uint2(0u, 0u);
                 if (ok) raw[k] = __ldg(reinterpret_cast<const uint2 *>(src + (k / MB) * BS + c * (BS / 4) + (k % MB) * 4));
             }
-            float fr = A.scale_log2;
+            float fr = A.scale_log2 * attn4_code_unscale(A.quant_type);
             if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
                 uint32_t mx = 0;                                     // largest magnitude of the row, as bits of bf16
 #pragma unroll
@@ -418,7 +418,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                         float w = pu * (j < 2 ? sv0[blk] : sv1[blk]);
                         if (masked && !(seen >> (nt * 4 + j) & 1u)) w = 0.0f;   // whatever lies in an unseen place
                         wt[blk][nt][j] = w;
-                        large |= w > 4096.0f;
+                        large |= w > 32768.0f;
                     }
                 }
             if (__any_sync(0xffffffffu, large)) {
@@ -435,8 +435,8 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                         }
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                        const int e = max(1, min(253, (int)(__float_as_uint(mx) >> 23)));
-                        const float un = fminf(up[nt][j], __int_as_float((254 - e) << 23));
+                        const int e = max(4, min(253, (int)(__float_as_uint(mx) >> 23)));
+                        const float un = fminf(up[nt][j], __int_as_float((257 - e) << 23));   // the largest comes to [8, 16)
                         const float k = un * __frcp_rn(up[nt][j]);    // powers of two: exact
                         up[nt][j] = un;
 #pragma unroll
@@ -497,7 +497,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 float M = m[nt][j];
 #pragma unroll
                 for (int w = 0; w < AD_WARPS; ++w) M = fmaxf(M, stat[w * RT + nt * 8 + 2 * c + j].x);
-                const float k = ex2(m[nt][j] - M) * __frcp_rn(up[nt][j]);
+                const float k = ex2(m[nt][j] - M) * __frcp_rn(up[nt][j]) * attn4_code_unscale(A.quant_type);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k; o[i][nt][j + 2] *= k; }
             }
@@ -689,6 +689,7 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.out = out; a.lse = lse; a.ws = (float *)workspace;
     a.heads = heads; a.group = group; a.causal = causal != 0; a.window = window; a.quant_type = cache->quant_type;
     a.scale_log2 = scale * 1.4426950408889634f;
+    if ((int64_t)seqs->new_tokens * group >= 128) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, (cudaStream_t)stream);
     const int nt = ad_nt(seqs, group);
     const int rts_max = (seqs->new_tokens * group + 8 * nt - 1) / (8 * nt);
     cudaStream_t st = (cudaStream_t)stream;

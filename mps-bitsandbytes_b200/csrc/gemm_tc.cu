@@ -318,7 +318,7 @@ extern "C" int mpsbnb_device_status(int *status_out, int reset) {
     const int rc4 = wq_status_fetch(&other, reset != 0);
     if (rc4 != MPSBNB_OK) return rc4;
     if (*status_out == 0) *status_out = other;
-    for (auto fetch : {kv4_append_status_fetch, kv4_status_fetch, attn4_decode_status_fetch}) {
+    for (auto fetch : {kv4_append_status_fetch, kv4_status_fetch, attn4_decode_status_fetch, attn4_prompt_status_fetch}) {
         const int rc5 = fetch(&other, reset != 0);
         if (rc5 != MPSBNB_OK) return rc5;
         if (*status_out == 0) *status_out = other;

@@ -94,5 +94,6 @@ inline Kv4Seqs kv4_seqs(const mpsbnb_kv4_seqs *s, const mpsbnb_kv4_cache *c) {
 int kv4_status_fetch(int *out, bool reset);              // kv4.cu
 int kv4_append_status_fetch(int *out, bool reset);       // quant4.cu
 int attn4_decode_status_fetch(int *out, bool reset);     // attn4_decode.cu
+int attn4_prompt_status_fetch(int *out, bool reset);     // attn4_prompt.cu
 
 }  // namespace mpsbnb

@@ -42,12 +42,14 @@ def attention(q, cache, layer, table, lens, starts, causal=True, window=None, sc
     """(out, lse, bound) in 64 bits; rows that belong to no sequence are NaN.  ``bound`` is how far the kernels may be off
     before their result is rounded to the cache's type:
 
-    a code enters the products with fp16's rounding, off by 2^-11 of itself at most (so does a bf16 query's part below 2^-14 of its
-    row's largest: under 2^-25 of that).  A score is then off by e = scale sum_d |q_d k_d| 2^-11 + scale max|q| sum_d |k_d| 2^-25,
-    a probability by a factor within exp(+-2 e_max) (numerator and denominator), the weight p * absmax by another 2^-11 or, far
-    below its row's largest weight (2^-14 of a reference that is at most 4096 times the first one), by 2^-25 of 4096 times the
-    largest; the value's code by 2^-11.  fp32 sums of n terms add 2^-24 each step at most: n * 2^-23 covers numerator and
-    denominator, scores' sums and the exponential's last bits included with 2^-18.
+    an element of K or V enters its product with two fp16 roundings at most, of its code and of code * absmax: off by 2 * 2^-11
+    of itself (and, under the power of two that brings the largest absmax of a tile to 2^8, by 2^-25 of that unit: 2^-33 of the
+    tile's largest).  A bf16 query is exact but for parts under 2^-14 of its row's largest, off by 2^-25 of that.  So a score is off by
+    e = scale (2 * 2^-11 sum_d |q_d k_d| + 2^-25 max|q| sum_d |k_d| + 2^-33 max|k| sum_d |q_d|) and a probability by a factor within
+    exp(+-2 e_max) (numerator and denominator).  A weight p * absmax, or p, is rounded to fp16: by 2^-11 of itself, or, being
+    small, by 2^-25 under a reference that is at least 8 for the largest weight (single tokens) or 2^7 for the largest p (prompts,
+    where V's own 2^-33 adds as much again at most).  fp32 sums of n terms add 2^-24 each step at most: n * 2^-23 covers numerator
+    and denominator, and 2^-18 the scores' sums and the last bits of the exponential.
     """
     T, H, D = q.shape
     group = H // cache.num_kv_heads
@@ -78,11 +80,13 @@ def attention(q, cache, layer, table, lens, starts, causal=True, window=None, sc
             out[a:e, h] = p @ vv
             if length == 0:
                 continue
-            err = abs(scale) * ((x.abs() @ kk.abs().T) * 2.0 ** -11 + x.abs().amax(-1, keepdim=True) * kk.abs().sum(-1)[None] * 2.0 ** -25)
+            err = abs(scale) * ((x.abs() @ kk.abs().T) * 2 * 2.0 ** -11 + x.abs().amax(-1, keepdim=True) * kk.abs().sum(-1)[None] * 2.0 ** -25
+                                + kk.abs().max() * x.abs().sum(-1, keepdim=True) * 2.0 ** -33)
             err = err.masked_fill(~seen, 0.0).amax(-1, keepdim=True)
-            rel = torch.expm1(2 * err) + 2 * 2.0 ** -11 + length * 2.0 ** -23 + 2.0 ** -18
-            top = (p[:, :, None] * vv.abs().amax(-1)[None, :, None]).amax(1) if n * length < 1 << 24 else vv.abs().max()
-            bound[a:e, h] = (p @ vv.abs()) * rel + length * 2.0 ** -25 * 4096 * top * 2.0 ** -14
+            rel = torch.expm1(2 * err) + 3 * 2.0 ** -11 + length * 2.0 ** -23 + 2.0 ** -18
+            size = vv.abs().amax(-1)                                 # per key
+            small = 2.0 ** -28 * (p * size).amax(-1, keepdim=True) + 2 * 2.0 ** -32 * p.amax(-1, keepdim=True) * size.max()
+            bound[a:e, h] = (p @ vv.abs()) * rel + length * small
     return out, lse, bound
 
 

@@ -1,14 +1,18 @@
 """The 4-bit key/value cache without a GPU: the book of pages against a plain model of sequences, the refusals of the
 C entry points (which check before they touch a device) and of the Python surface."""
 import ctypes as C
+import os
 import random
+import re
 
+import numpy as np
 import pytest
 import torch
 
 import mps_bitsandbytes_b200 as bnb
 from mps_bitsandbytes_b200 import _native as N
 from mps_bitsandbytes_b200.kv_cache import _PageBook
+from oracle import oracle_np as O
 
 
 class Book(_PageBook):
@@ -118,6 +122,25 @@ def test_a_fork_of_a_full_page_copies_nothing_and_a_shared_tail_is_copied_once_l
     book.extend([b, c, d], 1)                       # three on one tail: two copies
     assert book.num_pages - book.num_free_pages == used + 2
     assert len({book.pages(i)[1] for i in (b, c, d)}) == 3
+
+
+def test_the_scaled_codebook_rounds_better_than_nf4_itself():
+    """Rounding errors of the fp16 table over the codes of normal data, of which the kernel's comment speaks."""
+    src = open(os.path.join(os.path.dirname(N.LIB_PATH), "..", "csrc", "attn4.cuh")).read()
+    scale = float.fromhex(re.search(r"#define ATTN4_NF4_SCALE (\S+)f\b", src).group(1))
+    x = np.random.default_rng(0).standard_normal((20000, 64))
+    code = O.NF4_CODE.astype(np.float64)
+    idx = np.searchsorted((code[1:] + code[:-1]) / 2, x / np.abs(x).max(1, keepdims=True))
+    share = np.bincount(idx.ravel(), minlength=16) / idx.size
+
+    def errors(c):
+        table = (code.astype(np.float32) * np.float32(c)).astype(np.float16).astype(np.float64)
+        d = table / c - code
+        return np.sqrt((share * d * d).sum()), abs((share * d).sum())
+    plain, scaled = errors(1.0), errors(scale)
+    assert scaled[0] < 0.5 * plain[0] and scaled[1] < 0.25 * plain[1]
+    assert plain[0] == pytest.approx(7.3e-5, rel=0.02) and scaled[0] == pytest.approx(3.4e-5, rel=0.03)
+    assert np.array_equal(O.FP4_CODE.astype(np.float16).astype(np.float32), O.FP4_CODE)
 
 
 # ---------------------------------------------------------------------- C entry points
