@@ -486,8 +486,8 @@ int mpsbnb_kv4_copy_pages(const mpsbnb_kv4_cache *cache, const int32_t *src, con
  * keys at places max(0, p - window + 1) ... p when causal (window 0: no lower limit), all of the sequence otherwise
  * (window must then be 0).  A row that sees no key gives zeros and lse = -inf.  Rows past cu_seqlens[batch] are left
  * as they were.  A row that sees a page outside the cache gives NaN (device status 401).
- *   q    [tokens, heads, head_dim] in the cache's dtype, strides in elements, head_dim contiguous
- *   out  [tokens, heads, head_dim] contiguous, in the cache's dtype;  lse  NULL or fp32 [tokens, heads], natural log
+ *   q    [tokens, heads, head_dim] in the cache's dtype, strides in elements (multiples of 8), head_dim contiguous
+ *   out  [tokens, heads, head_dim] contiguous, in the cache's dtype; q and out 16-byte aligned;  lse  NULL or fp32 [tokens, heads], natural log
  * Scores, softmax statistics and sums are fp32; probabilities and codes enter the products as fp16.
  * workspace: mpsbnb_attention_4bit_workspace_bytes() bytes, 16-byte aligned, used by this call only while it runs. */
 size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads);

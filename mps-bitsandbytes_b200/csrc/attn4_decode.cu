@@ -19,7 +19,7 @@
 //    with the rounding of the 16 code values to fp16 only.
 //  * Softmax: probabilities are 2^(x - m) with a reference m that follows the running maximum only when a score
 //    exceeds it by 2^8: one vote per tile instead of a reduction, and fp32 sums lose nothing by it.  The weight
-//    p * absmax goes to fp16 under a power-of-two factor per row that is raised the same way (above 2^15).
+//    p * absmax goes to fp16; absmax is taken times a power of two that is lowered, in the same vote, when it exceeds 2^7.
 //    bf16 queries are brought to fp16 by a power of two per row: exact, but for parts below 2^-24 of the row's largest.
 #include <type_traits>
 
@@ -32,27 +32,36 @@ using namespace sm100;
 
 static __device__ int g_attn4_status = 0;
 
-constexpr int AD_WARPS = 8;
+constexpr int AD_WARPS = 8;                                          // of a team: the warps that share a run of tiles
 constexpr int AD_STAGES = 3;
+constexpr uint32_t AD_LUT = 65536;                                   // shared-window address of the table
+constexpr uint32_t AD_BASE = 1024;                                   // ... and of the dynamic shared memory
 
+// A block has one table (256 entries of 256 bytes, the lower 128 of which are in use: lane l's copy at 4 l) on a 64 KB
+// boundary, so that one byte permute makes a look-up's address.  It is too large for two blocks on an SM; instead a
+// block holds TEAMS teams of eight warps which do not wait on one another.
 template <int D, int BS, int NT> struct AdSmem {
+    static constexpr int TEAMS = D * NT <= 128 ? 2 : 1;              // by registers (accumulators and q): 128 or 255 a thread
+    static constexpr int THREADS = TEAMS * AD_WARPS * 32;
     static constexpr int GROUP = 2 * kv4_half_bytes(D, BS);
     static constexpr int RT = 8 * NT;
     static constexpr int RED_LD = 64 + 4;                            // floats per row of a merge pass
-    static constexpr int LUT = 0;
-    static constexpr int RING = 256 * 128;
-    static constexpr int RED = RING + AD_WARPS * AD_STAGES * GROUP;
-    static constexpr int STAT = RED + AD_WARPS * RT * RED_LD * 4;    // (maximum, sum) of every warp and row
-    static constexpr int BAR = STAT + AD_WARPS * RT * 8;
-    static constexpr int TOTAL = BAR + AD_WARPS * AD_STAGES * 8 + 16;
-    static constexpr int CTAS = D * NT <= 128 ? 2 : 1;               // per SM: by registers (accumulators and q)
-    static_assert(CTAS * (TOTAL + 1024) <= 228 * 1024, "shared memory of the decode kernel");
+    // window addresses: half of the warps' rings before the table, the other half and the rest behind it
+    static constexpr int RING_HALF = TEAMS * AD_WARPS / 2 * AD_STAGES * GROUP;
+    static constexpr uint32_t RING0 = AD_BASE, RING1 = AD_LUT + 65536;
+    static constexpr uint32_t RED = RING1 + RING_HALF;
+    static constexpr uint32_t STAT = RED + TEAMS * AD_WARPS * RT * RED_LD * 4;   // (maximum, sum) of every warp and row
+    static constexpr uint32_t BAR = STAT + TEAMS * AD_WARPS * RT * 8;
+    static constexpr uint32_t END = BAR + TEAMS * AD_WARPS * AD_STAGES * 8 + 16;
+    static constexpr int BYTES = END - AD_BASE;
+    static_assert(RING0 + RING_HALF <= AD_LUT && BYTES <= 227 * 1024, "shared memory of the decode kernel");
+    static_assert(RING_HALF % 128 == 0, "stages start on 16-byte boundaries");
 };
 
-__device__ __forceinline__ uint32_t ad_lut(uint32_t lut_lane, uint32_t word, int byte) {
-    const uint32_t off = byte == 0 ? (word << 7) : (word >> (8 * byte - 7));
+// value pair of byte `byte` of word; lut = AD_LUT + 4 lane, whose second byte is free
+__device__ __forceinline__ uint32_t ad_lut(uint32_t lut, uint32_t word, int byte) {
     uint32_t v;
-    asm("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(lut_lane + (off & 0x7F80u)));
+    asm("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(__byte_perm(word, lut, 0x7604 | (byte << 4))));
     return v;
 }
 __device__ __forceinline__ void ad_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -83,7 +92,7 @@ template <typename T, int NB> __device__ __forceinline__ void ad_scales(uint32_t
     }
 }
 
-// A walk over the pieces (runs of key tiles of one sequence, head and row tile) of a CTA's run of tiles.
+// A walk over the pieces (runs of key tiles of one sequence, head and row tile) of a team's run of tiles.
 struct AdPiece {
     Attn4Seq s;
     int b, h, r;                                 // sequence, kv head, row tile
@@ -140,52 +149,61 @@ struct AdPiece {
     }
 };
 
-// tiles per CTA: equal, and a multiple of the warps of a CTA
-__device__ __forceinline__ int64_t ad_per(int64_t total, int ctas) {
-    const int64_t per = (total + ctas - 1) / ctas;
+// tiles per team: equal, and a multiple of a team's warps
+__device__ __forceinline__ int64_t ad_per(int64_t total, int teams) {
+    const int64_t per = (total + teams - 1) / teams;
     return (per + AD_WARPS - 1) / AD_WARPS * AD_WARPS;
 }
-// partial result of CTA c, slot s (0: its first piece, 1: its last): RT x D sums, then RT (maximum, sum) pairs
+// partial result of team c, slot s (0: its first piece, 1: its last): RT x D sums, then RT (maximum, sum) pairs
 template <int D, int RT> __device__ __forceinline__ float *ad_partial(float *ws, int64_t c, int s) {
     return ws + (c * 2 + s) * (RT * (D + 2));
 }
 
 template <int D, int BS, int NT, typename T>
-__global__ void __launch_bounds__(AD_WARPS * 32, (AdSmem<D, BS, NT>::CTAS))
+__global__ void __launch_bounds__((AdSmem<D, BS, NT>::THREADS), 1)
 attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     using S = AdSmem<D, BS, NT>;
     constexpr int NB = D / BS, MT = D / 16, MB = BS / 16, RT = S::RT;   // MB: k steps, and channel tiles, per block
     constexpr int HALF = kv4_half_bytes(D, BS), SOFF = KV4_GROUP * (D / 2);
+    constexpr int WARPS = S::TEAMS * AD_WARPS;
     extern __shared__ __align__(128) unsigned char smem[];
-    const uint32_t sb = smem_u32(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + S::BAR + AD_WARPS * AD_STAGES * 8);
+    if (smem_u32(smem) != AD_BASE) {                                 // the layout counts on it
+        if (threadIdx.x == 0) atomicExch(&g_attn4_status, 403);
+        return;
+    }
+    const int cta_warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int in_team = cta_warp / AD_WARPS, warp = cta_warp % AD_WARPS;
+    const int team = blockIdx.x * S::TEAMS + in_team;
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + (S::END - 16 - AD_BASE));
 
-    // ------------------------------------------------------------ my run
+    // ------------------------------------------------------------ my team's run
     int64_t unused, total;
     attn4_prefix(A, RT, 0, unused, total);
-    const int64_t per = ad_per(total, gridDim.x);
-    const int64_t t0 = min(total, blockIdx.x * per), t1 = min(total, t0 + per);
+    const int64_t per = ad_per(total, gridDim.x * S::TEAMS);
+    const int64_t t0 = min(total, team * per), t1 = min(total, t0 + per);
     pdl_launch_dependents();
-    if (t0 >= t1) return;                                            // whole CTA
+    if (blockIdx.x * S::TEAMS * per >= total) return;                // nothing for any team of the block
 
     // ------------------------------------------------------------ table, barriers
     {
         const float mine = kCode[A.quant_type][lane & 15] * attn4_code_scale(A.quant_type);
-        for (int b = warp; b < 256; b += AD_WARPS) {
+        for (int b = cta_warp; b < 256; b += WARPS) {
             const float lo = __shfl_sync(0xffffffffu, mine, b & 15), hi = __shfl_sync(0xffffffffu, mine, b >> 4);
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(sb + (uint32_t)(S::LUT + b * 128 + lane * 4)), "r"(ad_half2(lo, hi)) : "memory");
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(AD_LUT + (uint32_t)(b * 256 + lane * 4)), "r"(ad_half2(lo, hi)) : "memory");
         }
         if (threadIdx.x == 0) {
-            for (int i = 0; i < AD_WARPS * AD_STAGES; ++i) mbar_init(sb + S::BAR + 8 * i, 1);
+            for (int i = 0; i < WARPS * AD_STAGES; ++i) mbar_init(S::BAR + 8 * i, 1);
             *abort_flag = 0;
             fence_mbar_init();
         }
     }
     __syncthreads();
-    const uint32_t lut = sb + S::LUT + lane * 4;
-    const uint32_t ring = sb + S::RING + warp * AD_STAGES * S::GROUP;
-    const uint32_t bars = sb + S::BAR + warp * AD_STAGES * 8;
+    if (t0 >= t1) return;                                            // whole team; no barrier of the block follows
+    auto team_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(in_team + 1), "n"(AD_WARPS * 32) : "memory"); };
+    const uint32_t lut = AD_LUT + lane * 4;
+    const uint32_t ring = cta_warp < WARPS / 2 ? S::RING0 + cta_warp * (AD_STAGES * S::GROUP) : S::RING1 + (cta_warp - WARPS / 2) * (AD_STAGES * S::GROUP);
+    const uint32_t bars = S::BAR + cta_warp * AD_STAGES * 8;
+    const bool negate = A.scale_log2 < 0.0f;                         // a negative scale goes into q: maxima stay maxima
 
     // ------------------------------------------------------------ producer side: this warp's tiles, in order
     AdPiece in;                                                      // piece the next copy belongs to
@@ -193,7 +211,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     AdPiece cur = in;
     bool in_more = true;
     int in_k = 0, in_page = 0;                                       // tile ordinal within the piece; pages of 32 ordinals
-    uint32_t put = 0;                                                // copies issued
+    uint32_t put = 0;                                                // next stage to fill
     auto issue = [&]() {                                             // whole warp
         while (in_more) {
             const int t = in.a + warp + in_k * AD_WARPS;
@@ -209,7 +227,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
         }
         const int page = __shfl_sync(0xffffffffu, in_page, in_k & 31);
         const int place = (in.s.tlo + in.a + warp + in_k * AD_WARPS) * 16;
-        const uint32_t st = put % AD_STAGES;
+        const uint32_t st = put;
         if (page >= 0 && page < A.kv.num_pages) {
             if (lane == 0) {
                 mbar_arrive_expect_tx(bars + 8 * st, S::GROUP);
@@ -222,14 +240,14 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
             __syncwarp();
             if (lane == 0) { atomicExch(&g_attn4_status, KV4_BAD_PAGE); mbar_arrive(bars + 8 * st); }
         }
-        ++put;
+        put = put == AD_STAGES - 1 ? 0 : put + 1;
         ++in_k;
     };
 #pragma unroll 1
     for (int i = 0; i < AD_STAGES; ++i) issue();
 
     // ------------------------------------------------------------ consumer side
-    uint32_t got = 0;                                                // stages consumed
+    uint32_t got = 0, phase = 0;                                     // next stage to read, its barrier's parity
     bool first_piece = true;
     do {
         const Attn4Seq &sq = cur.s;
@@ -247,8 +265,9 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
             for (int k = 0; k < NB * MB; ++k) {
                 raw[k] = make_uint2(0u, 0u);
                 if (ok) raw[k] = __ldg(reinterpret_cast<const uint2 *>(src + (k / MB) * BS + c * (BS / 4) + (k % MB) * 4));
+                if (negate) { raw[k].x ^= 0x80008000u; raw[k].y ^= 0x80008000u; }
             }
-            float fr = A.scale_log2 * attn4_code_unscale(A.quant_type);
+            float fr = fabsf(A.scale_log2) * attn4_code_unscale(A.quant_type);
             if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
                 uint32_t mx = 0;                                     // largest magnitude of the row, as bits of bf16
 #pragma unroll
@@ -269,6 +288,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
             }
 #pragma unroll
             for (int k = 0; k < NB * MB; ++k) { qf[nt][k][0] = raw[k].x; qf[nt][k][1] = raw[k].y; }
+            fr = fmaxf(fr, 0x1p-126f);                               // scale 0: -inf * f has to stay -inf
             f[nt][0] = __shfl_sync(0xffffffffu, fr, 8 * c);          // row 2c lives in lanes (2c, *)
             f[nt][1] = __shfl_sync(0xffffffffu, fr, 8 * c + 4);
         }
@@ -283,9 +303,11 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 low[nt][j] = A.window > 0 ? lim[nt][j] - A.window : 0;
             }
         const int i0 = (cur.r * RT) / A.group, i1 = min(sq.n - 1, (cur.r * RT + RT - 1) / A.group);
+        // places that some row sees: [any_lo, any_hi)
+        const int any_lo = A.window > 0 ? first + i0 + 1 - A.window : 0, any_hi = A.causal ? first + i1 + 1 : sq.len;
         const int full_lo = A.window > 0 ? first + i1 + 1 - A.window : 0, full_hi = A.causal ? first + i0 + 1 : sq.len;
 
-        float o[MT][NT][4], m[NT][2], l[NT][2], up[NT][2];           // up: 2^-(exponent of the weights' reference)
+        float o[MT][NT][4], m[NT][2], l[NT][2], up = 0x1p100f;       // up: power of two that the values' absmax is taken times
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -295,14 +317,14 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) { m[nt][j] = ATTN4_NONE; l[nt][j] = 0.0f; up[nt][j] = 0x1p100f; }
+            for (int j = 0; j < 2; ++j) { m[nt][j] = ATTN4_NONE; l[nt][j] = 0.0f; }
 
 #pragma unroll 1
         for (int t = cur.a + warp; t < cur.e; t += AD_WARPS) {
             const int place0 = (sq.tlo + t) * 16;
             if (place0 >= sq.len) break;                             // the dead tile of an empty sequence
-            const uint32_t st = got % AD_STAGES;
-            if (!mbar_wait(bars + 8 * st, (got / AD_STAGES) & 1u, abort_flag)) { atomicExch(&g_attn4_status, 402); *abort_flag = 1; }
+            const uint32_t st = got;
+            if (!mbar_wait(bars + 8 * st, phase, abort_flag)) { atomicExch(&g_attn4_status, 402); *abort_flag = 1; }
             const uint32_t kb = ring + st * S::GROUP, vb = kb + HALF;
             // A-operand row r of the tile is token r / 2 (even r) or r / 2 + 4 (odd r), + 8 for rows 8 .. 15: the k index
             // of P^T below then gives a lane the tokens c, c + 4, c + 8, c + 12
@@ -347,11 +369,13 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                     }
                 }
             }
+            float sv0[NB], sv1[NB], sm = 0.0f;
+            ad_scales<T, NB>(vb + SOFF + tok * NB * 2, sv0);
+            ad_scales<T, NB>(vb + SOFF + (tok + 8) * NB * 2, sv1);
             // s[nt][0..1]: token tok, columns 2c and 2c + 1; s[nt][2..3]: token tok + 8
             const bool masked = place0 < full_lo || place0 + 16 > full_hi;   // (full_hi <= len)
-            uint32_t seen = 0xffffffffu;                              // bit nt * 4 + j
+            uint32_t seen = 0;                                       // bit nt * 4 + j
             if (masked) {
-                seen = 0;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -360,93 +384,82 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                         if (place < lim[nt][j & 1] && place >= low[nt][j & 1]) seen |= 1u << (nt * 4 + j);
                         else s[nt][j] = __int_as_float(0xff800000);
                     }
+                // whatever lies in a place that no row sees
+                const bool in0 = place0 + tok >= any_lo && place0 + tok < any_hi, in1 = place0 + tok + 8 >= any_lo && place0 + tok + 8 < any_hi;
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) { sv0[blk] = in0 ? sv0[blk] : 0.0f; sv1[blk] = in1 ? sv1[blk] : 0.0f; }
             }
-            float p[NT][4];
-            bool above = false;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk) {
+                sv0[blk] *= up; sv1[blk] *= up;
+                sm = fmaxf(sm, fmaxf(sv0[blk], sv1[blk]));
+            }
+            float p[NT][4], top = -1.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    s[nt][j] *= f[nt][j & 1];
-                    p[nt][j] = s[nt][j] - m[nt][j & 1];
-                    above |= p[nt][j] > 8.0f;
+                    p[nt][j] = fmaf(s[nt][j], f[nt][j & 1], -m[nt][j & 1]);
+                    top = fmaxf(top, p[nt][j]);
                 }
-            // a negative scale turns the -inf of an unseen key round
-            if (masked) {
+            // p and absmax * up stay under 2^8 and 2^7, their product is at home in fp16
+            if (__any_sync(0xffffffffu, top > 8.0f || sm > 128.0f)) {
+                // (from the absmax itself: times `up` it may have left fp32)
+                ad_scales<T, NB>(vb + SOFF + tok * NB * 2, sv0);
+                ad_scales<T, NB>(vb + SOFF + (tok + 8) * NB * 2, sv1);
+                const bool in0 = place0 + tok >= any_lo && place0 + tok < any_hi, in1 = place0 + tok + 8 >= any_lo && place0 + tok + 8 < any_hi;
+                sm = 0.0f;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int blk = 0; blk < NB; ++blk) {
+                    sv0[blk] = in0 ? sv0[blk] : 0.0f; sv1[blk] = in1 ? sv1[blk] : 0.0f;
+                    sm = fmaxf(sm, fmaxf(sv0[blk], sv1[blk]));
+                }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (!(seen >> (nt * 4 + j) & 1u)) s[nt][j] = p[nt][j] = __int_as_float(0xff800000);
-                above = false;
+                for (int d = 1; d < 32; d <<= 1) sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, d));
+                float ku = 1.0f;
+                if (sm * up > 128.0f) {                              // the largest comes to [16, 32)
+                    const int e = max(5, (int)(__float_as_uint(fminf(sm, 3.4e38f)) >> 23));
+                    const float un = __int_as_float((258 - e) << 23);   // 2^(131 - e)
+                    ku = un * __frcp_rn(up);                         // (0 where the difference leaves fp32)
+                    up = un;
+                }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) above |= p[nt][j] > 8.0f;
-            }
-            if (__any_sync(0xffffffffu, above)) {
+                for (int blk = 0; blk < NB; ++blk) { sv0[blk] *= up; sv1[blk] *= up; }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float mx = fmaxf(s[nt][j], s[nt][j + 2]);
+                        float mx = fmaxf(s[nt][j], s[nt][j + 2]) * f[nt][j];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                        const float mn = fmaxf(m[nt][j], mx), k = ex2(m[nt][j] - mn);
+                        const float mn = mx > m[nt][j] + 8.0f ? mx : m[nt][j], k = ex2(m[nt][j] - mn);
                         m[nt][j] = mn;
                         l[nt][j] *= k;
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k; o[i][nt][j + 2] *= k; }
-                        p[nt][j] = s[nt][j] - mn;
-                        p[nt][j + 2] = s[nt][j + 2] - mn;
+                        for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k * ku; o[i][nt][j + 2] *= k * ku; }
+                        p[nt][j] = fmaf(s[nt][j], f[nt][j], -mn);
+                        p[nt][j + 2] = fmaf(s[nt][j + 2], f[nt][j], -mn);
                     }
             }
-            float sv0[NB], sv1[NB];
-            ad_scales<T, NB>(vb + SOFF + tok * NB * 2, sv0);
-            ad_scales<T, NB>(vb + SOFF + (tok + 8) * NB * 2, sv1);
             float wt[NB][NT][4];
-            bool large = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     p[nt][j] = ex2(p[nt][j]);
                     l[nt][j & 1] += p[nt][j];
-                    const float pu = p[nt][j] * up[nt][j & 1];
 #pragma unroll
-                    for (int blk = 0; blk < NB; ++blk) {
-                        float w = pu * (j < 2 ? sv0[blk] : sv1[blk]);
-                        if (masked && !(seen >> (nt * 4 + j) & 1u)) w = 0.0f;   // whatever lies in an unseen place
-                        wt[blk][nt][j] = w;
-                        large |= w > 32768.0f;
-                    }
+                    for (int blk = 0; blk < NB; ++blk) wt[blk][nt][j] = p[nt][j] * (j < 2 ? sv0[blk] : sv1[blk]);
                 }
-            if (__any_sync(0xffffffffu, large)) {
+            if (masked) {                                            // a value that is not finite is no matter of rows that do not see it
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        // the largest weight, without the present factor (which may have taken it past fp32)
-                        float mx = 0.0f;
+                    for (int j = 0; j < 4; ++j)
+                        if (!(seen >> (nt * 4 + j) & 1u)) {
 #pragma unroll
-                        for (int blk = 0; blk < NB; ++blk) {
-                            if (!masked || (seen >> (nt * 4 + j) & 1u)) mx = fmaxf(mx, p[nt][j] * sv0[blk]);
-                            if (!masked || (seen >> (nt * 4 + j + 2) & 1u)) mx = fmaxf(mx, p[nt][j + 2] * sv1[blk]);
+                            for (int blk = 0; blk < NB; ++blk) wt[blk][nt][j] = 0.0f;
                         }
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                        const int e = max(4, min(253, (int)(__float_as_uint(mx) >> 23)));
-                        const float un = fminf(up[nt][j], __int_as_float((257 - e) << 23));   // the largest comes to [8, 16)
-                        const float k = un * __frcp_rn(up[nt][j]);    // powers of two: exact
-                        up[nt][j] = un;
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k; o[i][nt][j + 2] *= k; }
-#pragma unroll
-                        for (int blk = 0; blk < NB; ++blk) {
-                            wt[blk][nt][j] = !masked || (seen >> (nt * 4 + j) & 1u) ? p[nt][j] * un * sv0[blk] : 0.0f;
-                            wt[blk][nt][j + 2] = !masked || (seen >> (nt * 4 + j + 2) & 1u) ? p[nt][j + 2] * un * sv1[blk] : 0.0f;
-                        }
-                    }
             }
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk) {
@@ -473,14 +486,14 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                     for (int nt = 0; nt < NT; ++nt) ad_mma(o[blk * MB + j][nt], a0, a1, a2, a3, b0[nt], b1[nt]);
                 }
             }
-            ++got;
+            if (++got == AD_STAGES) { got = 0; phase ^= 1; }
             __syncwarp();                                            // every lane has read the stage
             issue();
         }
 
         // ------------------------------------------------------------ join the warps
-        float *red = reinterpret_cast<float *>(smem + S::RED);
-        float2 *stat = reinterpret_cast<float2 *>(smem + S::STAT);
+        float *red = reinterpret_cast<float *>(smem + (S::RED - AD_BASE)) + in_team * (AD_WARPS * RT * S::RED_LD);
+        float2 *stat = reinterpret_cast<float2 *>(smem + (S::STAT - AD_BASE)) + in_team * (AD_WARPS * RT);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -489,7 +502,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 for (int d = 4; d < 32; d <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
                 if (g == 0) stat[warp * RT + nt * 8 + 2 * c + j] = make_float2(m[nt][j], l[nt][j]);
             }
-        __syncthreads();
+        team_sync();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -497,12 +510,12 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 float M = m[nt][j];
 #pragma unroll
                 for (int w = 0; w < AD_WARPS; ++w) M = fmaxf(M, stat[w * RT + nt * 8 + 2 * c + j].x);
-                const float k = ex2(m[nt][j] - M) * __frcp_rn(up[nt][j]) * attn4_code_unscale(A.quant_type);
+                const float k = ex2(m[nt][j] - M) * __frcp_rn(up) * attn4_code_unscale(A.quant_type);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k; o[i][nt][j + 2] *= k; }
             }
         const bool whole = cur.a == 0 && cur.e == sq.nt;
-        float *part = ad_partial<D, RT>(A.ws, blockIdx.x, first_piece ? 0 : 1);
+        float *part = ad_partial<D, RT>(A.ws, team, first_piece ? 0 : 1);
 #pragma unroll
         for (int d0 = 0; d0 < D; d0 += 64) {                         // 64 channels per pass
 #pragma unroll
@@ -515,8 +528,8 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                     for (int j = 0; j < 2; ++j)
                         *reinterpret_cast<float2 *>(red + (warp * RT + nt * 8 + 2 * c + j) * S::RED_LD + d) = make_float2(o[mt][nt][j], o[mt][nt][j + 2]);
             }
-            __syncthreads();
-            for (int x = threadIdx.x; x < RT * 32; x += AD_WARPS * 32) {
+            team_sync();
+            for (int x = warp * 32 + lane; x < RT * 32; x += AD_WARPS * 32) {
                 const int row = x >> 5, d = 2 * (x & 31);
                 const int R = cur.r * RT + row, i = R / A.group;
                 if (i < sq.n) {
@@ -542,7 +555,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                     }
                 }
             }
-            __syncthreads();                                         // red (and, at the end, stat) may be written again
+            team_sync();                                         // red (and, at the end, stat) may be written again
         }
         first_piece = false;
     } while (cur.next(A, RT));
@@ -551,7 +564,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
 // Joins the partial results of one (sequence, head, row tile, row): sum of 2^(m_i - M) O_i over sum of 2^(m_i - M) l_i.
 template <int D, int RT, typename T>
 __global__ void __launch_bounds__(256)
-attn4_combine_kernel(const __grid_constant__ Attn4Args A, int ctas, int rts_max) {
+attn4_combine_kernel(const __grid_constant__ Attn4Args A, int teams, int rts_max) {
     __shared__ float red[8][D];
     __shared__ float reds[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -567,9 +580,9 @@ attn4_combine_kernel(const __grid_constant__ Attn4Args A, int ctas, int rts_max)
     // every block waits, so that this kernel's end means the end of the one before it as well
     pdl_grid_dependency_wait();
     if (r >= s.rts || i >= s.n) return;                              // whole block
-    const int64_t per = ad_per(total, ctas);
+    const int64_t per = ad_per(total, teams);
     const int64_t t0 = before + (int64_t)(h * s.rts + r) * s.nt, c0 = t0 / per, c1 = (t0 + s.nt - 1) / per;
-    if (c0 == c1) return;                                            // one CTA had it all and has written it
+    if (c0 == c1) return;                                            // one team had it all and has written it
     float M = ATTN4_NONE;
     for (int64_t ci = c0 + lane; ci <= c1; ci += 32)
         M = fmaxf(M, ad_partial<D, RT>(A.ws, ci, t0 <= ci * per ? 0 : 1)[RT * D + 2 * row]);
@@ -610,7 +623,7 @@ attn4_combine_kernel(const __grid_constant__ Attn4Args A, int ctas, int rts_max)
 // 16 rows per tile where 8 do not hold a sequence's rows: the keys are then expanded half as often
 static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return (int64_t)s->new_tokens * group > 8 ? 2 : 1; }
 
-static int ad_ctas(int D, int NT) { return sm_count() * (D * NT <= 128 ? 2 : 1); }
+static int ad_teams(int D, int NT) { return sm_count() * (D * NT <= 128 ? 2 : 1); }
 
 template <int D, int BS, int NT, typename T>
 static int ad_launch(const Attn4Args &a, int rts_max, cudaStream_t st) {
@@ -619,11 +632,11 @@ static int ad_launch(const Attn4Args &a, int rts_max, cudaStream_t st) {
     int dev = 0;
     MPSBNB_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        MPSBNB_CUDA_TRY(cudaFuncSetAttribute(attn4_decode_kernel<D, BS, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
+        MPSBNB_CUDA_TRY(cudaFuncSetAttribute(attn4_decode_kernel<D, BS, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const int ctas = ad_ctas(D, NT);
-    attn4_decode_kernel<D, BS, NT, T><<<ctas, AD_WARPS * 32, S::TOTAL, st>>>(a);
+    const int teams = ad_teams(D, NT);
+    attn4_decode_kernel<D, BS, NT, T><<<teams / S::TEAMS, S::THREADS, S::BYTES, st>>>(a);
     int rc = check_launch();
     if (rc != MPSBNB_OK) return rc;
     const int64_t blocks = (int64_t)a.sq.batch * a.kv.kv_heads * rts_max * S::RT;
@@ -637,7 +650,7 @@ static int ad_launch(const Attn4Args &a, int rts_max, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    MPSBNB_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_combine_kernel<D, S::RT, T>, a, ctas, rts_max));
+    MPSBNB_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_combine_kernel<D, S::RT, T>, a, teams, rts_max));
     return check_launch();
 }
 
@@ -664,7 +677,7 @@ extern "C" size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *
     if (kv4_check_cache(cache, 0) != MPSBNB_OK || kv4_check_seqs(seqs, cache) != MPSBNB_OK) return 0;
     if (heads <= 0 || heads % cache->kv_heads != 0 || seqs->batch == 0 || seqs->tokens == 0) return 0;
     const int nt = ad_nt(seqs, heads / cache->kv_heads);
-    return (size_t)ad_ctas(cache->head_dim, nt) * 2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float);
+    return (size_t)ad_teams(cache->head_dim, nt) * 2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
@@ -681,7 +694,7 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     if ((int64_t)seqs->new_tokens * group > 0x3fffffffll) return MPSBNB_ERR_TOO_LARGE;
     if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < mpsbnb_attention_4bit_workspace_bytes(cache, seqs, heads)) return MPSBNB_ERR_WORKSPACE;
     // rows are fetched in 16-byte pieces
-    if (!aligned16(q) || ((q_token_stride | q_head_stride) & 7) != 0 || (reinterpret_cast<uintptr_t>(out) & 3) != 0) return MPSBNB_ERR_UNSUPPORTED;
+    if (!aligned16(q) || ((q_token_stride | q_head_stride) & 7) != 0 || !aligned16(out)) return MPSBNB_ERR_UNSUPPORTED;
     Attn4Args a;
     a.kv = kv4_layer(cache, layer);
     a.sq = kv4_seqs(seqs, cache);

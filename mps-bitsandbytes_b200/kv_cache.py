@@ -361,8 +361,8 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
     sq = _seqs(cache, page_table, seq_lens, cu_seqlens, qr.shape[0], max_seqlen)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if cu_seqlens is None else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}")
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() & 15:
+        raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}, 16-byte aligned")
     lse = None
     if return_lse:
         lse = torch.full(q.shape[:-1], float("-inf"), dtype=torch.float32, device=q.device)

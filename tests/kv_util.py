@@ -47,9 +47,9 @@ def attention(q, cache, layer, table, lens, starts, causal=True, window=None, sc
     tile's largest).  A bf16 query is exact but for parts under 2^-14 of its row's largest, off by 2^-25 of that.  So a score is off by
     e = scale (2 * 2^-11 sum_d |q_d k_d| + 2^-25 max|q| sum_d |k_d| + 2^-33 max|k| sum_d |q_d|) and a probability by a factor within
     exp(+-2 e_max) (numerator and denominator).  A weight p * absmax, or p, is rounded to fp16: by 2^-11 of itself, or, being
-    small, by 2^-25 under a reference that is at least 8 for the largest weight (single tokens) or 2^7 for the largest p (prompts,
-    where V's own 2^-33 adds as much again at most).  fp32 sums of n terms add 2^-24 each step at most: n * 2^-23 covers numerator
-    and denominator, and 2^-18 the scores' sums and the last bits of the exponential.
+    small, by 2^-25 under factors that bring the largest absmax to 16 at least and the largest p to 1 (single tokens: 2^-29 of
+    their product) or the largest p to 2^7 (prompts: 2^-32, and as much again for V's own 2^-33).  fp32 sums of n terms add 2^-24
+    each step at most: n * 2^-23 covers numerator and denominator, and 2^-18 the scores' sums and the last bits of the exponential.
     """
     T, H, D = q.shape
     group = H // cache.num_kv_heads
@@ -84,8 +84,7 @@ def attention(q, cache, layer, table, lens, starts, causal=True, window=None, sc
                                 + kk.abs().max() * x.abs().sum(-1, keepdim=True) * 2.0 ** -33)
             err = err.masked_fill(~seen, 0.0).amax(-1, keepdim=True)
             rel = torch.expm1(2 * err) + 3 * 2.0 ** -11 + length * 2.0 ** -23 + 2.0 ** -18
-            size = vv.abs().amax(-1)                                 # per key
-            small = 2.0 ** -28 * (p * size).amax(-1, keepdim=True) + 2 * 2.0 ** -32 * p.amax(-1, keepdim=True) * size.max()
+            small = 2.0 ** -29 * p.amax(-1, keepdim=True) * vv.abs().max()
             bound[a:e, h] = (p @ vv.abs()) * rel + length * small
     return out, lse, bound
 

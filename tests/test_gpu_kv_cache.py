@@ -220,6 +220,27 @@ def test_attention(case):
     assert_device_ok()
 
 
+@pytest.mark.parametrize("head_dim,heads,kv_heads", [(64, 8, 2), (128, 8, 1), (256, 4, 2)])
+def test_many_sequences_of_all_kinds(head_dim, heads, kv_heads):
+    """More blocks of rows than there are SMs, in an order that mixes sequences with one and with two row tiles, without new tokens,
+    without keys, and shorter than their new tokens."""
+    import random
+    import kv_util as U
+    rng = random.Random(head_dim)
+    news = [rng.choice([0, 1, 5, 16, 30, 31, 40, 64, 70, 100, 129]) for _ in range(180)]
+    lens = [rng.choice([0, n // 2, n, n, n + rng.randint(0, 60), rng.randint(0, 160)]) for n in news]
+    starts = _starts(news)
+    cache = U.make_cache(180 * 6, kv_heads, head_dim, 32, seed=6)
+    table = U.random_table(180, 6, 180 * 6)
+    q = torch.randn(starts[-1], heads, head_dim, device="cuda", dtype=F16)
+    for window in (None, 23):
+        want, want_lse, bound = U.attention(q, cache, 0, table, lens, starts, window=window)
+        got, lse = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), 129, window=window, return_lse=True)
+        U.check(got, want, bound, F16)
+        assert torch.equal(torch.isinf(lse), torch.isinf(want_lse))
+    assert_device_ok()
+
+
 @pytest.mark.parametrize("heads,new", [(8, 6), (8, 200)])
 def test_rows_without_keys_are_zero_and_rows_past_the_last_sequence_stay(heads, new):
     import kv_util as U
