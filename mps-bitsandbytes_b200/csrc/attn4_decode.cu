@@ -4,12 +4,12 @@
 // Bound: HBM, for the cached bytes (head_dim / 2 + 2 head_dim / blocksize per token, head and side) are read once and
 // the arithmetic per byte is small; what stands in the way is turning 4-bit codes into operands at that rate.
 //
-//  * Work is a list of (sequence, kv head, row tile, 16-token key tile), cut into equal runs of tiles, one per CTA,
+//  * Work is a list of (sequence, kv head, row tile, key tile), cut into equal runs, one per team of four warps,
 //    whatever the sequences' lengths are: the lengths are read on the device, so a captured graph follows them.
 //    A run that begins or ends inside a (sequence, head, row tile) leaves a partial result in the workspace, and
 //    attn4_combine_kernel joins the partials.
-//  * A key tile is one group of the cache: one bulk copy into the warp's own ring of stages.  No barrier between warps
-//    while tiles stream; a warp waits on its own mbarriers only.
+//  * A key tile is one or two groups of the cache: a bulk copy each into the warp's own ring of stages.  No barrier between
+//    warps while tiles stream; a warp waits on its own mbarriers only.
 //  * S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16: tokens (then channels) are the 16 rows and the query rows
 //    the 8 columns, so a group of up to 8 heads wastes nothing of the tile.  (tcgen05 would want 128 rows and the
 //    operands in shared memory: here they are made in registers.)  Codes become fp16 pairs by a 256-entry table
@@ -32,30 +32,36 @@ using namespace sm100;
 
 static __device__ int g_attn4_status = 0;
 
-constexpr int AD_WARPS = 8;                                          // of a team: the warps that share a run of tiles
-constexpr int AD_STAGES = 3;
+constexpr int AD_WARPS = 4;                                          // of a team: the warps that share a run of tiles
+// What a (sequence, head, row tile) counts besides its tokens, in tokens: q, the joining of the warps
+constexpr int AD_COST_TOKENS = 256;
 constexpr uint32_t AD_LUT = 65536;                                   // shared-window address of the table
 constexpr uint32_t AD_BASE = 1024;                                   // ... and of the dynamic shared memory
 
 // A block has one table (256 entries of 256 bytes, the lower 128 of which are in use: lane l's copy at 4 l) on a 64 KB
 // boundary, so that one byte permute makes a look-up's address.  It is too large for two blocks on an SM; instead a
-// block holds TEAMS teams of eight warps which do not wait on one another.
+// block holds TEAMS teams of four warps which do not wait on one another.
 template <int D, int BS, int NT> struct AdSmem {
-    static constexpr int TEAMS = D * NT <= 128 ? 2 : 1;              // by registers (accumulators and q): 128 or 255 a thread
-    static constexpr int THREADS = TEAMS * AD_WARPS * 32;
+    static constexpr int WARPS = D * NT <= 128 ? 12 : 8, THREADS = WARPS * 32;   // 168 or 255 registers a thread
+    static constexpr int TEAMS = WARPS / AD_WARPS;
     static constexpr int GROUP = 2 * kv4_half_bytes(D, BS);
+    static constexpr int G = D == 256 ? 1 : 2;                       // groups of 16 tokens per tile
+    static constexpr int TOK = 16 * G;                               // tokens per tile
+    static constexpr int STAGE = G * GROUP, STAGES = D == 128 ? 2 : 3;   // of a warp's ring
+    static constexpr int COST = AD_COST_TOKENS / TOK;
     static constexpr int RT = 8 * NT;
-    static constexpr int RED_LD = 64 + 4;                            // floats per row of a merge pass
-    // window addresses: half of the warps' rings before the table, the other half and the rest behind it
-    static constexpr int RING_HALF = TEAMS * AD_WARPS / 2 * AD_STAGES * GROUP;
+    static constexpr int RED_D = D == 256 ? 64 : D, RED_LD = RED_D + 2;   // channels, floats per row of a merge pass
+    // window addresses: the rings of as many warps as fit before the table, the others and the rest behind it
+    static constexpr int FIT = (AD_LUT - AD_BASE) / (STAGES * STAGE);
+    static constexpr int WARPS0 = FIT < WARPS ? FIT : WARPS;
     static constexpr uint32_t RING0 = AD_BASE, RING1 = AD_LUT + 65536;
-    static constexpr uint32_t RED = RING1 + RING_HALF;
-    static constexpr uint32_t STAT = RED + TEAMS * AD_WARPS * RT * RED_LD * 4;   // (maximum, sum) of every warp and row
-    static constexpr uint32_t BAR = STAT + TEAMS * AD_WARPS * RT * 8;
-    static constexpr uint32_t END = BAR + TEAMS * AD_WARPS * AD_STAGES * 8 + 16;
+    static constexpr uint32_t RED = RING1 + (WARPS - WARPS0) * STAGES * STAGE;
+    static constexpr uint32_t STAT = RED + WARPS * RT * RED_LD * 4;  // (maximum, sum) of every warp and row
+    static constexpr uint32_t BAR = STAT + WARPS * RT * 8;
+    static constexpr uint32_t END = BAR + WARPS * STAGES * 8 + 16;
     static constexpr int BYTES = END - AD_BASE;
-    static_assert(RING0 + RING_HALF <= AD_LUT && BYTES <= 227 * 1024, "shared memory of the decode kernel");
-    static_assert(RING_HALF % 128 == 0, "stages start on 16-byte boundaries");
+    static_assert(BYTES <= 227 * 1024, "shared memory of the decode kernel");
+    static_assert(GROUP % 16 == 0, "bulk copies go by 16 bytes");
 };
 
 // value pair of byte `byte` of word; lut = AD_LUT + 4 lane, whose second byte is free
@@ -71,20 +77,21 @@ __device__ __forceinline__ void ad_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 }
 __device__ __forceinline__ uint32_t ad_transpose(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ uint32_t ad_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// NB consecutive 16-bit absmax values as floats
+// NB consecutive 16-bit absmax values as floats.  This and the loads of codes are volatile, which keeps them between the waits
+// and releases of their stage, but clobber nothing: the look-ups may be scheduled around them.
 template <typename T, int NB> __device__ __forceinline__ void ad_scales(uint32_t addr, float (&s)[NB]) {
     uint32_t w[(NB + 1) / 2];
-    if constexpr (NB == 1) { uint16_t h; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr) : "memory"); w[0] = h; }
-    else if constexpr (NB == 2) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
-    else if constexpr (NB == 4) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
-    else asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+    if constexpr (NB == 1) { uint16_t h; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr)); w[0] = h; }
+    else if constexpr (NB == 2) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+    else if constexpr (NB == 4) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+    else asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
         const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
@@ -92,21 +99,47 @@ template <typename T, int NB> __device__ __forceinline__ void ad_scales(uint32_t
     }
 }
 
-// A walk over the pieces (runs of key tiles of one sequence, head and row tile) of a team's run of tiles.
-struct AdPiece {
-    Attn4Seq s;
+// A sequence as this kernel walks it: rows = (new token, head of the group) pairs in tiles of RT rows, keys in tiles of TOK places.
+struct AdSeq {
+    int row0, n, len;                            // first row of q, new tokens, places
+    int tlo, nt;                                 // first key tile and number of key tiles (one dead tile if there is no key)
+    int rts;                                     // row tiles
+    template <class S> __device__ __forceinline__ void get(const Attn4Args &a, int b) {
+        a.sq.get(b, row0, n, len);
+        const int low = a.window > 0 ? max(0, len - n - a.window + 1) : 0;
+        tlo = low / S::TOK;
+        nt = n > 0 ? max((len + S::TOK - 1) / S::TOK - tlo, 1) : 0;
+        rts = (n * a.group + S::RT - 1) / S::RT;
+    }
+    // units of work: key tiles, and COST more for each (head, row tile)
+    template <class S> __device__ __forceinline__ int64_t units(const Attn4Args &a) const { return nt > 0 ? (int64_t)(nt + S::COST) * rts * a.kv.kv_heads : 0; }
+};
+template <class S> __device__ __forceinline__ int64_t ad_units(const Attn4Args &a, int b) {
+    if (b >= a.sq.batch) return 0;
+    AdSeq s;
+    s.get<S>(a, b);
+    return s.units<S>(a);
+}
+// n / d for n >= 0, d > 0, in 32 bits where they do
+__device__ __forceinline__ int64_t ad_div(int64_t n, int64_t d) {
+    return n < 0x7fffffffll && d < 0x7fffffffll ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
+}
+
+// A walk over the pieces (runs of key tiles of one sequence, head and row tile) of a team's run.  Runs are cut in units: a
+// (sequence, head, row tile) counts COST units at its beginning and then its key tiles.
+template <class S> struct AdPiece {
+    AdSeq s;
     int b, h, r;                                 // sequence, kv head, row tile
     int a, e;                                    // key tiles of the piece, relative to s.tlo
-    int64_t left;                                // tiles of the run after this piece
+    int64_t left;                                // units of the run after this piece
 
-    // first piece of the run [t0, t1) of the whole list; whole warp
-    __device__ __forceinline__ void start(const Attn4Args &A, int rt, int64_t t0, int64_t t1) {
+    // first piece of the run [t0, t1) of the whole list (false: the run holds none of its tiles); whole warp.
+    // w: units of sequence `lane`
+    __device__ __forceinline__ bool start(const Attn4Args &A, int64_t w, int64_t t0, int64_t t1) {
         const int lane = threadIdx.x & 31;
         int64_t base = 0;
         for (int b0 = 0;; b0 += 32) {
-            Attn4Seq q;
-            int64_t w = 0;
-            if (b0 + lane < A.sq.batch) { q.get(A, b0 + lane, rt); w = q.work(A.kv.kv_heads); }
+            if (b0 > 0) w = ad_units<S>(A, b0 + lane);
             int64_t inc = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -122,50 +155,62 @@ struct AdPiece {
             }
             base += __shfl_sync(0xffffffffu, inc, 31);
         }
-        s.get(A, b, rt);
+        s.get<S>(A, b);
         const int64_t off = t0 - base;
-        const int sub = (int)(off / s.nt);
+        const int units = s.nt + S::COST, sub = (int)ad_div(off, units);
         h = sub / s.rts;
         r = sub - h * s.rts;
-        a = (int)(off - (int64_t)sub * s.nt);
         left = t1 - t0;
-        e = (int)min((int64_t)s.nt, a + left);
-        left -= e - a;
+        take((int)(off - (int64_t)sub * units));
+        return e > 0 || next(A);
+    }
+    // the piece that begins `from` units into its (sequence, head, row tile)
+    __device__ __forceinline__ void take(int from) {
+        const int to = (int)min((int64_t)(s.nt + S::COST), from + left);
+        left -= to - from;
+        a = max(0, from - S::COST);
+        e = max(0, to - S::COST);
     }
     // next piece; false when the run is done
-    __device__ __forceinline__ bool next(const Attn4Args &A, int rt) {
-        if (left == 0) return false;
-        if (++r == s.rts) {
-            r = 0;
-            if (++h == A.kv.kv_heads) {
-                h = 0;
-                do { ++b; s.get(A, b, rt); } while (s.nt == 0);
+    __device__ __forceinline__ bool next(const Attn4Args &A) {
+        do {
+            if (left == 0) return false;
+            if (++r == s.rts) {
+                r = 0;
+                if (++h == A.kv.kv_heads) {
+                    h = 0;
+                    do { ++b; s.get<S>(A, b); } while (s.nt == 0);
+                }
             }
-        }
-        a = 0;
-        e = (int)min((int64_t)s.nt, left);
-        left -= e;
+            take(0);
+        } while (e == 0);
         return true;
     }
 };
 
-// tiles per team: equal, and a multiple of a team's warps
-__device__ __forceinline__ int64_t ad_per(int64_t total, int teams) {
-    const int64_t per = (total + teams - 1) / teams;
-    return (per + AD_WARPS - 1) / AD_WARPS * AD_WARPS;
-}
+// units per team: equal, and a few tiles for each of a team's warps
+__device__ __forceinline__ int64_t ad_per(int64_t total, int teams) { return max(ad_div(total + teams - 1, teams), (int64_t)(4 * AD_WARPS)); }
+
 // partial result of team c, slot s (0: its first piece, 1: its last): RT x D sums, then RT (maximum, sum) pairs
 template <int D, int RT> __device__ __forceinline__ float *ad_partial(float *ws, int64_t c, int s) {
     return ws + (c * 2 + s) * (RT * (D + 2));
+}
+// behind the partials: what the team's last piece wants joined, if more teams share its (sequence, head, row tile)
+struct AdJoin {
+    int n, slot;                                 // parts, in the teams from this one on (0: nothing to join); the first's slot
+    int row0, rows, r, h;                        // the sequence's first row and number of (token, head) rows; row tile, kv head
+};
+template <int D, int RT> __device__ __forceinline__ AdJoin *ad_join(float *ws, int teams) {
+    return reinterpret_cast<AdJoin *>(ws + (int64_t)teams * 2 * RT * (D + 2));
 }
 
 template <int D, int BS, int NT, typename T>
 __global__ void __launch_bounds__((AdSmem<D, BS, NT>::THREADS), 1)
 attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     using S = AdSmem<D, BS, NT>;
-    constexpr int NB = D / BS, MT = D / 16, MB = BS / 16, RT = S::RT;   // MB: k steps, and channel tiles, per block
+    using Piece = AdPiece<S>;
+    constexpr int NB = D / BS, MT = D / 16, MB = BS / 16, RT = S::RT, G = S::G;   // MB: k steps, and channel tiles, per block
     constexpr int HALF = kv4_half_bytes(D, BS), SOFF = KV4_GROUP * (D / 2);
-    constexpr int WARPS = S::TEAMS * AD_WARPS;
     extern __shared__ __align__(128) unsigned char smem[];
     if (smem_u32(smem) != AD_BASE) {                                 // the layout counts on it
         if (threadIdx.x == 0) atomicExch(&g_attn4_status, 403);
@@ -173,84 +218,106 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     }
     const int cta_warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int in_team = cta_warp / AD_WARPS, warp = cta_warp % AD_WARPS;
-    const int team = blockIdx.x * S::TEAMS + in_team;
+    const int teams = gridDim.x * S::TEAMS, team = blockIdx.x * S::TEAMS + in_team;
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + (S::END - 16 - AD_BASE));
-
-    // ------------------------------------------------------------ my team's run
-    int64_t unused, total;
-    attn4_prefix(A, RT, 0, unused, total);
-    const int64_t per = ad_per(total, gridDim.x * S::TEAMS);
-    const int64_t t0 = min(total, team * per), t1 = min(total, t0 + per);
+    int64_t units = ad_units<S>(A, lane);                            // (its loads are under way while the table is made)
     pdl_launch_dependents();
-    if (blockIdx.x * S::TEAMS * per >= total) return;                // nothing for any team of the block
 
     // ------------------------------------------------------------ table, barriers
     {
-        const float mine = kCode[A.quant_type][lane & 15] * attn4_code_scale(A.quant_type);
-        for (int b = cta_warp; b < 256; b += WARPS) {
+        const float mine = A.code[lane & 15];
+        for (int b = cta_warp; b < 256; b += S::WARPS) {
             const float lo = __shfl_sync(0xffffffffu, mine, b & 15), hi = __shfl_sync(0xffffffffu, mine, b >> 4);
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(AD_LUT + (uint32_t)(b * 256 + lane * 4)), "r"(ad_half2(lo, hi)) : "memory");
         }
-        if (threadIdx.x == 0) {
-            for (int i = 0; i < WARPS * AD_STAGES; ++i) mbar_init(S::BAR + 8 * i, 1);
-            *abort_flag = 0;
-            fence_mbar_init();
-        }
+        if (threadIdx.x < S::WARPS * S::STAGES) mbar_init(S::BAR + 8 * threadIdx.x, G);
+        if (threadIdx.x == 0) *abort_flag = 0;
+        fence_mbar_init();
     }
     __syncthreads();
-    if (t0 >= t1) return;                                            // whole team; no barrier of the block follows
+
+    // ------------------------------------------------------------ my team's run
+    int64_t total = units;
+    for (int b = 32 + lane; b < A.sq.batch; b += 32) total += ad_units<S>(A, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int64_t per = ad_per(total, teams), t0 = min(total, team * per), t1 = min(total, t0 + per);
+    // what the teams leave for attn4_combine_kernel (a team's thread 0 writes both)
+    AdJoin *join = ad_join<D, RT>(A.ws, teams) + team;
+    if (warp == 0 && lane == 0) join->n = 0;
+    Piece in;                                                        // piece the next copy belongs to
+    if (t0 >= t1 || !in.start(A, units, t0, t1)) return;             // whole team; no barrier of the block follows
+    Piece cur = in;                                                  // piece being worked on
     auto team_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(in_team + 1), "n"(AD_WARPS * 32) : "memory"); };
     const uint32_t lut = AD_LUT + lane * 4;
-    const uint32_t ring = cta_warp < WARPS / 2 ? S::RING0 + cta_warp * (AD_STAGES * S::GROUP) : S::RING1 + (cta_warp - WARPS / 2) * (AD_STAGES * S::GROUP);
-    const uint32_t bars = S::BAR + cta_warp * AD_STAGES * 8;
+    const uint32_t ring = cta_warp < S::WARPS0 ? S::RING0 + cta_warp * (S::STAGES * S::STAGE) : S::RING1 + (cta_warp - S::WARPS0) * (S::STAGES * S::STAGE);
+    const uint32_t bars = S::BAR + cta_warp * S::STAGES * 8;
     const bool negate = A.scale_log2 < 0.0f;                         // a negative scale goes into q: maxima stay maxima
 
     // ------------------------------------------------------------ producer side: this warp's tiles, in order
-    AdPiece in;                                                      // piece the next copy belongs to
-    in.start(A, RT, t0, t1);
-    AdPiece cur = in;
-    bool in_more = true;
-    int in_k = 0, in_page = 0;                                       // tile ordinal within the piece; pages of 32 ordinals
+    // tiles of a piece that this warp takes (every fourth; none of an empty sequence's dead tile)
+    auto tiles_of = [&](const Piece &p) {
+        const int end = min(p.e, (p.s.len + S::TOK - 1) / S::TOK - p.s.tlo);
+        return max(0, (end - p.a - warp + AD_WARPS - 1) / AD_WARPS);
+    };
+    constexpr int BATCH = 32 / G;                                    // tiles whose addresses the lanes hold, a group each
+    int in_k = 0, in_n = tiles_of(in);                               // next of how many
+    uint64_t in_addr = 0;                                            // where my group lies; 0: nowhere
+    uint32_t in_bad = 0;                                             // lanes whose group is in a page outside the cache
     uint32_t put = 0;                                                // next stage to fill
+    bool in_more = true;
     auto issue = [&]() {                                             // whole warp
-        while (in_more) {
-            const int t = in.a + warp + in_k * AD_WARPS;
-            if (t < in.e && (in.s.tlo + t) * 16 < in.s.len) break;
-            in_more = in.next(A, RT);
+        while (in_k == in_n) {
+            if (!in_more) return;
+            in_more = in.next(A);
             in_k = 0;
+            in_n = in_more ? tiles_of(in) : 0;
         }
-        if (!in_more) return;
-        if ((in_k & 31) == 0) {
-            const int t = in.a + warp + (in_k + lane) * AD_WARPS;
-            in_page = -1;
-            if (t < in.e) in_page = __ldg(A.sq.table + (int64_t)in.b * A.sq.table_ld + (((in.s.tlo + t) * 16) >> A.kv.page_shift));
-        }
-        const int page = __shfl_sync(0xffffffffu, in_page, in_k & 31);
-        const int place = (in.s.tlo + in.a + warp + in_k * AD_WARPS) * 16;
-        const uint32_t st = put;
-        if (page >= 0 && page < A.kv.num_pages) {
-            if (lane == 0) {
-                mbar_arrive_expect_tx(bars + 8 * st, S::GROUP);
-                bulk_load_1d(ring + st * S::GROUP, A.kv.group(page, in.h, place), S::GROUP, bars + 8 * st);
+        const int at = in_k % BATCH;
+        if (at == 0) {
+            in_addr = 0;
+            bool bad = false;
+            const int place = (in.s.tlo + in.a + warp + (in_k + lane / G) * AD_WARPS) * S::TOK + (lane % G) * 16;
+            if (in_k + lane / G < in_n && place < in.s.len) {
+                const int page = __ldg(A.sq.table + (int64_t)in.b * A.sq.table_ld + (place >> A.kv.page_shift));
+                bad = page < 0 || page >= A.kv.num_pages;
+                if (!bad) in_addr = reinterpret_cast<uint64_t>(A.kv.group(page, in.h, place));
             }
-        } else {
-            // a page outside the cache: its keys' absmax is NaN, and so is every row that sees them
-            for (int i = lane; i < KV4_GROUP * NB; i += 32)
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(ring + st * S::GROUP + SOFF + 2 * i), "h"((uint16_t)0x7fff) : "memory");
-            __syncwarp();
-            if (lane == 0) { atomicExch(&g_attn4_status, KV4_BAD_PAGE); mbar_arrive(bars + 8 * st); }
+            in_bad = __ballot_sync(0xffffffffu, bad);
         }
-        put = put == AD_STAGES - 1 ? 0 : put + 1;
+        const uint32_t full = bars + 8 * put, dst = ring + put * S::STAGE;
+        if (in_bad >> (at * G) & ((1u << G) - 1u)) {
+            // a page outside the cache: its keys' absmax is NaN, and so is every row that sees them
+#pragma unroll
+            for (int x = 0; x < G; ++x)
+                if (in_bad >> (at * G + x) & 1u)
+                    for (int i = lane; i < KV4_GROUP * NB; i += 32)
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + x * S::GROUP + SOFF + 2 * i), "h"((uint16_t)0x7fff) : "memory");
+            if (lane == 0) atomicExch(&g_attn4_status, KV4_BAD_PAGE);
+            __syncwarp();
+        }
+        if (lane / G == at) {                                        // each of the tile's lanes fetches its own group
+            if (in_addr != 0) {
+                mbar_arrive_expect_tx(full, S::GROUP);
+                bulk_load_1d(dst + (lane % G) * S::GROUP, reinterpret_cast<const void *>(in_addr), S::GROUP, full);
+            } else {
+                mbar_arrive(full);
+            }
+        }
+        put = put == S::STAGES - 1 ? 0 : put + 1;
         ++in_k;
     };
 #pragma unroll 1
-    for (int i = 0; i < AD_STAGES; ++i) issue();
+    for (int i = 0; i < S::STAGES; ++i) issue();
 
     // ------------------------------------------------------------ consumer side
+    // A-operand row r of a group is token r / 2 (even r) or r / 2 + 4 (odd r), + 8 for rows 8 .. 15: the k index of P^T
+    // below then gives a lane the tokens c, c + 4, c + 8, c + 12
+    const int tok = (g >> 1) + 4 * (g & 1);
     uint32_t got = 0, phase = 0;                                     // next stage to read, its barrier's parity
     bool first_piece = true;
     do {
-        const Attn4Seq &sq = cur.s;
+        const AdSeq &sq = cur.s;
         const int first = sq.len - sq.n;
         // q as the B operand: lane (g, c) holds row g's channels blk * BS + c * (BS / 4) + ks * 4 + 0 .. 3
         uint32_t qf[NT][NB * MB][2];
@@ -319,35 +386,29 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) { m[nt][j] = ATTN4_NONE; l[nt][j] = 0.0f; }
 
+        int place0 = (sq.tlo + cur.a + warp) * S::TOK;
 #pragma unroll 1
-        for (int t = cur.a + warp; t < cur.e; t += AD_WARPS) {
-            const int place0 = (sq.tlo + t) * 16;
-            if (place0 >= sq.len) break;                             // the dead tile of an empty sequence
-            const uint32_t st = got;
-            if (!mbar_wait(bars + 8 * st, phase, abort_flag)) { atomicExch(&g_attn4_status, 402); *abort_flag = 1; }
-            const uint32_t kb = ring + st * S::GROUP, vb = kb + HALF;
-            // A-operand row r of the tile is token r / 2 (even r) or r / 2 + 4 (odd r), + 8 for rows 8 .. 15: the k index
-            // of P^T below then gives a lane the tokens c, c + 4, c + 8, c + 12
-            const int tok = (g >> 1) + 4 * (g & 1);
-            float s[NT][4];
+        for (int left = tiles_of(cur); left > 0; --left, place0 += AD_WARPS * S::TOK) {
+            if (!mbar_wait(bars + 8 * got, phase, abort_flag)) { atomicExch(&g_attn4_status, 402); *abort_flag = 1; }
+            const uint32_t kb = ring + got * S::STAGE;
+            // scores: s[x][nt][0..1] token tok of group x, columns 2c and 2c + 1; s[x][nt][2..3] token tok + 8
+            float s[G][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
-            {
+            for (int x = 0; x < G; ++x) {
+                const uint32_t kx = kb + x * S::GROUP;
                 float sc0[NB], sc1[NB];
-                ad_scales<T, NB>(kb + SOFF + tok * NB * 2, sc0);
-                ad_scales<T, NB>(kb + SOFF + (tok + 8) * NB * 2, sc1);
+                ad_scales<T, NB>(kx + SOFF + tok * NB * 2, sc0);
+                ad_scales<T, NB>(kx + SOFF + (tok + 8) * NB * 2, sc1);
 #pragma unroll
                 for (int blk = 0; blk < NB; ++blk) {
                     uint32_t w0[MB / 2], w1[MB / 2];
-                    const uint32_t ka = kb + tok * (D / 2) + blk * (BS / 2) + c * (BS / 8);
+                    const uint32_t ka = kx + tok * (D / 2) + blk * (BS / 2) + c * (BS / 8);
                     if constexpr (BS == 64) {
-                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w0[0]), "=r"(w0[1]) : "r"(ka) : "memory");
-                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w1[0]), "=r"(w1[1]) : "r"(ka + 8 * (D / 2)) : "memory");
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w0[0]), "=r"(w0[1]) : "r"(ka));
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w1[0]), "=r"(w1[1]) : "r"(ka + 8 * (D / 2)));
                     } else {
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0[0]) : "r"(ka) : "memory");
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1[0]) : "r"(ka + 8 * (D / 2)) : "memory");
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0[0]) : "r"(ka));
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1[0]) : "r"(ka + 8 * (D / 2)));
                     }
                     float acc[NT][4];
 #pragma unroll
@@ -363,57 +424,61 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                         for (int nt = 0; nt < NT; ++nt) ad_mma(acc[nt], a0, a1, a2, a3, qf[nt][blk * MB + ks][0], qf[nt][blk * MB + ks][1]);
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        s[nt][0] = fmaf(sc0[blk], acc[nt][0], s[nt][0]); s[nt][1] = fmaf(sc0[blk], acc[nt][1], s[nt][1]);
-                        s[nt][2] = fmaf(sc1[blk], acc[nt][2], s[nt][2]); s[nt][3] = fmaf(sc1[blk], acc[nt][3], s[nt][3]);
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float sc = j < 2 ? sc0[blk] : sc1[blk];
+                            s[x][nt][j] = blk == 0 ? sc * acc[nt][j] : fmaf(sc, acc[nt][j], s[x][nt][j]);
+                        }
+                }
+            }
+            // absmax of the values, token tok (+ 8) of group x
+            float sv[G][2][NB], sm = 0.0f;
+#pragma unroll
+            for (int x = 0; x < G; ++x) {
+                ad_scales<T, NB>(kb + x * S::GROUP + HALF + SOFF + tok * NB * 2, sv[x][0]);
+                ad_scales<T, NB>(kb + x * S::GROUP + HALF + SOFF + (tok + 8) * NB * 2, sv[x][1]);
+            }
+            uint32_t seen = 0xffffffffu;                             // bit (x * NT + nt) * 4 + j
+            if (place0 < full_lo || place0 + S::TOK > full_hi) {     // some row does not see some key (full_hi <= len)
+                seen = 0;
+#pragma unroll
+                for (int x = 0; x < G; ++x) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int place = place0 + 16 * x + tok + 8 * (j >> 1);
+                            if (place < lim[nt][j & 1] && place >= low[nt][j & 1]) seen |= 1u << ((x * NT + nt) * 4 + j);
+                            else s[x][nt][j] = __int_as_float(0xff800000);
+                        }
+                    // whatever lies in a place that no row sees
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int place = place0 + 16 * x + tok + 8 * y;
+                        if (place < any_lo || place >= any_hi) {
+#pragma unroll
+                            for (int blk = 0; blk < NB; ++blk) sv[x][y][blk] = 0.0f;
+                        }
                     }
                 }
             }
-            float sv0[NB], sv1[NB], sm = 0.0f;
-            ad_scales<T, NB>(vb + SOFF + tok * NB * 2, sv0);
-            ad_scales<T, NB>(vb + SOFF + (tok + 8) * NB * 2, sv1);
-            // s[nt][0..1]: token tok, columns 2c and 2c + 1; s[nt][2..3]: token tok + 8
-            const bool masked = place0 < full_lo || place0 + 16 > full_hi;   // (full_hi <= len)
-            uint32_t seen = 0;                                       // bit nt * 4 + j
-            if (masked) {
+#pragma unroll
+            for (int x = 0; x < G; ++x)
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) sm = fmaxf(sm, fmaxf(sv[x][0][blk], sv[x][1][blk]));
+            float p[G][NT][4], top = -1.0f;
+#pragma unroll
+            for (int x = 0; x < G; ++x)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int place = place0 + tok + 8 * (j >> 1);
-                        if (place < lim[nt][j & 1] && place >= low[nt][j & 1]) seen |= 1u << (nt * 4 + j);
-                        else s[nt][j] = __int_as_float(0xff800000);
+                        p[x][nt][j] = fmaf(s[x][nt][j], f[nt][j & 1], -m[nt][j & 1]);
+                        top = fmaxf(top, p[x][nt][j]);
                     }
-                // whatever lies in a place that no row sees
-                const bool in0 = place0 + tok >= any_lo && place0 + tok < any_hi, in1 = place0 + tok + 8 >= any_lo && place0 + tok + 8 < any_hi;
-#pragma unroll
-                for (int blk = 0; blk < NB; ++blk) { sv0[blk] = in0 ? sv0[blk] : 0.0f; sv1[blk] = in1 ? sv1[blk] : 0.0f; }
-            }
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk) {
-                sv0[blk] *= up; sv1[blk] *= up;
-                sm = fmaxf(sm, fmaxf(sv0[blk], sv1[blk]));
-            }
-            float p[NT][4], top = -1.0f;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    p[nt][j] = fmaf(s[nt][j], f[nt][j & 1], -m[nt][j & 1]);
-                    top = fmaxf(top, p[nt][j]);
-                }
             // p and absmax * up stay under 2^8 and 2^7, their product is at home in fp16
-            if (__any_sync(0xffffffffu, top > 8.0f || sm > 128.0f)) {
-                // (from the absmax itself: times `up` it may have left fp32)
-                ad_scales<T, NB>(vb + SOFF + tok * NB * 2, sv0);
-                ad_scales<T, NB>(vb + SOFF + (tok + 8) * NB * 2, sv1);
-                const bool in0 = place0 + tok >= any_lo && place0 + tok < any_hi, in1 = place0 + tok + 8 >= any_lo && place0 + tok + 8 < any_hi;
-                sm = 0.0f;
-#pragma unroll
-                for (int blk = 0; blk < NB; ++blk) {
-                    sv0[blk] = in0 ? sv0[blk] : 0.0f; sv1[blk] = in1 ? sv1[blk] : 0.0f;
-                    sm = fmaxf(sm, fmaxf(sv0[blk], sv1[blk]));
-                }
+            if (__any_sync(0xffffffffu, top > 8.0f || sm * up > 128.0f)) {
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, d));
                 float ku = 1.0f;
@@ -424,12 +489,12 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                     up = un;
                 }
 #pragma unroll
-                for (int blk = 0; blk < NB; ++blk) { sv0[blk] *= up; sv1[blk] *= up; }
-#pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float mx = fmaxf(s[nt][j], s[nt][j + 2]) * f[nt][j];
+                        float mx = fmaxf(s[0][nt][j], s[0][nt][j + 2]);
+                        if (G == 2) mx = fmaxf(mx, fmaxf(s[G - 1][nt][j], s[G - 1][nt][j + 2]));
+                        mx *= f[nt][j];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
                         const float mn = mx > m[nt][j] + 8.0f ? mx : m[nt][j], k = ex2(m[nt][j] - mn);
@@ -437,56 +502,61 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                         l[nt][j] *= k;
 #pragma unroll
                         for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k * ku; o[i][nt][j + 2] *= k * ku; }
-                        p[nt][j] = fmaf(s[nt][j], f[nt][j], -mn);
-                        p[nt][j + 2] = fmaf(s[nt][j + 2], f[nt][j], -mn);
+#pragma unroll
+                        for (int x = 0; x < G; ++x) {
+                            p[x][nt][j] = fmaf(s[x][nt][j], f[nt][j], -mn);
+                            p[x][nt][j + 2] = fmaf(s[x][nt][j + 2], f[nt][j], -mn);
+                        }
                     }
             }
-            float wt[NB][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    p[nt][j] = ex2(p[nt][j]);
-                    l[nt][j & 1] += p[nt][j];
-#pragma unroll
-                    for (int blk = 0; blk < NB; ++blk) wt[blk][nt][j] = p[nt][j] * (j < 2 ? sv0[blk] : sv1[blk]);
-                }
-            if (masked) {                                            // a value that is not finite is no matter of rows that do not see it
+            for (int x = 0; x < G; ++x)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (!(seen >> (nt * 4 + j) & 1u)) {
+                    for (int j = 0; j < 4; ++j) {
+                        p[x][nt][j] = ex2(p[x][nt][j]);
+                        l[nt][j & 1] += p[x][nt][j];
+                    }
+            // O^T += V^T P^T
 #pragma unroll
-                            for (int blk = 0; blk < NB; ++blk) wt[blk][nt][j] = 0.0f;
+            for (int x = 0; x < G; ++x) {
+                const uint32_t vb = kb + x * S::GROUP + HALF;
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) {
+                    const float s0 = sv[x][0][blk] * up, s1 = sv[x][1][blk] * up;
+                    uint32_t b0[NT], b1[NT];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float wt[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) wt[j] = p[x][nt][j] * (j < 2 ? s0 : s1);
+                        if (seen != 0xffffffffu) {                   // a value that is not finite is no matter of rows that do not see it
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) if (!(seen >> ((x * NT + nt) * 4 + j) & 1u)) wt[j] = 0.0f;
                         }
-            }
+                        b0[nt] = ad_transpose(ad_half2(wt[0], wt[1]));
+                        b1[nt] = ad_transpose(ad_half2(wt[2], wt[3]));
+                    }
+                    // lane (g, c): channels blk * BS + g * (BS / 8) + 0 .. BS / 8 - 1 of the tokens c, c + 4, c + 8, c + 12
+                    uint32_t w[4];
 #pragma unroll
-            for (int blk = 0; blk < NB; ++blk) {
-                uint32_t b0[NT], b1[NT];
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t va = vb + (c + 4 * i) * (D / 2) + blk * (BS / 2) + g * (BS / 16);
+                        if constexpr (BS == 64) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(va));
+                        else { uint16_t h; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(va)); w[i] = h; }
+                    }
+                    const uint32_t ev0 = (w[0] & 0x0F0F0F0Fu) | ((w[1] << 4) & 0xF0F0F0F0u), od0 = ((w[0] >> 4) & 0x0F0F0F0Fu) | (w[1] & 0xF0F0F0F0u);
+                    const uint32_t ev1 = (w[2] & 0x0F0F0F0Fu) | ((w[3] << 4) & 0xF0F0F0F0u), od1 = ((w[2] >> 4) & 0x0F0F0F0Fu) | (w[3] & 0xF0F0F0F0u);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    b0[nt] = ad_transpose(ad_half2(wt[blk][nt][0], wt[blk][nt][1]));
-                    b1[nt] = ad_transpose(ad_half2(wt[blk][nt][2], wt[blk][nt][3]));
-                }
-                // lane (g, c): channels blk * BS + g * (BS / 8) + 0 .. BS / 8 - 1 of the tokens c, c + 4, c + 8, c + 12
-                uint32_t w[4];
+                    for (int j = 0; j < MB; ++j) {
+                        const uint32_t a0 = ad_lut(lut, ev0, j), a1 = ad_lut(lut, od0, j), a2 = ad_lut(lut, ev1, j), a3 = ad_lut(lut, od1, j);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t va = vb + (c + 4 * i) * (D / 2) + blk * (BS / 2) + g * (BS / 16);
-                    if constexpr (BS == 64) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(va) : "memory");
-                    else { uint16_t h; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(va) : "memory"); w[i] = h; }
-                }
-                const uint32_t ev0 = (w[0] & 0x0F0F0F0Fu) | ((w[1] << 4) & 0xF0F0F0F0u), od0 = ((w[0] >> 4) & 0x0F0F0F0Fu) | (w[1] & 0xF0F0F0F0u);
-                const uint32_t ev1 = (w[2] & 0x0F0F0F0Fu) | ((w[3] << 4) & 0xF0F0F0F0u), od1 = ((w[2] >> 4) & 0x0F0F0F0Fu) | (w[3] & 0xF0F0F0F0u);
-#pragma unroll
-                for (int j = 0; j < MB; ++j) {
-                    const uint32_t a0 = ad_lut(lut, ev0, j), a1 = ad_lut(lut, od0, j), a2 = ad_lut(lut, ev1, j), a3 = ad_lut(lut, od1, j);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) ad_mma(o[blk * MB + j][nt], a0, a1, a2, a3, b0[nt], b1[nt]);
+                        for (int nt = 0; nt < NT; ++nt) ad_mma(o[blk * MB + j][nt], a0, a1, a2, a3, b0[nt], b1[nt]);
+                    }
                 }
             }
-            if (++got == AD_STAGES) { got = 0; phase ^= 1; }
+            if (++got == S::STAGES) { got = 0; phase ^= 1; }
             __syncwarp();                                            // every lane has read the stage
             issue();
         }
@@ -516,12 +586,16 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
             }
         const bool whole = cur.a == 0 && cur.e == sq.nt;
         float *part = ad_partial<D, RT>(A.ws, team, first_piece ? 0 : 1);
+        if (cur.a == 0 && !whole && warp == 0 && lane == 0) {
+            join->n = 1 + (int)((sq.nt - cur.e + per - 1) / per);
+            join->slot = first_piece ? 0 : 1;
+            join->row0 = sq.row0; join->rows = sq.n * A.group; join->r = cur.r; join->h = cur.h;
+        }
 #pragma unroll
-        for (int d0 = 0; d0 < D; d0 += 64) {                         // 64 channels per pass
+        for (int d0 = 0; d0 < D; d0 += S::RED_D) {                   // a pass is all channels, or 64 of 256
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-                const int mt = d0 / 16 + i4, blk = mt / MB, j2 = mt % MB;
-                const int d = blk * BS + g * (BS / 8) + 2 * j2 - d0;
+            for (int mt = d0 / 16; mt < (d0 + S::RED_D) / 16; ++mt) {
+                const int d = mt / MB * BS + g * (BS / 8) + 2 * (mt % MB) - d0;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -529,89 +603,82 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                         *reinterpret_cast<float2 *>(red + (warp * RT + nt * 8 + 2 * c + j) * S::RED_LD + d) = make_float2(o[mt][nt][j], o[mt][nt][j + 2]);
             }
             team_sync();
-            for (int x = warp * 32 + lane; x < RT * 32; x += AD_WARPS * 32) {
-                const int row = x >> 5, d = 2 * (x & 31);
-                const int R = cur.r * RT + row, i = R / A.group;
-                if (i < sq.n) {
-                    float M = stat[row].x, L = 0.0f;
-                    float2 v = make_float2(0.0f, 0.0f);
+            constexpr int PAIRS = S::RED_D / 2;
 #pragma unroll
-                    for (int w = 1; w < AD_WARPS; ++w) M = fmaxf(M, stat[w * RT + row].x);
+            for (int x = warp * 32 + lane; x < RT * PAIRS; x += AD_WARPS * 32) {
+                const int row = x / PAIRS, d = 2 * (x % PAIRS), R = cur.r * RT + row, i = R / A.group;
+                if (i >= sq.n) continue;
+                float M = stat[row].x, L = 0.0f;
+                float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-                    for (int w = 0; w < AD_WARPS; ++w) {
-                        const float2 y = *reinterpret_cast<const float2 *>(red + (w * RT + row) * S::RED_LD + d), z = stat[w * RT + row];
-                        v.x += y.x; v.y += y.y;
-                        L = fmaf(z.y, ex2(z.x - M), L);
-                    }
-                    if (whole) {
-                        const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
-                        const int64_t orow = (int64_t)(sq.row0 + i) * A.heads + cur.h * A.group + (R - i * A.group);
-                        T pr[2] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv)};
-                        *reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(A.out) + orow * D + d0 + d) = *reinterpret_cast<const uint32_t *>(pr);
-                        if (A.lse != nullptr && d0 == 0 && d == 0) A.lse[orow] = L == 0.0f ? __int_as_float(0xff800000) : (M + __log2f(L)) * 0.69314718f;
-                    } else {
-                        *reinterpret_cast<float2 *>(part + row * D + d0 + d) = v;
-                        if (d0 == 0 && d == 0) *reinterpret_cast<float2 *>(part + RT * D + 2 * row) = make_float2(M, L);
-                    }
+                for (int w = 1; w < AD_WARPS; ++w) M = fmaxf(M, stat[w * RT + row].x);
+#pragma unroll
+                for (int w = 0; w < AD_WARPS; ++w) {
+                    const float2 y = *reinterpret_cast<const float2 *>(red + (w * RT + row) * S::RED_LD + d), z = stat[w * RT + row];
+                    v.x += y.x; v.y += y.y;
+                    L = fmaf(z.y, ex2(z.x - M), L);
+                }
+                if (whole) {
+                    const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
+                    const int64_t orow = (int64_t)(sq.row0 + i) * A.heads + cur.h * A.group + (R - i * A.group);
+                    T pr[2] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv)};
+                    *reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(A.out) + orow * D + d0 + d) = *reinterpret_cast<const uint32_t *>(pr);
+                    if (A.lse != nullptr && d0 == 0 && d == 0) A.lse[orow] = L == 0.0f ? __int_as_float(0xff800000) : (M + __log2f(L)) * 0.69314718f;
+                } else {
+                    *reinterpret_cast<float2 *>(part + row * D + d0 + d) = v;
+                    if (d0 == 0 && d == 0) *reinterpret_cast<float2 *>(part + RT * D + 2 * row) = make_float2(M, L);
                 }
             }
-            team_sync();                                         // red (and, at the end, stat) may be written again
+            team_sync();                                             // red (and, at the end, stat) may be written again
         }
         first_piece = false;
-    } while (cur.next(A, RT));
+    } while (cur.next(A));
 }
 
-// Joins the partial results of one (sequence, head, row tile, row): sum of 2^(m_i - M) O_i over sum of 2^(m_i - M) l_i.
+// Joins partial results: sum of 2^(m_i - M) O_i over sum of 2^(m_i - M) l_i.  A block is one row of what one team began and others
+// went on with; its warps share the parts, each with a running maximum of its own.
+constexpr int AD_JOIN_WARPS = 4;
 template <int D, int RT, typename T>
-__global__ void __launch_bounds__(256)
-attn4_combine_kernel(const __grid_constant__ Attn4Args A, int teams, int rts_max) {
-    __shared__ float red[8][D];
-    __shared__ float reds[8];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int x = blockIdx.x;
-    const int row = x % RT; x /= RT;
-    const int r = x % rts_max; x /= rts_max;
-    const int h = x % A.kv.kv_heads, b = x / A.kv.kv_heads;
-    Attn4Seq s;
-    s.get(A, b, RT);
-    const int R = r * RT + row, i = R / A.group;
-    int64_t before, total;
-    attn4_prefix(A, RT, b, before, total);
+__global__ void __launch_bounds__(AD_JOIN_WARPS * 32)
+attn4_combine_kernel(const __grid_constant__ Attn4Args A, int teams) {
+    __shared__ float red[AD_JOIN_WARPS][D + 2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c0 = blockIdx.x, row = blockIdx.y;
     // every block waits, so that this kernel's end means the end of the one before it as well
     pdl_grid_dependency_wait();
-    if (r >= s.rts || i >= s.n) return;                              // whole block
-    const int64_t per = ad_per(total, teams);
-    const int64_t t0 = before + (int64_t)(h * s.rts + r) * s.nt, c0 = t0 / per, c1 = (t0 + s.nt - 1) / per;
-    if (c0 == c1) return;                                            // one team had it all and has written it
-    float M = ATTN4_NONE;
-    for (int64_t ci = c0 + lane; ci <= c1; ci += 32)
-        M = fmaxf(M, ad_partial<D, RT>(A.ws, ci, t0 <= ci * per ? 0 : 1)[RT * D + 2 * row]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float L = 0.0f, v[D / 32];
+    const AdJoin p = ad_join<D, RT>(A.ws, teams)[c0];
+    const int R = p.r * RT + row;
+    if (p.n == 0 || R >= p.rows) return;
+    float M = ATTN4_NONE, L = 0.0f, v[D / 32];
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) v[j] = 0.0f;
-    for (int64_t ci = c0 + warp; ci <= c1; ci += 8) {
-        const float *p = ad_partial<D, RT>(A.ws, ci, t0 <= ci * per ? 0 : 1);
-        const float2 ml = *reinterpret_cast<const float2 *>(p + RT * D + 2 * row);
-        const float k = ex2(ml.x - M);
-        L = fmaf(ml.y, k, L);
+#pragma unroll 4
+    for (int x = warp; x < p.n; x += AD_JOIN_WARPS) {
+        const float *q = ad_partial<D, RT>(A.ws, c0 + x, x == 0 ? p.slot : 0);
+        const float2 ml = *reinterpret_cast<const float2 *>(q + RT * D + 2 * row);
+        const float mn = fmaxf(M, ml.x), ko = ex2(M - mn), kn = ex2(ml.x - mn);
+        M = mn;
+        L = L * ko + ml.y * kn;
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) v[j] = fmaf(p[row * D + j * 32 + lane], k, v[j]);
+        for (int j = 0; j < D / 32; ++j) v[j] = v[j] * ko + q[row * D + j * 32 + lane] * kn;
     }
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) red[warp][j * 32 + lane] = v[j];
-    if (lane == 0) reds[warp] = L;
+    if (lane == 0) { red[warp][D] = M; red[warp][D + 1] = L; }
     __syncthreads();
+    M = red[0][D];
+#pragma unroll
+    for (int w = 1; w < AD_JOIN_WARPS; ++w) M = fmaxf(M, red[w][D]);
+    float k[AD_JOIN_WARPS];
     L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) L += reds[w];
+    for (int w = 0; w < AD_JOIN_WARPS; ++w) { k[w] = ex2(red[w][D] - M); L = fmaf(red[w][D + 1], k[w], L); }
+    const int i = R / A.group;
     const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
-    const int64_t orow = (int64_t)(s.row0 + i) * A.heads + h * A.group + (R - i * A.group);
-    for (int d = threadIdx.x; d < D; d += 256) {
+    const int64_t orow = (int64_t)(p.row0 + i) * A.heads + p.h * A.group + (R - i * A.group);
+    for (int d = threadIdx.x; d < D; d += AD_JOIN_WARPS * 32) {
         float y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) y += red[w][d];
+        for (int w = 0; w < AD_JOIN_WARPS; ++w) y = fmaf(red[w][d], k[w], y);
         reinterpret_cast<T *>(A.out)[orow * D + d] = from_f32<T>(y * inv);
     }
     if (A.lse != nullptr && threadIdx.x == 0) A.lse[orow] = L == 0.0f ? __int_as_float(0xff800000) : (M + __log2f(L)) * 0.69314718f;
@@ -623,10 +690,10 @@ attn4_combine_kernel(const __grid_constant__ Attn4Args A, int teams, int rts_max
 // 16 rows per tile where 8 do not hold a sequence's rows: the keys are then expanded half as often
 static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return (int64_t)s->new_tokens * group > 8 ? 2 : 1; }
 
-static int ad_teams(int D, int NT) { return sm_count() * (D * NT <= 128 ? 2 : 1); }
+static int ad_teams(int D, int NT) { return sm_count() * ((D * NT <= 128 ? 12 : 8) / AD_WARPS); }
 
 template <int D, int BS, int NT, typename T>
-static int ad_launch(const Attn4Args &a, int rts_max, cudaStream_t st) {
+static int ad_launch(const Attn4Args &a, cudaStream_t st) {
     using S = AdSmem<D, BS, NT>;
     static bool configured[64] = {};
     int dev = 0;
@@ -639,25 +706,23 @@ static int ad_launch(const Attn4Args &a, int rts_max, cudaStream_t st) {
     attn4_decode_kernel<D, BS, NT, T><<<teams / S::TEAMS, S::THREADS, S::BYTES, st>>>(a);
     int rc = check_launch();
     if (rc != MPSBNB_OK) return rc;
-    const int64_t blocks = (int64_t)a.sq.batch * a.kv.kv_heads * rts_max * S::RT;
-    if (blocks > 0x7fffffffll) return MPSBNB_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(teams, S::RT);
+    cfg.blockDim = dim3(AD_JOIN_WARPS * 32);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    MPSBNB_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_combine_kernel<D, S::RT, T>, a, teams, rts_max));
+    MPSBNB_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_combine_kernel<D, S::RT, T>, a, teams));
     return check_launch();
 }
 
 template <int D, int BS>
-static int ad_launch_t(const Attn4Args &a, int dtype, int nt, int rts_max, cudaStream_t st) {
-    if (dtype == MPSBNB_F16) return nt == 1 ? ad_launch<D, BS, 1, __half>(a, rts_max, st) : ad_launch<D, BS, 2, __half>(a, rts_max, st);
-    return nt == 1 ? ad_launch<D, BS, 1, __nv_bfloat16>(a, rts_max, st) : ad_launch<D, BS, 2, __nv_bfloat16>(a, rts_max, st);
+static int ad_launch_t(const Attn4Args &a, int dtype, int nt, cudaStream_t st) {
+    if (dtype == MPSBNB_F16) return nt == 1 ? ad_launch<D, BS, 1, __half>(a, st) : ad_launch<D, BS, 2, __half>(a, st);
+    return nt == 1 ? ad_launch<D, BS, 1, __nv_bfloat16>(a, st) : ad_launch<D, BS, 2, __nv_bfloat16>(a, st);
 }
 
 int attn4_decode_status_fetch(int *out, bool reset) {
@@ -677,7 +742,7 @@ extern "C" size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *
     if (kv4_check_cache(cache, 0) != MPSBNB_OK || kv4_check_seqs(seqs, cache) != MPSBNB_OK) return 0;
     if (heads <= 0 || heads % cache->kv_heads != 0 || seqs->batch == 0 || seqs->tokens == 0) return 0;
     const int nt = ad_nt(seqs, heads / cache->kv_heads);
-    return (size_t)ad_teams(cache->head_dim, nt) * 2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float);
+    return (size_t)ad_teams(cache->head_dim, nt) * (2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float) + sizeof(AdJoin));
 }
 
 extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
@@ -702,17 +767,18 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.out = out; a.lse = lse; a.ws = (float *)workspace;
     a.heads = heads; a.group = group; a.causal = causal != 0; a.window = window; a.quant_type = cache->quant_type;
     a.scale_log2 = scale * 1.4426950408889634f;
+    static const float codes[2][16] = {MPSBNB_NF4_TABLE, MPSBNB_FP4_TABLE};
+    for (int i = 0; i < 16; ++i) a.code[i] = codes[cache->quant_type][i] * attn4_code_scale(cache->quant_type);
     if ((int64_t)seqs->new_tokens * group >= 128) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, (cudaStream_t)stream);
     const int nt = ad_nt(seqs, group);
-    const int rts_max = (seqs->new_tokens * group + 8 * nt - 1) / (8 * nt);
     cudaStream_t st = (cudaStream_t)stream;
     const int dt = cache->dtype;
     if (cache->blocksize == 32) {
-        if (cache->head_dim == 64) return ad_launch_t<64, 32>(a, dt, nt, rts_max, st);
-        if (cache->head_dim == 128) return ad_launch_t<128, 32>(a, dt, nt, rts_max, st);
-        return ad_launch_t<256, 32>(a, dt, nt, rts_max, st);
+        if (cache->head_dim == 64) return ad_launch_t<64, 32>(a, dt, nt, st);
+        if (cache->head_dim == 128) return ad_launch_t<128, 32>(a, dt, nt, st);
+        return ad_launch_t<256, 32>(a, dt, nt, st);
     }
-    if (cache->head_dim == 64) return ad_launch_t<64, 64>(a, dt, nt, rts_max, st);
-    if (cache->head_dim == 128) return ad_launch_t<128, 64>(a, dt, nt, rts_max, st);
-    return ad_launch_t<256, 64>(a, dt, nt, rts_max, st);
+    if (cache->head_dim == 64) return ad_launch_t<64, 64>(a, dt, nt, st);
+    if (cache->head_dim == 128) return ad_launch_t<128, 64>(a, dt, nt, st);
+    return ad_launch_t<256, 64>(a, dt, nt, st);
 }

@@ -157,7 +157,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
         tmem_relinquish();
     }
     if (warp >= AP_EXPAND && warp < AP_MMA) {
-        const float mine = kCode[A.quant_type][lane & 15] * attn4_code_scale(A.quant_type);
+        const float mine = A.code[lane & 15];
         for (int x = warp - AP_EXPAND; x < 256; x += 8) {
             const float c0 = __shfl_sync(0xffffffffu, mine, x & 15), c1 = __shfl_sync(0xffffffffu, mine, x >> 4);
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(sb + (uint32_t)(S::LUT + x * 128 + lane * 4)), "r"(ap_half2(c0, c1)) : "memory");

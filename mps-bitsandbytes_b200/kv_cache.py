@@ -26,7 +26,6 @@ import torch
 from torch import Tensor
 
 from . import _native as N
-from .functional import _workspace
 
 _GROUP = 16                                         # tokens per group of the layout (include/mpsbnb_b200.h)
 
@@ -293,6 +292,11 @@ def _on(device: torch.device):
     return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _stream(device: torch.device) -> int:
+    """The current stream's handle, without the Stream object that torch.cuda.current_stream() makes (3 us of a 20 us call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 # ---------------------------------------------------------------------- operators
 def append_kv_4bit(cache: KVCache4bit, layer: int, k: Tensor, v: Tensor, page_table: Tensor, seq_lens: Tensor,
                    cu_seqlens: Optional[Tensor] = None) -> None:
@@ -313,7 +317,7 @@ def append_kv_4bit(cache: KVCache4bit, layer: int, k: Tensor, v: Tensor, page_ta
     with _on(cache.device):
         N.check(N.lib().mpsbnb_kv4_append(cache._ref, layer, C.byref(sq), kr.data_ptr(), kr.stride(0), kr.stride(1),
                                           vr.data_ptr(), vr.stride(0), vr.stride(1),
-                                          torch.cuda.current_stream().cuda_stream), "append_kv_4bit")
+                                          _stream(cache.device)), "append_kv_4bit")
 
 
 def dequantize_kv_4bit(cache: KVCache4bit, layer: int, page_table: Tensor, seq_lens: Tensor,
@@ -327,11 +331,10 @@ def dequantize_kv_4bit(cache: KVCache4bit, layer: int, page_table: Tensor, seq_l
     if max_len < 0:
         raise ValueError(f"max_len must not be negative, got {max_len}")
     shape = (page_table.shape[0], int(max_len), cache.num_kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-    v = torch.empty(shape, dtype=cache.dtype, device=cache.device)
+    k, v = cache.k_absmax.new_empty(shape), cache.k_absmax.new_empty(shape)
     with _on(cache.device):
         N.check(N.lib().mpsbnb_kv4_dequantize(cache._ref, layer, C.byref(sq), max_len, k.data_ptr(), v.data_ptr(),
-                                              torch.cuda.current_stream().cuda_stream), "dequantize_kv_4bit")
+                                              _stream(cache.device)), "dequantize_kv_4bit")
     return k, v
 
 
@@ -360,7 +363,7 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
         raise ValueError(f"window must be positive and needs causal=True, got {window}")
     sq = _seqs(cache, page_table, seq_lens, cu_seqlens, qr.shape[0], max_seqlen)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if cu_seqlens is None else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape) if cu_seqlens is None else q.new_zeros(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}, 16-byte aligned")
     lse = None
@@ -369,11 +372,11 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
     lib = N.lib()
     with _on(cache.device):
         nbytes = lib.mpsbnb_attention_4bit_workspace_bytes(cache._ref, C.byref(sq), heads)
-        ws = _workspace(nbytes, cache.device)
+        ws = cache.data.new_empty(nbytes)
         N.check(lib.mpsbnb_attention_4bit(
             cache._ref, layer, C.byref(sq), qr.data_ptr(), qr.stride(0), qr.stride(1), heads, int(causal), int(window or 0),
             float(cache.head_dim ** -0.5 if scale is None else scale), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream), "attention_4bit")
+            ws.data_ptr(), nbytes, _stream(cache.device)), "attention_4bit")
     return (out, lse) if return_lse else out
 
 
@@ -397,4 +400,4 @@ def copy_kv_pages_4bit(cache: KVCache4bit, src: Sequence[int], dst: Sequence[int
     array = C.c_int32 * len(src)
     with _on(cache.device):
         N.check(N.lib().mpsbnb_kv4_copy_pages(cache._ref, array(*src), array(*dst), len(src),
-                                              torch.cuda.current_stream().cuda_stream), "copy_kv_pages_4bit")
+                                              _stream(cache.device)), "copy_kv_pages_4bit")
