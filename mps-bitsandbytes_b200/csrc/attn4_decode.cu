@@ -34,7 +34,7 @@ static __device__ int g_attn4_status = 0;
 
 constexpr int AD_WARPS = 4;                                          // of a team: the warps that share a run of tiles
 // What a (sequence, head, row tile) counts besides its tokens, in tokens: q, the joining of the warps
-constexpr int AD_COST_TOKENS = 256;
+constexpr int AD_COST_TOKENS = 512;
 constexpr uint32_t AD_LUT = 65536;                                   // shared-window address of the table
 constexpr uint32_t AD_BASE = 1024;                                   // ... and of the dynamic shared memory
 
@@ -188,8 +188,8 @@ template <class S> struct AdPiece {
     }
 };
 
-// units per team: equal, and a few tiles for each of a team's warps
-__device__ __forceinline__ int64_t ad_per(int64_t total, int teams) { return max(ad_div(total + teams - 1, teams), (int64_t)(4 * AD_WARPS)); }
+// units per team: equal, and worth a piece with a few tiles for each of the warps
+__device__ __forceinline__ int64_t ad_per(int64_t total, int teams, int cost) { return max(ad_div(total + teams - 1, teams), (int64_t)(cost + 4 * AD_WARPS)); }
 
 // partial result of team c, slot s (0: its first piece, 1: its last): RT x D sums, then RT (maximum, sum) pairs
 template <int D, int RT> __device__ __forceinline__ float *ad_partial(float *ws, int64_t c, int s) {
@@ -241,7 +241,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     for (int b = 32 + lane; b < A.sq.batch; b += 32) total += ad_units<S>(A, b);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int64_t per = ad_per(total, teams), t0 = min(total, team * per), t1 = min(total, t0 + per);
+    const int64_t per = ad_per(total, teams, S::COST), t0 = min(total, team * per), t1 = min(total, t0 + per);
     // what the teams leave for attn4_combine_kernel (a team's thread 0 writes both)
     AdJoin *join = ad_join<D, RT>(A.ws, teams) + team;
     if (warp == 0 && lane == 0) join->n = 0;

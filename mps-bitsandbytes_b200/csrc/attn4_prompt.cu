@@ -3,18 +3,21 @@
 //
 // Bound: the tensor pipe (4 rows keys head_dim operations) and, close behind, the exponentials (16 a clock and SM).
 //
-// One CTA takes 256 rows (or the last 128) of one (sequence, kv head); a row is a (new token, head of the group) pair,
-// so all heads of a group share each expanded tile.  Two 128-row tiles A and B alternate: while the softmax warps of
-// one work, the tensor core does the other's products.  head_dim 256 takes one tile of 128 rows (tensor memory: 256
-// columns of O) and 64 keys at a time.  Roles:
-//   warps 0-3, 4-7  softmax of tile A / B, one row per thread: S from tensor memory twice (maximum; exponentials), P back
-//                   over S as fp16, the row's sum in fp32.  O stays in tensor memory; it is rescaled by these warps only
-//                   when a row's maximum has grown by more than 2^8 since the reference was last moved.
-//   warps 8-15      expand a tile of KT keys: byte -> fp16 pair by a table held once per lane, times the block's absmax,
+// A block takes 256 rows (or the last 128) of one (sequence, kv head) at a time, long ones first; a row is a (new token,
+// head of the group) pair, so all heads of a group share each expanded tile.  Two 128-row tiles A and B alternate: while
+// the softmax warps of one work, the tensor core does the other's products.  head_dim 256 takes one tile of 128 rows
+// (tensor memory: 256 columns of O), 64 keys at a time and two buffers of S instead.  Roles:
+//   warps 0-3, 4-7  softmax of tile A / B, one row per thread: S from tensor memory, P back over S as fp16, the row's sum
+//                   in fp32.  The reference m follows the maximum only when that exceeds it by more than 2^8; O stays in
+//                   tensor memory and is rescaled only then.
+//   warps 8-11      expand a tile of KT keys: byte -> fp16 pair by a table held once per lane, times the block's absmax,
 //                   into 128-byte-swizzled panels [KT][64 channels].  For K that is the K-major operand of S = Q K^T,
-//                   for V - the same layout read the other way - the MN-major operand of O = P V.
-//   warp 16         issues the MMAs: S_A, S_B, then per key tile O_A += P_A V, S_A(next), O_B += P_B V, S_B(next).
-//   warp 17         fetches the codes: one bulk copy per group of 16 tokens, two tiles ahead.
+//                   for V - the same layout read the other way - the MN-major operand of O = P V.  K and V take turns in
+//                   a ring of three buffers, so expanding runs ahead of the products.
+//   warp 12         issues the MMAs: S_A, S_B, then per key tile O_A += P_A V, S_A(next), O_B += P_B V, S_B(next), on
+//                   into the next block of rows without a pause.
+//   warp 13         fetches the codes: one bulk copy per group of 16 tokens, two tiles ahead.
+//   warps 14, 15    bring the next rows of q as soon as the last products with the present ones have been issued.
 // fp16 operands hold bf16 caches too: the absmax of a K tile (and, carried along, of the V tiles) is brought near 2^8 by
 // a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.
 #include <type_traits>
@@ -31,42 +34,66 @@ static __device__ int g_attn4_prompt_status = 0;
 // P is 2^(x - m + 7): at most 2^15 while the reference m lags by 2^8, and what lies 2^21 below the reference still has
 // fp16's full precision.
 constexpr float AP_LIFT = 7.0f;
-constexpr int AP_EXPAND = 8;                                         // first expander warp (of eight)
-constexpr int AP_MMA = 16, AP_LOAD = 17, AP_THREADS = 18 * 32;
+constexpr int AP_EXPAND = 8, AP_EXPANDERS = 4;                       // first expander warp, their number
+constexpr int AP_MMA = 12, AP_LOAD = 13, AP_Q = 14, AP_THREADS = 16 * 32;
+// Registers: launched with 128 a thread (512 threads: all of the SM's); the warpgroups then share them out anew.  (A spilled
+// register costs a trip to L2 here: shared memory leaves next to nothing of L1.)
+constexpr int AP_REGS = 128, AP_REGS_SOFTMAX = 160, AP_REGS_EXPAND = 112, AP_REGS_OTHER = 80;
+static_assert(2 * AP_REGS_SOFTMAX + AP_REGS_EXPAND + AP_REGS_OTHER <= 4 * AP_REGS, "a raise beyond the launch's registers would wait for ever");
+template <int N> __device__ __forceinline__ void ap_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void ap_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int D, int BS> struct ApSmem {
     static constexpr int TILES = D > 128 ? 1 : 2;                    // 128-row tiles
     static constexpr int KT = D > 128 ? 64 : 128;                    // keys per tile
-    static constexpr int PANELS = D / 64, PANEL = KT * 128, Q_PANEL = 128 * 128;
+    static constexpr int PANELS = D / 64, PANEL = KT * 128, Q_PANEL = 128 * 128, BUF = PANELS * PANEL;
     static constexpr int GROUP = 2 * kv4_half_bytes(D, BS), CODES = KT / KV4_GROUP * GROUP;
+    static constexpr int NBUF = D > 64 && BS == 32 ? 2 : 3;          // operand buffers (what fits)
     static constexpr int Q = 0;
-    static constexpr int K = Q + TILES * PANELS * Q_PANEL;
-    static constexpr int V = K + PANELS * PANEL;
-    static constexpr int LUT = V + PANELS * PANEL;
+    static constexpr int RING = Q + TILES * PANELS * Q_PANEL;
+    static constexpr int LUT = RING + NBUF * BUF;
     static constexpr int RAW = LUT + 256 * 128;
-    static constexpr int BAR = RAW + 2 * CODES;
-    static constexpr int TOTAL = BAR + 32 * 8;
+    static constexpr int EXPO = RAW + 2 * CODES;                     // [2][TILES * 128] bytes: exponent that a bf16 row of q was brought down by
+    static constexpr int BAR = EXPO + 2 * TILES * 128;
+    static constexpr int TOTAL = BAR + 256;
     // tensor memory columns
-    static constexpr int S_COL = 0, O_COL = TILES * 128;
+    static constexpr int S_COL = 0, S_STEP = TILES == 2 ? 128 : 64, O_COL = 2 * S_STEP;
     static_assert(O_COL + TILES * D <= 512, "tensor memory");
-    static_assert(TOTAL + 1024 <= 227 * 1024, "shared memory of the prompt kernel");
 };
 
-// MN-major operand with the 128-byte swizzle: panels of 64 elements (128 bytes) along MN, `panel` bytes apart; groups of
-// eight k-rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t ap_desc_mn(uint32_t addr, int panel) {
-    uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(panel >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
+// Matrix descriptors with the 128-byte swizzle, by halves (the upper one is a constant): rows of 128 bytes, groups of
+// eight of them 1024 bytes apart.  K-major: a row is one of M or N, 64 elements of K.  MN-major: a row is one of K, 64
+// elements of M or N; the next 64 are `panel` bytes on.
+constexpr uint32_t AP_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t ap_desc_k(uint32_t addr) { return (addr & 0x3FFFFu) >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t ap_desc_mn(uint32_t addr, int panel) { return (addr & 0x3FFFFu) >> 4 | (uint32_t)(panel >> 4) << 16; }
+__device__ __forceinline__ void ap_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(AP_DESC_HI)
+        : "memory");
+}
+__device__ __forceinline__ void ap_mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(AP_DESC_HI)
+        : "memory");
 }
 __device__ __forceinline__ void ap_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void ap_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ uint32_t ap_half2(float lo, float hi) {
@@ -127,27 +154,34 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
     constexpr bool BF = !std::is_same<T, __half>::value;
     constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
     using Item = ApItem<TILES, KT>;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t sb = smem_u32(smem), bar = sb + S::BAR;
-    const uint32_t k_full = bar + 8, k_empty = bar + 16, v_full = bar + 24, v_empty = bar + 32;
-    auto raw_full = [&](int s) { return bar + 40 + 8u * s; };
-    auto raw_empty = [&](int s) { return bar + 56 + 8u * s; };
-    auto s_full = [&](int t) { return bar + 72 + 8u * t; };
-    auto p_full = [&](int t) { return bar + 88 + 8u * t; };
-    auto o_done = [&](int t) { return bar + 104 + 8u * t; };
-    auto q_full = [&](int t) { return bar + 120 + 8u * t; };
+    if ((sb & 1023u) != 0) {                                         // the swizzle counts on it
+        if (threadIdx.x == 0) atomicExch(&g_attn4_prompt_status, 410);
+        return;
+    }
+    auto buf_full = [&](int s) { return bar + 8u * s; };             // [3]
+    auto buf_empty = [&](int s) { return bar + 24 + 8u * s; };       // [3]
+    auto raw_full = [&](int s) { return bar + 48 + 8u * s; };        // [2] each from here on
+    auto raw_empty = [&](int s) { return bar + 64 + 8u * s; };
+    auto s_full = [&](int s) { return bar + 80 + 8u * s; };          // by buffer of S: the row tile, or (one row tile) turn about
+    auto p_full = [&](int s) { return bar + 96 + 8u * s; };
+    auto o_done = [&](int s) { return bar + 112 + 8u * s; };         // by buffer of S
+    auto q_full = [&](int t) { return bar + 128 + 8u * t; };
+    auto q_empty = [&](int t) { return bar + 144 + 8u * t; };
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + S::BAR + 160);
     volatile uint32_t *abort_flag = tmem_slot + 1, *never = tmem_slot + 2;               // never: stays 0
-    volatile float *k_pow = reinterpret_cast<volatile float *>(smem + S::BAR + 176);     // [2]: power of two of a K tile
-    volatile int *v_exp = reinterpret_cast<volatile int *>(smem + S::BAR + 192);         // [2]: V's exponent from a tile on
+    volatile float *k_pow = reinterpret_cast<volatile float *>(smem + S::BAR + 176);     // [4]: power of two of a K tile
+    volatile int *v_exp = reinterpret_cast<volatile int *>(smem + S::BAR + 192);         // [4]: V's exponent from a tile on
+    volatile uint8_t *q_exp = smem + S::EXPO;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(k_full, 8); mbar_init(k_empty, 1); mbar_init(v_full, 8); mbar_init(v_empty, 1);
+        for (int i = 0; i < S::NBUF; ++i) { mbar_init(buf_full(i), AP_EXPANDERS); mbar_init(buf_empty(i), 1); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(raw_full(i), 1); mbar_init(raw_empty(i), 8);
-            mbar_init(s_full(i), 1); mbar_init(p_full(i), 4); mbar_init(o_done(i), 1); mbar_init(q_full(i), 4);
+            mbar_init(raw_full(i), 1); mbar_init(raw_empty(i), AP_EXPANDERS);
+            mbar_init(s_full(i), 1); mbar_init(p_full(i), 4); mbar_init(o_done(i), 1);
+            mbar_init(q_full(i), 2); mbar_init(q_empty(i), 1);
         }
         *abort_flag = *never = 0;
         fence_mbar_init();
@@ -158,7 +192,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
     }
     if (warp >= AP_EXPAND && warp < AP_MMA) {
         const float mine = A.code[lane & 15];
-        for (int x = warp - AP_EXPAND; x < 256; x += 8) {
+        for (int x = warp - AP_EXPAND; x < 256; x += AP_EXPANDERS) {
             const float c0 = __shfl_sync(0xffffffffu, mine, x & 15), c1 = __shfl_sync(0xffffffffu, mine, x >> 4);
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(sb + (uint32_t)(S::LUT + x * 128 + lane * 4)), "r"(ap_half2(c0, c1)) : "memory");
         }
@@ -167,109 +201,220 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    // Every role walks the block's items by itself; what it counts runs on from item to item: key tiles (jj), and tiles
-    // of scores per row tile.
+    // Every role walks the block's items by itself; what it counts (key tiles, operands, tiles of scores) runs on from item
+    // to item.
 #define AP_WAIT(b_, ph_, code_) if (!mbar_wait(b_, ph_, abort_flag)) { atomicExch(&g_attn4_prompt_status, code_); *abort_flag = 1; break; }
 
-    if (warp == AP_LOAD) {
-        // ------------------------------------------------------------ codes
-        int jj = 0;
-        for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
-            Item w;
-            if (!w.get(A, item, blocks)) continue;
-            for (int j = 0; j < w.nk; ++j, ++jj) {
-                const int st = jj & 1;
-                AP_WAIT(raw_empty(st), ((jj >> 1) & 1) ^ 1, 411);
-                const int place = w.start + j * KT + lane * KV4_GROUP;
-                const bool want = lane < KT / KV4_GROUP && place < w.hi;
-                int page = -1;
-                if (want) page = __ldg(A.sq.table + (int64_t)w.b * A.sq.table_ld + (place >> A.kv.page_shift));
-                const bool good = want && page >= 0 && page < A.kv.num_pages;
-                const uint32_t dst = sb + S::RAW + st * S::CODES + lane * S::GROUP;
-                if (want && !good) {
-                    // a page outside the cache: its keys are NaN
-                    atomicExch(&g_attn4_prompt_status, KV4_BAD_PAGE);
-                    for (int i = 0; i < KV4_GROUP * NB; ++i) {
-                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + SOFF + 2 * i), "h"((uint16_t)0x7fff) : "memory");
-                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + HALF + SOFF + 2 * i), "h"((uint16_t)0) : "memory");
-                    }
-                }
-                const uint32_t goods = __ballot_sync(0xffffffffu, good);
-                __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(raw_full(st), (uint32_t)(__popc(goods) * S::GROUP));
-                __syncwarp();
-                if (good) bulk_load_1d(dst, A.kv.group(page, w.h, place), S::GROUP, raw_full(st));
-            }
-        }
-        // no copy may be in flight when the block ends (they are not, unless a wait has run out)
-        for (int j = max(0, jj - 2); j < jj; ++j) mbar_wait(raw_full(j & 1), (j >> 1) & 1, never);
-    } else if (warp == AP_MMA) {
-        // ------------------------------------------------------------ products
-        if (lane == 0) {
-            const uint32_t idesc_s = umma_idesc_f16(0, 128, KT);
-            const uint32_t idesc_o = umma_idesc_f16(0, 128, D) | (1u << 16);             // B is MN-major
-            auto scores = [&](int t) {
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t da = umma_desc_k_sw128(sb + S::Q + (t * S::PANELS + k / 4) * S::Q_PANEL) + 2 * (k & 3);
-                    const uint64_t db = umma_desc_k_sw128(sb + S::K + (k / 4) * S::PANEL) + 2 * (k & 3);
-                    umma_f16(tmem + S::S_COL + t * 128, da, db, idesc_s, k > 0);
-                }
-                umma_commit(s_full(t));
-            };
-            int jj = 0, count[2] = {0, 0}, done[2] = {0, 0};         // key tiles; score tiles and items of either row tile
+    if (warp >= AP_MMA) {
+        ap_regs_down<AP_REGS_OTHER>();
+        if (warp == AP_LOAD) {
+            // -------------------------------------------------------- codes
+            int jj = 0;
             for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
                 Item w;
                 if (!w.get(A, item, blocks)) continue;
-                if (w.nk == 0) continue;
-                bool ok = false;
-                do {
-                    AP_WAIT(k_full, jj & 1, 413);
-                    AP_WAIT(q_full(0), done[0] & 1, 412);
-                    ++done[0];
-                    tc_fence_after();
-                    scores(0);
-                    if (w.tiles == 2) {
-                        AP_WAIT(q_full(1), done[1] & 1, 412);
-                        ++done[1];
-                        tc_fence_after();
-                        scores(1);
-                    }
-                    umma_commit(k_empty);
-                    ok = true;
-                } while (false);
-                for (int j = 0; j < w.nk && ok; ++j, ++jj) {
-#pragma unroll
-                    for (int t = 0; t < TILES; ++t) {
-                        if (t >= w.tiles) break;
-                        ok = false;
-                        AP_WAIT(p_full(t), count[t] & 1, 414);
-                        ++count[t];
-                        if (t == 0) { AP_WAIT(v_full, jj & 1, 415); }
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < KT / 16; ++k)
-                            umma_f16_tmem_a(tmem + S::O_COL + t * D, tmem + S::S_COL + t * 128 + k * 8,
-                                            ap_desc_mn(sb + S::V + k * 16 * 128, S::PANEL), idesc_o, j > 0 || k > 0);
-                        umma_commit(o_done(t));
-                        if (t == w.tiles - 1) umma_commit(v_empty);
-                        if (j + 1 < w.nk) {
-                            if (t == 0) { AP_WAIT(k_full, (jj + 1) & 1, 416); tc_fence_after(); }
-                            scores(t);                               // over P: the MMAs run in the order of their issue
-                            if (t == w.tiles - 1) umma_commit(k_empty);
+                for (int j = 0; j < w.nk; ++j, ++jj) {
+                    const int st = jj & 1;
+                    AP_WAIT(raw_empty(st), ((jj >> 1) & 1) ^ 1, 411);
+                    const int place = w.start + j * KT + lane * KV4_GROUP;
+                    const bool want = lane < KT / KV4_GROUP && place < w.hi;
+                    int page = -1;
+                    if (want) page = __ldg(A.sq.table + (int64_t)w.b * A.sq.table_ld + (place >> A.kv.page_shift));
+                    const bool good = want && page >= 0 && page < A.kv.num_pages;
+                    const uint32_t dst = sb + S::RAW + st * S::CODES + lane * S::GROUP;
+                    if (want && !good) {
+                        // a page outside the cache: its keys are NaN
+                        atomicExch(&g_attn4_prompt_status, KV4_BAD_PAGE);
+                        for (int i = 0; i < KV4_GROUP * NB; ++i) {
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + SOFF + 2 * i), "h"((uint16_t)0x7fff) : "memory");
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + HALF + SOFF + 2 * i), "h"((uint16_t)0) : "memory");
                         }
+                    }
+                    const uint32_t goods = __ballot_sync(0xffffffffu, good);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_expect_tx(raw_full(st), (uint32_t)(__popc(goods) * S::GROUP));
+                    __syncwarp();
+                    if (good) bulk_load_1d(dst, A.kv.group(page, w.h, place), S::GROUP, raw_full(st));
+                }
+            }
+            // no copy may be in flight when the block ends (they are not, unless a wait has run out)
+            for (int j = max(0, jj - 2); j < jj; ++j) mbar_wait(raw_full(j & 1), (j >> 1) & 1, never);
+        } else if (warp >= AP_Q) {
+            // -------------------------------------------------------- q: 16 bytes per lane, LPR lanes a row
+            // Straight into the swizzled panels by asynchronous copies, all of a lane's under way at once (the rows were asked
+            // of L2 before); a bf16 row is then turned into fp16 where it lies, by the lanes that brought it.
+            constexpr int LPR = D / 8, ROWS = 32 / LPR, STEPS = 64 / ROWS;
+            const uint32_t negate = A.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale goes into q: maxima stay maxima
+            const int k = lane % LPR;
+            int count[2] = {0, 0};
+            for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
+                Item w;
+                if (!w.get(A, item, blocks) || w.nk == 0) continue;
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (t >= w.tiles) break;
+                    auto place = [&](int s, int &rr, bool &live) -> const void * {   // row and source of step s
+                        rr = (warp - AP_Q) * 64 + s * ROWS + lane / LPR;
+                        const int r = w.r0 + t * 128 + rr, i = r / A.group;
+                        live = r < w.rows;
+                        return reinterpret_cast<const T *>(A.q) + (int64_t)(w.row0 + i) * A.q_ts + (int64_t)(w.h * A.group + (r - i * A.group)) * A.q_hs + k * 8;
+                    };
+                    auto dest = [&](int rr) { return sb + S::Q + (t * S::PANELS + k / 8) * S::Q_PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4); };
+                    int rr; bool live;
+#pragma unroll 4
+                    for (int s = 0; s < STEPS; ++s) {
+                        const void *src = place(s, rr, live);
+                        if (live) asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+                    }
+                    AP_WAIT(q_empty(t), (count[t] & 1) ^ 1, 423);
+#pragma unroll 4
+                    for (int s = 0; s < STEPS; ++s) {
+                        const void *src = place(s, rr, live);
+                        if (live) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dest(rr)), "l"(src) : "memory");
+                        else asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dest(rr)), "r"(0u) : "memory");
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    if (BF || negate != 0) {
+#pragma unroll 4
+                        for (int s = 0; s < STEPS; ++s) {
+                            place(s, rr, live);
+                            const uint32_t at = dest(rr);
+                            uint4 x;
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at));
+                            float down = 1.0f;
+                            if constexpr (BF) {                      // a row's largest comes to [1, 2)
+                                auto two = [](uint32_t v) { return max(v & 0x7fffu, (v >> 16) & 0x7fffu); };
+                                uint32_t mx = max(max(two(x.x), two(x.y)), max(two(x.z), two(x.w)));
+#pragma unroll
+                                for (int o = 1; o < LPR; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                                const int e = max(1, min(253, (int)(mx >> 7)));
+                                down = __int_as_float((254 - e) << 23);
+                                if (k == 0) q_exp[(count[t] & 1) * (TILES * 128) + t * 128 + rr] = (uint8_t)e;
+                            }
+                            auto cv = [&](uint32_t v) {
+                                v ^= negate;
+                                return BF ? ap_half2(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down) : v;
+                            };
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(cv(x.x)), "r"(cv(x.y)), "r"(cv(x.z)), "r"(cv(x.w)) : "memory");
+                        }
+                    }
+                    ++count[t];
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(q_full(t));
+                }
+            }
+        } else if (elect_one()) {
+            // -------------------------------------------------------- products
+            const uint32_t idesc_s = umma_idesc_f16(0, 128, KT);
+            const uint32_t idesc_o = umma_idesc_f16(0, 128, D) | (1u << 16);             // B is MN-major
+            int slot = 0; uint32_t ring_phase = 0;                   // operand buffer that comes next, in the order K, V, K, V, ...
+            int nq[2] = {0, 0}, np[2] = {0, 0}, ns = 0;              // items begun, score tiles done (by row tile); score tiles begun
+            auto step = [&]() { if (++slot == S::NBUF) { slot = 0; ring_phase ^= 1; } };
+            auto scores = [&](int t, int buf, bool last) {           // S = Q_t K^T into its buffer
+                const int s = TILES == 2 ? t : ns & 1;
+                const uint32_t da = ap_desc_k(sb + S::Q + t * S::PANELS * S::Q_PANEL), db = ap_desc_k(sb + S::RING + buf * S::BUF);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    ap_mma(tmem + S::S_COL + s * S::S_STEP, da + (k / 4) * (S::Q_PANEL >> 4) + 2 * (k & 3), db + (k / 4) * (S::PANEL >> 4) + 2 * (k & 3), idesc_s, k > 0);
+                umma_commit(s_full(s));
+                if (last) umma_commit(q_empty(t));                   // the item's last products with q
+                ++ns;
+            };
+            auto values = [&](int t, int s, int buf, bool first) {   // O_t (+)= P V
+                const uint32_t db = ap_desc_mn(sb + S::RING + buf * S::BUF, S::PANEL);
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k)
+                    ap_mma_tmem(tmem + S::O_COL + t * D, tmem + S::S_COL + s * S::S_STEP + k * 8, db + k * (16 * 128 >> 4), idesc_o, !first || k > 0);
+                umma_commit(o_done(s));
+            };
+            Item cur, nxt;
+            int item = blockIdx.x;
+            auto fetch = [&](Item &w) -> bool {                      // next item with keys
+                for (; item < items; item += gridDim.x)
+                    if (w.get(A, item, blocks) && w.nk > 0) { item += gridDim.x; return true; }
+                return false;
+            };
+            bool more = fetch(nxt), ok = true, begun = false;
+            // the first scores of `nxt` for row tile t
+            auto begin = [&](int t) -> bool {
+                do {
+                    AP_WAIT(q_full(t), nq[t] & 1, 412);
+                    if (t == 0) { AP_WAIT(buf_full(slot), ring_phase, 413); }
+                    ++nq[t];
+                    tc_fence_after();
+                    scores(t, slot, nxt.nk == 1);
+                    if (t == nxt.tiles - 1) { umma_commit(buf_empty(slot)); step(); }
+                    return true;
+                } while (false);
+                return false;
+            };
+            while (more && ok) {
+                if (!begun) {
+                    for (int t = 0; t < nxt.tiles && ok; ++t) ok = begin(t);
+                    if (!ok) break;
+                }
+                cur = nxt;
+                more = false;
+                begun = false;
+                for (int j = 0; j < cur.nk && ok; ++j) {
+                    const bool last = j == cur.nk - 1;
+                    if (last) more = fetch(nxt);
+                    if (TILES == 2) {
+                        const int vbuf = slot; const uint32_t vphase = ring_phase;   // V(j); the K after it is next
+                        step();
+                        const int kbuf = slot; const uint32_t kphase = ring_phase;
+                        for (int t = 0; t < 2 && ok; ++t) {
+                            if (t < cur.tiles) {
+                                ok = false;
+                                AP_WAIT(p_full(t), np[t] & 1, 414);
+                                if (t == 0) { AP_WAIT(buf_full(vbuf), vphase, 415); }
+                                ++np[t];
+                                tc_fence_after();
+                                values(t, t, vbuf, j == 0);
+                                if (t == cur.tiles - 1) umma_commit(buf_empty(vbuf));
+                                ok = true;
+                                if (!last) {
+                                    ok = false;
+                                    if (t == 0) { AP_WAIT(buf_full(kbuf), kphase, 416); tc_fence_after(); }
+                                    scores(t, kbuf, j + 2 == cur.nk);   // over P: the MMAs run in the order of their issue
+                                    if (t == cur.tiles - 1) { umma_commit(buf_empty(kbuf)); step(); }
+                                    ok = true;
+                                }
+                            }
+                            if (last && more && t < nxt.tiles) { ok = begin(t); begun = true; }
+                        }
+                    } else {
+                        // S has two buffers: the next scores go before this tile's products with V
+                        const int s = (ns - 1) & 1, vbuf = slot; const uint32_t vphase = ring_phase;
+                        step();
+                        ok = false;
+                        if (!last) {
+                            AP_WAIT(buf_full(slot), ring_phase, 416);
+                            tc_fence_after();
+                            scores(0, slot, j + 2 == cur.nk);
+                            umma_commit(buf_empty(slot));
+                            step();
+                        }
+                        AP_WAIT(p_full(s), (np[0] >> 1) & 1, 414);
+                        AP_WAIT(buf_full(vbuf), vphase, 415);
+                        ++np[0];
+                        tc_fence_after();
+                        values(0, s, vbuf, j == 0);
+                        umma_commit(buf_empty(vbuf));
                         ok = true;
+                        if (last && more) { ok = begin(0); begun = true; }
                     }
                 }
-                if (!ok) break;
             }
         }
     } else if (warp >= AP_EXPAND) {
+        ap_regs_down<AP_REGS_EXPAND>();
         // ------------------------------------------------------------ operand tiles from codes
         const int w0 = warp - AP_EXPAND;
         constexpr int CH = D / 32;                                   // 32-channel pieces (16 bytes of codes) of a row
-        constexpr int PER = KT * CH / 256;                           // pieces per thread and side
-        constexpr int STEP = 256 / CH;                               // tokens from one piece of a thread to its next
+        constexpr int PER = KT * CH / (AP_EXPANDERS * 32);           // pieces per thread and side
+        constexpr int STEP = AP_EXPANDERS * 32 / CH;                               // tokens from one piece of a thread to its next
         static_assert(STEP % KV4_GROUP == 0, "a thread's pieces have the same place in their groups");
         const uint32_t lut = sb + S::LUT + lane * 4;
         const int tok = (w0 * 32 + lane) / CH, q = lane % CH, panel = q >> 1, half = q & 1;
@@ -281,7 +426,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
         uint32_t col[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) col[i] = panel * S::PANEL + tok * 128 + ((((half << 2) | (i ^ turn)) ^ (tok & 7)) << 4);
-        int jj = 0;
+        int jj = 0, slot = 0; uint32_t ring_phase = 0;
         for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
             Item w;
             if (!w.get(A, item, blocks)) continue;
@@ -303,8 +448,8 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
 #pragma unroll
                         for (int e = 0; e < NB; ++e) {
                             uint16_t x, y;
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at + 2 * e) : "memory");
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(at + HALF + 2 * e) : "memory");
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at + 2 * e));
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(at + HALF + 2 * e));
                             const uint32_t xx = x & 0x7fffu, yy = y & 0x7fffu;
                             mk = max(mk, xx < limit ? xx : 0u);
                             mv = max(mv, yy < limit ? yy : 0u);
@@ -324,28 +469,29 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                 const int ek = exponent(mk), ev = exponent(mv);
                 if (j == 0 || ev > v_cur + 6) v_cur = ev;            // V stays under 2^15
                 const float down_k = __int_as_float((262 - ek) << 23), down_v = __int_as_float((262 - v_cur) << 23);
-                AP_WAIT(k_empty, (jj & 1) ^ 1, 418);
-                if (w0 == 0 && lane == 0) { k_pow[st] = __int_as_float((ek - 8) << 23); v_exp[st] = v_cur; }
 #pragma unroll
                 for (int side = 0; side < 2; ++side) {
-                    if (side == 1) { AP_WAIT(v_empty, (jj & 1) ^ 1, 419); }
-                    const uint32_t tile = sb + (side == 0 ? S::K : S::V);
+                    uint32_t c[PER][4];
+                    uint16_t sbits[PER];
 #pragma unroll
                     for (int it = 0; it < PER; ++it) {
                         const uint32_t src = raw + side * HALF + it * (STEP / KV4_GROUP * S::GROUP);
-                        uint32_t c[4];
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-                                     : "r"(src + src0) : "memory");
-                        uint16_t sbits;
-                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sbits) : "r"(src + sc0) : "memory");
-                        float s = to_f32<T>(*reinterpret_cast<const T *>(&sbits));
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(c[it][0]), "=r"(c[it][1]), "=r"(c[it][2]), "=r"(c[it][3]) : "r"(src + src0));
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sbits[it]) : "r"(src + sc0));
+                    }
+                    AP_WAIT(buf_empty(slot), ring_phase ^ 1, 418);
+                    if (side == 0 && w0 == 0 && lane == 0) { k_pow[jj & 3] = __int_as_float((ek - 8) << 23); v_exp[jj & 3] = v_cur; }
+                    const uint32_t tile = sb + S::RING + slot * S::BUF;
+#pragma unroll
+                    for (int it = 0; it < PER; ++it) {
+                        float s = to_f32<T>(*reinterpret_cast<const T *>(&sbits[it]));
                         if (side == 0) {
                             s *= down_k;
                             if (odd) {                               // it has to reach the rows that see it and no others: through its key
 #pragma unroll
                                 for (int e = 0; e < NB; ++e) {
                                     uint16_t y;
-                                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(src + sc0 - 2 * (q * 32 / BS) + HALF + 2 * e) : "memory");
+                                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(raw + it * (STEP / KV4_GROUP * S::GROUP) + sc0 - 2 * (q * 32 / BS) + HALF + 2 * e));
                                     if ((y & INF) == INF) s = __int_as_float(0x7fc00000);
                                 }
                             }
@@ -353,177 +499,160 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                             s *= down_v;
                             const int place = place0 + tok + it * STEP;
                             if (part && (place < w.lo || place >= w.hi)) s = 0.0f;
-                            if (odd && (sbits & INF) == INF) s = 0.0f;
+                            if (odd && (sbits[it] & INF) == INF) s = 0.0f;
                         }
                         const __half2 s2 = __float2half2_rn(s);
-                        if (turn & 1) { uint32_t x = c[0]; c[0] = c[1]; c[1] = x; x = c[2]; c[2] = c[3]; c[3] = x; }
-                        if (turn & 2) { uint32_t x = c[0]; c[0] = c[2]; c[2] = x; x = c[1]; c[1] = c[3]; c[3] = x; }
+                        if (turn & 1) { uint32_t x = c[it][0]; c[it][0] = c[it][1]; c[it][1] = x; x = c[it][2]; c[it][2] = c[it][3]; c[it][3] = x; }
+                        if (turn & 2) { uint32_t x = c[it][0]; c[it][0] = c[it][2]; c[it][2] = x; x = c[it][1]; c[it][1] = c[it][3]; c[it][3] = x; }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             uint32_t o[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const uint32_t p = ap_lut(lut, c[i], e);
+                                const uint32_t p = ap_lut(lut, c[it][i], e);
                                 const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&p), s2);
                                 o[e] = *reinterpret_cast<const uint32_t *>(&y);
                             }
                             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(tile + col[i] + it * (STEP * 128)),
-                                         "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                                         "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]));
                         }
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(side == 0 ? k_full : v_full);
+                        mbar_arrive(buf_full(slot));
                         if (side == 1) mbar_arrive(raw_empty(st));
                     }
+                    if (++slot == S::NBUF) { slot = 0; ring_phase ^= 1; }
                 }
                 if (*abort_flag) break;
             }
         }
-    } else if (warp < 4 * TILES) {
+    } else {
+        if (warp < 4 * TILES) ap_regs_up<AP_REGS_SOFTMAX>();
         // ------------------------------------------------------------ softmax: one row per thread
         const int t = warp >> 2, rr = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + S::S_COL + t * 128 + lanes, t_o = tmem + S::O_COL + t * D + lanes;
-        const uint32_t negate = A.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale goes into q: maxima stay maxima
-        int jj = 0, count = 0;
+        const uint32_t t_o = tmem + S::O_COL + t * D + lanes;
+        int jj = 0, count = 0, nq = 0;                               // key tiles; score tiles and items of this row tile
         bool ok = true;
-        for (int item = blockIdx.x; item < items && ok && !*abort_flag; item += gridDim.x) {
+        for (int item = blockIdx.x; warp < 4 * TILES && item < items && ok && !*abort_flag; item += gridDim.x) {
             Item w;
             if (!w.get(A, item, blocks)) continue;
             if (t >= w.tiles) { jj += w.nk; continue; }
-            const int r = w.r0 + threadIdx.x, i = r / A.group, g = r - i * A.group;
+            const int r = w.r0 + t * 128 + rr, i = r / A.group, g = r - i * A.group;
             const bool live = r < w.rows;
-            float f = fabsf(A.scale_log2) * attn4_code_unscale(A.quant_type);   // score -> power of two
-            if (w.nk > 0) {                                          // (an item without keys has no products: q is not announced)
-                const T *src = reinterpret_cast<const T *>(A.q) + (int64_t)(w.row0 + i) * A.q_ts + (int64_t)(w.h * A.group + g) * A.q_hs;
-                uint4 x[D / 8];
-#pragma unroll
-                for (int k = 0; k < D / 8; ++k) {
-                    x[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (live) x[k] = __ldg(reinterpret_cast<const uint4 *>(src) + k);
-                }
-                float down = 1.0f;
-                if constexpr (BF) {
-                    uint32_t mx = 0;
-                    auto upd = [&](uint32_t y) { mx = max(mx, max(y & 0x7fffu, (y >> 16) & 0x7fffu)); };
-#pragma unroll
-                    for (int k = 0; k < D / 8; ++k) { upd(x[k].x); upd(x[k].y); upd(x[k].z); upd(x[k].w); }
-                    const int e = max(1, min(253, (int)(mx >> 7)));
-                    down = __int_as_float((254 - e) << 23);
-                    f *= __int_as_float(e << 23);
-                }
-                auto cv = [&](uint32_t y) {
-                    y ^= negate;
-                    return BF ? ap_half2(__uint_as_float(y << 16) * down, __uint_as_float(y & 0xffff0000u) * down) : y;
-                };
-#pragma unroll
-                for (int k = 0; k < D / 8; ++k) {
-                    const uint32_t dst = sb + S::Q + (t * S::PANELS + k / 8) * S::Q_PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(cv(x[k].x)), "r"(cv(x[k].y)), "r"(cv(x[k].z)), "r"(cv(x[k].w)) : "memory");
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full(t));
-            }
             const int lim = live ? (A.causal ? w.first + i + 1 : w.len) : 0, low = A.window > 0 ? lim - A.window : 0;
             // keys that every row of this warp sees: [wh, wl)
             const int wl = __reduce_min_sync(0xffffffffu, live ? lim : 0x7fffffff), wh = __reduce_max_sync(0xffffffffu, live ? low : 0);
-            float m = ATTN4_NONE;
+            float m = ATTN4_NONE, f = fabsf(A.scale_log2) * attn4_code_unscale(A.quant_type);   // f: score -> power of two
             uint64_t l2 = 0;                                         // two partial sums
             int ve = 0;
             for (int j = 0; j < w.nk; ++j, ++jj, ++count) {
                 ok = false;
-                AP_WAIT(s_full(t), count & 1, 420);
+                const int s = TILES == 2 ? t : count & 1;
+                const uint32_t t_s = tmem + S::S_COL + s * S::S_STEP + lanes;
+                AP_WAIT(s_full(s), (TILES == 2 ? count : count >> 1) & 1, 420);
                 tc_fence_after();
+                if (BF && j == 0) f *= __int_as_float((int)q_exp[(nq & 1) * (TILES * 128) + t * 128 + rr] << 23);   // (q was there before its products)
                 const int place0 = w.start + j * KT;
-                const float fj = f * k_pow[jj & 1];
-                const int vn = v_exp[jj & 1];
-                bool bad = false;
-                // MASKED: some row of the warp does not see some key of the tile
-                auto tile = [&](auto MASKED) {
-                    auto hidden = [&](int c) { const int place = place0 + c; return !(place < lim && place >= low); };
-                    uint32_t v[32];
-                    float mx = __int_as_float(0xff800000);
+                const float fj = fmaxf(f * k_pow[jj & 3], 0x1p-126f);        // scale 0: -inf * fj has to stay -inf
+                const int vn = v_exp[jj & 3];
+                const bool part = place0 < wh || place0 + KT > wl;   // some row of the warp does not see some key of the tile
+                const int seen_lo = low - place0, seen_hi = lim - place0;
+                auto load = [&](uint32_t (&v)[32], int c0) { tmem_ld_32x32(t_s + c0, v); };
+                auto mask = [&](uint32_t (&v)[32], int c0) {
+                    if (part) {
 #pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += 32) {
-                        tmem_ld_32x32(t_s + c0, v);
-                        tmem_ld_wait();
-                        float a0 = mx, a1 = mx;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            if (MASKED) {
-#pragma unroll
-                                for (int x = 0; x < 4; ++x) if (hidden(c0 + e + x)) v[e + x] = 0xff800000u;
-                            }
-                            a0 = fmaxf(a0, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                            a1 = fmaxf(a1, fmaxf(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])));
-                        }
-                        mx = fmaxf(a0, a1);
-                    }
-                    mx = mx == __int_as_float(0xff800000) ? ATTN4_NONE : mx * fj;
-                    float k = 1.0f;
-                    if (mx > m + 8.0f) {
-                        k = ex2(m - mx);
-                        m = mx;
-                        float x, y;
-                        ap_unpack2(l2, x, y);
-                        l2 = ap_pack2(__float_as_uint(x * k), __float_as_uint(y * k));
-                    }
-                    if (j > 0) {
-                        if (vn != ve) k *= __int_as_float(max(0, 127 + ve - vn) << 23);
-                        if (__any_sync(0xffffffffu, k != 1.0f)) {
-                            if (!mbar_wait(o_done(t), (count - 1) & 1, abort_flag)) { atomicExch(&g_attn4_prompt_status, 421); *abort_flag = 1; bad = true; return; }
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int c0 = 0; c0 < D; c0 += 32) {
-                                tmem_ld_32x32(t_o + c0, v);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * k);
-                                tmem_st_32x32(t_o + c0, v);
-                            }
-                            tmem_st_wait();
-                        }
-                    }
-                    ve = vn;
-                    const uint64_t f2 = ap_pack2(__float_as_uint(fj), __float_as_uint(fj));
-                    const uint64_t b2 = ap_pack2(__float_as_uint(AP_LIFT - m), __float_as_uint(AP_LIFT - m));
-#pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += 32) {
-                        uint32_t p[16];
-                        tmem_ld_32x32(t_s + c0, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float x, y;
-                            ap_unpack2(ap_fma2(ap_pack2(v[2 * e], v[2 * e + 1]), f2, b2), x, y);
-                            if (MASKED) {
-                                if (hidden(c0 + 2 * e)) x = __int_as_float(0xff800000);
-                                if (hidden(c0 + 2 * e + 1)) y = __int_as_float(0xff800000);
-                            }
-                            x = ex2(x);
-                            y = ex2(y);
-                            l2 = ap_add2(l2, ap_pack2(__float_as_uint(x), __float_as_uint(y)));
-                            p[e] = ap_half2(x, y);
-                        }
-                        ap_tmem_st16(t_s + c0 / 2, p);               // over columns of S that have been read
+                        for (int e = 0; e < 32; ++e) if (c0 + e < seen_lo || c0 + e >= seen_hi) v[e] = 0xff800000u;
                     }
                 };
-                if (place0 < wh || place0 + KT > wl) tile(std::true_type{});
-                else tile(std::false_type{});
-                if (bad) break;
+                float a0 = __int_as_float(0xff800000), a1 = a0;
+                auto maximum = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        a0 = fmaxf(a0, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                        a1 = fmaxf(a1, fmaxf(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])));
+                    }
+                };
+                // the first 64 columns are read twice (for the maximum, for P), the others kept
+                uint32_t u[2][32], v[2][32];
+                if constexpr (KT == 128) {
+                    load(u[0], 0); load(u[1], 32);
+                    tmem_ld_wait();
+                    mask(u[0], 0); mask(u[1], 32);
+                    maximum(u[0]); maximum(u[1]);
+                }
+                load(v[0], KT - 64); load(v[1], KT - 32);
+                tmem_ld_wait();
+                mask(v[0], KT - 64); mask(v[1], KT - 32);
+                maximum(v[0]); maximum(v[1]);
+                a0 = fmaxf(a0, a1);
+                const float top = a0 == __int_as_float(0xff800000) ? ATTN4_NONE : a0 * fj;
+                float k = 1.0f;
+                if (top > m + 8.0f) { k = ex2(m - top); m = top; }
+                const uint64_t f2 = ap_pack2(__float_as_uint(fj), __float_as_uint(fj));
+                const uint64_t b2 = ap_pack2(__float_as_uint(AP_LIFT - m), __float_as_uint(AP_LIFT - m));
+                uint64_t add = 0;
+                auto powers = [&](const uint32_t (&x)[32], uint32_t (&p)[16]) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float y, z;
+                        ap_unpack2(ap_fma2(ap_pack2(x[2 * e], x[2 * e + 1]), f2, b2), y, z);
+                        y = ex2(y);
+                        z = ex2(z);
+                        add = ap_add2(add, ap_pack2(__float_as_uint(y), __float_as_uint(z)));
+                        p[e] = ap_half2(y, z);
+                    }
+                };
+                uint32_t p0[16], p1[16];
+                powers(v[0], p0); powers(v[1], p1);
+                if constexpr (KT == 128) {
+                    uint32_t p2[16];
+                    load(u[0], 0); load(u[1], 32);
+                    tmem_ld_wait();
+                    mask(u[0], 0); powers(u[0], p2);
+                    ap_tmem_st16(t_s, p2);                           // P, over S
+                    mask(u[1], 32); powers(u[1], p2);
+                    ap_tmem_st16(t_s + 16, p2);
+                }
+                ap_tmem_st16(t_s + (KT - 64) / 2, p0);
+                ap_tmem_st16(t_s + (KT - 32) / 2, p1);
+                {
+                    float x, y, ax, ay;
+                    ap_unpack2(l2, x, y);
+                    ap_unpack2(add, ax, ay);
+                    l2 = ap_pack2(__float_as_uint(fmaf(x, k, ax)), __float_as_uint(fmaf(y, k, ay)));
+                }
+                if (j > 0) {
+                    if (vn != ve) k *= __int_as_float(max(0, 127 + ve - vn) << 23);
+                    if (__any_sync(0xffffffffu, k != 1.0f)) {
+                        AP_WAIT(o_done(TILES == 2 ? t : s ^ 1), (TILES == 2 ? count - 1 : (count - 1) >> 1) & 1, 421);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c0 = 0; c0 < D; c0 += 16) {
+                            uint32_t x[16];
+                            ap_tmem_ld16(t_o + c0, x);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * k);
+                            ap_tmem_st16(t_o + c0, x);
+                        }
+                    }
+                }
+                ve = vn;
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(t));
+                if (lane == 0) mbar_arrive(p_full(s));
                 ok = true;
             }
             if (!ok) break;
             if (w.nk > 0) {
+                ++nq;
                 ok = false;
-                AP_WAIT(o_done(t), (count - 1) & 1, 422);
+                // (with one row tile the products may be two tiles behind the scores: hence a barrier for each buffer)
+                AP_WAIT(o_done(TILES == 2 ? t : (count - 1) & 1), (TILES == 2 ? count - 1 : (count - 1) >> 1) & 1, 422);
                 ok = true;
                 tc_fence_after();
             }
@@ -571,12 +700,16 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
 template <int D, int BS, typename T>
 static int ap_launch(const Attn4Args &a, cudaStream_t st) {
     using S = ApSmem<D, BS>;
-    constexpr int smem = S::TOTAL + 1024;
+    constexpr int smem = S::TOTAL;
+    static_assert(smem <= 227 * 1024, "shared memory of the prompt kernel");
     static bool configured[64] = {};
     int dev = 0;
     MPSBNB_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
         MPSBNB_CUDA_TRY(cudaFuncSetAttribute(attn4_prompt_kernel<D, BS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        cudaFuncAttributes at;
+        MPSBNB_CUDA_TRY(cudaFuncGetAttributes(&at, attn4_prompt_kernel<D, BS, T>));
+        if (at.numRegs != AP_REGS) return MPSBNB_ERR_UNSUPPORTED;    // the warpgroups' shares are made for this number
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     const int64_t bh = (int64_t)a.sq.batch * a.kv.kv_heads, blocks = ((int64_t)a.sq.new_tokens * a.group + S::TILES * 128 - 1) / (S::TILES * 128);
