@@ -10,14 +10,14 @@
 //   warps 0-3, 4-7  softmax of tile A / B, one row per thread: S from tensor memory, P back over S as fp16, the row's sum
 //                   in fp32.  The reference m follows the maximum only when that exceeds it by more than 2^8; O stays in
 //                   tensor memory and is rescaled only then.
-//   warps 8-11      expand a tile of KT keys: byte -> fp16 pair by a table held once per lane, times the block's absmax,
+//   warps 8-15      expand a tile of KT keys: byte -> fp16 pair by a table held once per lane, times the block's absmax,
 //                   into 128-byte-swizzled panels [KT][64 channels].  For K that is the K-major operand of S = Q K^T,
 //                   for V - the same layout read the other way - the MN-major operand of O = P V.  K and V take turns in
 //                   a ring of three buffers, so expanding runs ahead of the products.
-//   warp 12         issues the MMAs: S_A, S_B, then per key tile O_A += P_A V, S_A(next), O_B += P_B V, S_B(next), on
+//   warp 16         issues the MMAs: S_A, S_B, then per key tile O_A += P_A V, S_A(next), O_B += P_B V, S_B(next), on
 //                   into the next block of rows without a pause.
-//   warp 13         fetches the codes: one bulk copy per group of 16 tokens, two tiles ahead.
-//   warps 14, 15    bring the next rows of q as soon as the last products with the present ones have been issued.
+//   warp 17         fetches the codes: one bulk copy per group of 16 tokens, two tiles ahead.
+//   warps 18, 19    bring the next rows of q as soon as the last products with the present ones have been issued.
 // fp16 operands hold bf16 caches too: the absmax of a K tile (and, carried along, of the V tiles) is brought near 2^8 by
 // a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.
 #include <type_traits>
@@ -34,12 +34,12 @@ static __device__ int g_attn4_prompt_status = 0;
 // P is 2^(x - m + 7): at most 2^15 while the reference m lags by 2^8, and what lies 2^21 below the reference still has
 // fp16's full precision.
 constexpr float AP_LIFT = 7.0f;
-constexpr int AP_EXPAND = 8, AP_EXPANDERS = 4;                       // first expander warp, their number
-constexpr int AP_MMA = 12, AP_LOAD = 13, AP_Q = 14, AP_THREADS = 16 * 32;
-// Registers: launched with 128 a thread (512 threads: all of the SM's); the warpgroups then share them out anew.  (A spilled
-// register costs a trip to L2 here: shared memory leaves next to nothing of L1.)
-constexpr int AP_REGS = 128, AP_REGS_SOFTMAX = 160, AP_REGS_EXPAND = 112, AP_REGS_OTHER = 80;
-static_assert(2 * AP_REGS_SOFTMAX + AP_REGS_EXPAND + AP_REGS_OTHER <= 4 * AP_REGS, "a raise beyond the launch's registers would wait for ever");
+constexpr int AP_EXPAND = 8, AP_EXPANDERS = 8;                       // first expander warp, their number
+constexpr int AP_MMA = 16, AP_LOAD = 17, AP_Q = 18, AP_THREADS = 20 * 32;
+// Registers: launched with 96 a thread (640 threads); the warpgroups then share them out anew.  (A spilled register costs a
+// trip to L2 here: shared memory leaves next to nothing of L1.)
+constexpr int AP_REGS = 96, AP_REGS_SOFTMAX = 128, AP_REGS_EXPAND = 72, AP_REGS_OTHER = 80;
+static_assert(2 * AP_REGS_SOFTMAX + 2 * AP_REGS_EXPAND + AP_REGS_OTHER <= 5 * AP_REGS, "a raise beyond the launch's registers would wait for ever");
 template <int N> __device__ __forceinline__ void ap_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void ap_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
@@ -106,6 +106,7 @@ __device__ __forceinline__ uint32_t ap_lut(uint32_t lut_lane, uint32_t word, int
     asm("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(__byte_perm(word, 0u, 0x4440 | byte) * 128u + lut_lane));
     return v;
 }
+__device__ __forceinline__ float ap_max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 __device__ __forceinline__ uint64_t ap_pack2(uint32_t lo, uint32_t hi) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi)); return r; }
 __device__ __forceinline__ void ap_unpack2(uint64_t x, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
 __device__ __forceinline__ uint64_t ap_fma2(uint64_t a, uint64_t b, uint64_t c) {
@@ -438,29 +439,52 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                 const bool part = place0 < w.lo || place0 + KT > w.hi;
                 // largest absmax of the tile's keys and values (bits of a 16-bit type; an infinity or a NaN is the largest)
                 uint32_t mk = 0, mv = 0;
-                auto scan = [&](uint32_t limit) {
-                    mk = mv = 0;
+                {
+                    uint32_t k2 = 0, v2 = 0;                         // two at a time
 #pragma unroll
                     for (int i = 0; i < KT / 32; ++i) {
                         const int t = lane + 32 * i;
                         if (part && (place0 + t < w.lo || place0 + t >= w.hi)) continue;
                         const uint32_t at = raw + (t >> 4) * S::GROUP + SOFF + (t & 15) * (2 * NB);
 #pragma unroll
+                        for (int e = 0; e < (NB + 1) / 2; ++e) {
+                            uint32_t x, y;
+                            if constexpr (NB == 1) {
+                                uint16_t x1, y1;
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x1) : "r"(at));
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y1) : "r"(at + HALF));
+                                x = x1; y = y1;
+                            } else {
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at + 4 * e));
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(y) : "r"(at + HALF + 4 * e));
+                            }
+                            k2 = __vmaxu2(k2, x & 0x7fff7fffu);
+                            v2 = __vmaxu2(v2, y & 0x7fff7fffu);
+                        }
+                    }
+                    mk = __reduce_max_sync(0xffffffffu, max(k2 & 0xffffu, k2 >> 16));
+                    mv = __reduce_max_sync(0xffffffffu, max(v2 & 0xffffu, v2 >> 16));
+                }
+                const bool odd = mv >= INF;                          // some value is not finite
+                if (mk >= INF || odd) {                              // the largest of those that are
+                    mk = mv = 0;
+#pragma unroll 1
+                    for (int t = lane; t < KT; t += 32) {
+                        if (part && (place0 + t < w.lo || place0 + t >= w.hi)) continue;
+                        const uint32_t at = raw + (t >> 4) * S::GROUP + SOFF + (t & 15) * (2 * NB);
+#pragma unroll 1
                         for (int e = 0; e < NB; ++e) {
                             uint16_t x, y;
                             asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at + 2 * e));
                             asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(at + HALF + 2 * e));
                             const uint32_t xx = x & 0x7fffu, yy = y & 0x7fffu;
-                            mk = max(mk, xx < limit ? xx : 0u);
-                            mv = max(mv, yy < limit ? yy : 0u);
+                            mk = max(mk, xx < INF ? xx : 0u);
+                            mv = max(mv, yy < INF ? yy : 0u);
                         }
                     }
                     mk = __reduce_max_sync(0xffffffffu, mk);
                     mv = __reduce_max_sync(0xffffffffu, mv);
-                };
-                scan(0x8000u);
-                const bool odd = mv >= INF;                          // some value is not finite
-                if (mk >= INF || odd) scan(INF);
+                }
                 auto exponent = [&](uint32_t bits) -> int {
                     const uint16_t x = (uint16_t)bits;
                     const int e = (int)(__float_as_uint(to_f32<T>(*reinterpret_cast<const T *>(&x))) >> 23);
@@ -528,15 +552,17 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                 if (*abort_flag) break;
             }
         }
+    } else if (TILES == 1 && warp >= 4) {
+        ap_regs_down<AP_REGS_OTHER>();                               // (no second row tile)
     } else {
-        if (warp < 4 * TILES) ap_regs_up<AP_REGS_SOFTMAX>();
+        ap_regs_up<AP_REGS_SOFTMAX>();
         // ------------------------------------------------------------ softmax: one row per thread
         const int t = warp >> 2, rr = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_o = tmem + S::O_COL + t * D + lanes;
         int jj = 0, count = 0, nq = 0;                               // key tiles; score tiles and items of this row tile
         bool ok = true;
-        for (int item = blockIdx.x; warp < 4 * TILES && item < items && ok && !*abort_flag; item += gridDim.x) {
+        for (int item = blockIdx.x; item < items && ok && !*abort_flag; item += gridDim.x) {
             Item w;
             if (!w.get(A, item, blocks)) continue;
             if (t >= w.tiles) { jj += w.nk; continue; }
@@ -571,8 +597,8 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                 auto maximum = [&](const uint32_t (&v)[32]) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
-                        a0 = fmaxf(a0, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                        a1 = fmaxf(a1, fmaxf(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])));
+                        a0 = ap_max3(a0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                        a1 = ap_max3(a1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
                     }
                 };
                 // the first 64 columns are read twice (for the maximum, for P), the others kept
@@ -608,13 +634,15 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                 uint32_t p0[16], p1[16];
                 powers(v[0], p0); powers(v[1], p1);
                 if constexpr (KT == 128) {
-                    uint32_t p2[16];
-                    load(u[0], 0); load(u[1], 32);
-                    tmem_ld_wait();
-                    mask(u[0], 0); powers(u[0], p2);
-                    ap_tmem_st16(t_s, p2);                           // P, over S
-                    mask(u[1], 32); powers(u[1], p2);
-                    ap_tmem_st16(t_s + 16, p2);
+#pragma unroll
+                    for (int c0 = 0; c0 < 64; c0 += 32) {
+                        uint32_t p2[16];
+                        load(u[0], c0);
+                        tmem_ld_wait();
+                        mask(u[0], c0);
+                        powers(u[0], p2);
+                        ap_tmem_st16(t_s + c0 / 2, p2);              // P, over S
+                    }
                 }
                 ap_tmem_st16(t_s + (KT - 64) / 2, p0);
                 ap_tmem_st16(t_s + (KT - 32) / 2, p1);
@@ -660,7 +688,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
             ap_unpack2(l2, la, lb);
             const float l = la + lb;
             const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l) * __int_as_float(max(1, ve - 8) << 23) * attn4_code_unscale(A.quant_type);
-            const int64_t orow = (int64_t)(w.row0 + i) * A.heads + w.h * A.group + g;
+            const int64_t orow = live ? (int64_t)(w.row0 + i) * A.heads + w.h * A.group + g : -1;
             T *dst = reinterpret_cast<T *>(A.out) + orow * D;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -676,13 +704,13 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                     if (l != 0.0f) { pr[0] = from_f32<T>(__uint_as_float(v[2 * e]) * inv); pr[1] = from_f32<T>(__uint_as_float(v[2 * e + 1]) * inv); }
                     y[e] = *reinterpret_cast<const uint32_t *>(pr);
                 }
-                if (live) {
+                if (orow >= 0) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4 *>(dst + c0 + 8 * e) = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
                 }
             }
             tc_fence_before();                                       // O has been read before the next item's P is announced
-            if (live && A.lse != nullptr) A.lse[orow] = l == 0.0f ? __int_as_float(0xff800000) : (m - AP_LIFT + __log2f(l)) * 0.69314718f;
+            if (orow >= 0 && A.lse != nullptr) A.lse[orow] = l == 0.0f ? __int_as_float(0xff800000) : (m - AP_LIFT + __log2f(l)) * 0.69314718f;
         }
     }
 #undef AP_WAIT
