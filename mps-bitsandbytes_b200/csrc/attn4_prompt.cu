@@ -55,7 +55,7 @@ template <int D, int BS> struct ApSmem {
     static constexpr int RAW = LUT + 256 * 128;
     static constexpr int EXPO = RAW + 2 * CODES;                     // [2][TILES * 128] bytes: exponent that a bf16 row of q was brought down by
     static constexpr int BAR = EXPO + 2 * TILES * 128;
-    static constexpr int TOTAL = BAR + 256;
+    static constexpr int TOTAL = BAR + 336;
     // tensor memory columns
     static constexpr int S_COL = 0, S_STEP = TILES == 2 ? 128 : 64, O_COL = 2 * S_STEP;
     static_assert(O_COL + TILES * D <= 512, "tensor memory");
@@ -126,16 +126,10 @@ template <int TILES, int KT> struct ApItem {
     int tiles;                                                       // 128-row tiles that hold rows
     int lo, hi, start, nk;                                           // keys any row sees: [lo, hi), from place `start` in nk tiles
 
-    // false: no rows
-    __device__ __forceinline__ bool get(const Attn4Args &A, int item, int blocks) {
-        const int bh = A.sq.batch * A.kv.kv_heads;
-        const int blk = item / bh, x = item - blk * bh;
-        b = x / A.kv.kv_heads;
-        h = x - b * A.kv.kv_heads;
-        r0 = (blocks - 1 - blk) * (TILES * 128);                     // rows with many keys first
+    __device__ __forceinline__ void set(const Attn4Args &A, int b_, int h_, int r0_) {
+        b = b_; h = h_; r0 = r0_;
         A.sq.get(b, row0, n, len);
         rows = n * A.group;
-        if (r0 >= rows) return false;
         tiles = TILES == 2 && r0 + 128 < rows ? 2 : 1;
         first = len - n;
         const int i_lo = r0 / A.group, i_hi = min(n - 1, (r0 + TILES * 128 - 1) / A.group);
@@ -143,13 +137,41 @@ template <int TILES, int KT> struct ApItem {
         lo = A.window > 0 ? max(0, first + i_lo + 1 - A.window) : 0;
         start = lo & ~(KV4_GROUP - 1);
         nk = hi > lo ? (hi - start + KT - 1) / KT : 0;
+    }
+};
+
+// The items of a call, blocks of rows from the last of the longest sequence to the first of all: level by level, so that items
+// with many keys come first.  Whole warp.
+template <int STEP> struct ApList {
+    int level, chunk;                                                // block of rows; 32 sequences
+    int64_t before;                                                  // items before this chunk of this level
+    uint32_t has;                                                    // sequences of the chunk that have a block at this level
+    __device__ __forceinline__ void look(const Attn4Args &A) {
+        const int b = chunk * 32 + (threadIdx.x & 31);
+        int row0, n = 0, len;
+        if (b < A.sq.batch) A.sq.get(b, row0, n, len);
+        has = __ballot_sync(0xffffffffu, (int64_t)n * A.group > (int64_t)level * STEP);
+    }
+    __device__ __forceinline__ void begin(const Attn4Args &A, int blocks) { level = blocks - 1; chunk = 0; before = 0; look(A); }
+    // item j, at or behind the one found last; false: there are not so many
+    __device__ __forceinline__ bool find(const Attn4Args &A, int64_t j, int &b, int &h, int &r0) {
+        while (j >= before + __popc(has) * A.kv.kv_heads) {
+            before += __popc(has) * A.kv.kv_heads;
+            if ((++chunk) * 32 >= A.sq.batch) { chunk = 0; --level; }
+            if (level < 0) return false;
+            look(A);
+        }
+        const int off = (int)(j - before), s = off / A.kv.kv_heads;
+        h = off - s * A.kv.kv_heads;
+        b = chunk * 32 + (int)__fns(has, 0, s + 1);
+        r0 = level * STEP;
         return true;
     }
 };
 
 template <int D, int BS, typename T>
 __global__ void __launch_bounds__(AP_THREADS, 1)
-attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) {
+attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
     using S = ApSmem<D, BS>;
     constexpr int TILES = S::TILES, KT = S::KT, NB = D / BS, SOFF = KV4_GROUP * (D / 2), HALF = kv4_half_bytes(D, BS);
     constexpr bool BF = !std::is_same<T, __half>::value;
@@ -175,6 +197,9 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
     volatile float *k_pow = reinterpret_cast<volatile float *>(smem + S::BAR + 176);     // [4]: power of two of a K tile
     volatile int *v_exp = reinterpret_cast<volatile int *>(smem + S::BAR + 192);         // [4]: V's exponent from a tile on
     volatile uint8_t *q_exp = smem + S::EXPO;
+    volatile int *queue = reinterpret_cast<volatile int *>(smem + S::BAR + 208);         // [4][4]: items (sequence, or -1; head; row)
+    auto item_full = [&](int s) { return bar + 272 + 8u * s; };      // [4] each
+    auto item_empty = [&](int s) { return bar + 304 + 8u * s; };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -184,6 +209,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
             mbar_init(s_full(i), 1); mbar_init(p_full(i), 4); mbar_init(o_done(i), 1);
             mbar_init(q_full(i), 2); mbar_init(q_empty(i), 1);
         }
+        for (int i = 0; i < 4; ++i) { mbar_init(item_full(i), 1); mbar_init(item_empty(i), 4 * TILES + AP_EXPANDERS + 3); }   // (the issuer, two q warps)
         *abort_flag = *never = 0;
         fence_mbar_init();
     }
@@ -202,8 +228,21 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    // Every role walks the block's items by itself; what it counts (key tiles, operands, tiles of scores) runs on from item
-    // to item.
+    // The loader finds the block's items - every second time round in the opposite direction, which evens the blocks out - and
+    // queues them for the other roles.  What a role counts (key tiles, operands, tiles of scores) runs on from item to item.
+    int turn_ = 0;                                                   // of the queue
+    // the next item; false: no more.  Whole warp (or the one thread of the issuer)
+    auto next_item = [&](Item &w, bool one) -> bool {
+        const int s = turn_ & 3;
+        if (!mbar_wait(item_full(s), (turn_ >> 2) & 1, abort_flag)) { atomicExch(&g_attn4_prompt_status, 424); *abort_flag = 1; return false; }
+        const int b = queue[4 * s], h = queue[4 * s + 1], r0 = queue[4 * s + 2];
+        if (!one) __syncwarp();
+        if (one || lane == 0) mbar_arrive(item_empty(s));
+        ++turn_;
+        if (b < 0) return false;
+        w.set(A, b, h, r0);
+        return true;
+    };
 #define AP_WAIT(b_, ph_, code_) if (!mbar_wait(b_, ph_, abort_flag)) { atomicExch(&g_attn4_prompt_status, code_); *abort_flag = 1; break; }
 
     if (warp >= AP_MMA) {
@@ -211,9 +250,20 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
         if (warp == AP_LOAD) {
             // -------------------------------------------------------- codes
             int jj = 0;
-            for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
+            ApList<TILES * 128> list;
+            list.begin(A, blocks);
+            for (int turn = 0; !*abort_flag; ++turn) {
+                int b = -1, h = 0, r0 = 0;
+                if (!list.find(A, (int64_t)turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), b, h, r0)) b = -1;
+                const int qs = turn & 3;
+                AP_WAIT(item_empty(qs), ((turn >> 2) & 1) ^ 1, 425);
+                if (lane == 0) {
+                    queue[4 * qs] = b; queue[4 * qs + 1] = h; queue[4 * qs + 2] = r0;
+                    mbar_arrive(item_full(qs));
+                }
+                if (b < 0) break;
                 Item w;
-                if (!w.get(A, item, blocks)) continue;
+                w.set(A, b, h, r0);
                 for (int j = 0; j < w.nk; ++j, ++jj) {
                     const int st = jj & 1;
                     AP_WAIT(raw_empty(st), ((jj >> 1) & 1) ^ 1, 411);
@@ -248,55 +298,62 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
             const uint32_t negate = A.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale goes into q: maxima stay maxima
             const int k = lane % LPR;
             int count[2] = {0, 0};
-            for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
-                Item w;
-                if (!w.get(A, item, blocks) || w.nk == 0) continue;
+            Item w;
+            while (!*abort_flag && next_item(w, false)) {
+                if (w.nk == 0) continue;
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
                     if (t >= w.tiles) break;
-                    auto place = [&](int s, int &rr, bool &live) -> const void * {   // row and source of step s
-                        rr = (warp - AP_Q) * 64 + s * ROWS + lane / LPR;
-                        const int r = w.r0 + t * 128 + rr, i = r / A.group;
-                        live = r < w.rows;
-                        return reinterpret_cast<const T *>(A.q) + (int64_t)(w.row0 + i) * A.q_ts + (int64_t)(w.h * A.group + (r - i * A.group)) * A.q_hs + k * 8;
+                    const int first_rr = (warp - AP_Q) * 64 + lane / LPR, first_r = w.r0 + t * 128 + first_rr;
+                    const int first_i = first_r / A.group, first_g = first_r - first_i * A.group;
+                    // every row of this lane: f(row of the tile, source or nullptr)
+                    auto each = [&](auto f) {
+                        int rr = first_rr, i = first_i, g = first_g;
+#pragma unroll 8
+                        for (int s = 0; s < STEPS; ++s, rr += ROWS) {
+                            f(rr, i < w.n ? reinterpret_cast<const T *>(A.q) + (int64_t)(w.row0 + i) * A.q_ts + (int64_t)(w.h * A.group + g) * A.q_hs + k * 8 : nullptr);
+                            g += ROWS;
+                            while (g >= A.group) { g -= A.group; ++i; }
+                        }
                     };
                     auto dest = [&](int rr) { return sb + S::Q + (t * S::PANELS + k / 8) * S::Q_PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4); };
-                    int rr; bool live;
-#pragma unroll 4
-                    for (int s = 0; s < STEPS; ++s) {
-                        const void *src = place(s, rr, live);
-                        if (live) asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
-                    }
+                    each([&](int, const T *src) { if (src != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(src)); });
                     AP_WAIT(q_empty(t), (count[t] & 1) ^ 1, 423);
-#pragma unroll 4
-                    for (int s = 0; s < STEPS; ++s) {
-                        const void *src = place(s, rr, live);
-                        if (live) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dest(rr)), "l"(src) : "memory");
-                        else asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dest(rr)), "r"(0u) : "memory");
-                    }
+                    each([&](int rr, const T *src) {
+                        if (src != nullptr) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dest(rr)), "l"(src));
+                        else asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dest(rr)), "r"(0u));
+                    });
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     if (BF || negate != 0) {
-#pragma unroll 4
-                        for (int s = 0; s < STEPS; ++s) {
-                            place(s, rr, live);
-                            const uint32_t at = dest(rr);
-                            uint4 x;
-                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at));
-                            float down = 1.0f;
-                            if constexpr (BF) {                      // a row's largest comes to [1, 2)
-                                auto two = [](uint32_t v) { return max(v & 0x7fffu, (v >> 16) & 0x7fffu); };
-                                uint32_t mx = max(max(two(x.x), two(x.y)), max(two(x.z), two(x.w)));
+                        constexpr int FLY = 8;                       // rows worked on side by side
+#pragma unroll 1
+                        for (int s0 = 0; s0 < STEPS; s0 += FLY) {
+                            uint4 x[FLY];
+                            uint32_t mx[FLY];
 #pragma unroll
-                                for (int o = 1; o < LPR; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                                const int e = max(1, min(253, (int)(mx >> 7)));
-                                down = __int_as_float((254 - e) << 23);
-                                if (k == 0) q_exp[(count[t] & 1) * (TILES * 128) + t * 128 + rr] = (uint8_t)e;
+                            for (int y = 0; y < FLY; ++y) {
+                                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[y].x), "=r"(x[y].y), "=r"(x[y].z), "=r"(x[y].w) : "r"(dest(first_rr + (s0 + y) * ROWS)));
+                                // largest magnitude, two halves at a time
+                                const uint32_t m2 = __vmaxu2(__vmaxu2(x[y].x & 0x7fff7fffu, x[y].y & 0x7fff7fffu), __vmaxu2(x[y].z & 0x7fff7fffu, x[y].w & 0x7fff7fffu));
+                                mx[y] = max(m2 & 0xffffu, m2 >> 16);
                             }
-                            auto cv = [&](uint32_t v) {
-                                v ^= negate;
-                                return BF ? ap_half2(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down) : v;
-                            };
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(cv(x.x)), "r"(cv(x.y)), "r"(cv(x.z)), "r"(cv(x.w)) : "memory");
+                            if constexpr (BF) {
+#pragma unroll
+                                for (int o = 1; o < LPR; o <<= 1)
+#pragma unroll
+                                    for (int y = 0; y < FLY; ++y) mx[y] = max(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], o));
+                            }
+#pragma unroll
+                            for (int y = 0; y < FLY; ++y) {
+                                const int rr = first_rr + (s0 + y) * ROWS, e = max(1, min(253, (int)(mx[y] >> 7)));
+                                const float down = __int_as_float((254 - e) << 23);   // a row's largest comes to [1, 2)
+                                if (BF && k == 0) q_exp[(count[t] & 1) * (TILES * 128) + t * 128 + rr] = (uint8_t)e;
+                                auto cv = [&](uint32_t v) {
+                                    v ^= negate;
+                                    return BF ? ap_half2(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down) : v;
+                                };
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dest(rr)), "r"(cv(x[y].x)), "r"(cv(x[y].y)), "r"(cv(x[y].z)), "r"(cv(x[y].w)));
+                            }
                         }
                     }
                     ++count[t];
@@ -330,10 +387,9 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
                 umma_commit(o_done(s));
             };
             Item cur, nxt;
-            int item = blockIdx.x;
             auto fetch = [&](Item &w) -> bool {                      // next item with keys
-                for (; item < items; item += gridDim.x)
-                    if (w.get(A, item, blocks) && w.nk > 0) { item += gridDim.x; return true; }
+                while (next_item(w, true))
+                    if (w.nk > 0) return true;
                 return false;
             };
             bool more = fetch(nxt), ok = true, begun = false;
@@ -428,9 +484,8 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
 #pragma unroll
         for (int i = 0; i < 4; ++i) col[i] = panel * S::PANEL + tok * 128 + ((((half << 2) | (i ^ turn)) ^ (tok & 7)) << 4);
         int jj = 0, slot = 0; uint32_t ring_phase = 0;
-        for (int item = blockIdx.x; item < items && !*abort_flag; item += gridDim.x) {
-            Item w;
-            if (!w.get(A, item, blocks)) continue;
+        Item w;
+        while (!*abort_flag && next_item(w, false)) {
             int v_cur = 0;                                           // exponent (biased) that V is brought down by
             for (int j = 0; j < w.nk; ++j, ++jj) {
                 const int st = jj & 1, place0 = w.start + j * KT;
@@ -562,9 +617,8 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int items, int blocks) 
         const uint32_t t_o = tmem + S::O_COL + t * D + lanes;
         int jj = 0, count = 0, nq = 0;                               // key tiles; score tiles and items of this row tile
         bool ok = true;
-        for (int item = blockIdx.x; item < items && ok && !*abort_flag; item += gridDim.x) {
-            Item w;
-            if (!w.get(A, item, blocks)) continue;
+        Item w;
+        while (ok && !*abort_flag && next_item(w, false)) {
             if (t >= w.tiles) { jj += w.nk; continue; }
             const int r = w.r0 + t * 128 + rr, i = r / A.group, g = r - i * A.group;
             const bool live = r < w.rows;
@@ -740,10 +794,11 @@ static int ap_launch(const Attn4Args &a, cudaStream_t st) {
         if (at.numRegs != AP_REGS) return MPSBNB_ERR_UNSUPPORTED;    // the warpgroups' shares are made for this number
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const int64_t bh = (int64_t)a.sq.batch * a.kv.kv_heads, blocks = ((int64_t)a.sq.new_tokens * a.group + S::TILES * 128 - 1) / (S::TILES * 128);
-    if (bh * blocks > 0x7fffffffll) return MPSBNB_ERR_TOO_LARGE;
-    const int items = (int)(bh * blocks), sms = sm_count();
-    attn4_prompt_kernel<D, BS, T><<<items < sms ? items : sms, AP_THREADS, smem, st>>>(a, items, (int)blocks);
+    const int64_t blocks = ((int64_t)a.sq.new_tokens * a.group + S::TILES * 128 - 1) / (S::TILES * 128);
+    // no more blocks than there can be items: a sequence's last block of rows may be partly filled
+    const int64_t most = a.kv.kv_heads * (((int64_t)a.sq.tokens * a.group) / (S::TILES * 128) + a.sq.batch);
+    const int sms = sm_count();
+    attn4_prompt_kernel<D, BS, T><<<(int)(most < sms ? most : sms), AP_THREADS, smem, st>>>(a, (int)blocks);
     return check_launch();
 }
 
