@@ -690,6 +690,20 @@ attn4_combine_kernel(const __grid_constant__ Attn4Args A, int teams) {
 // 16 rows per tile where 8 do not hold a sequence's rows: the keys are then expanded half as often
 static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return (int64_t)s->new_tokens * group > 8 ? 2 : 1; }
 
+// The tensor-core kernel of attn4_prompt.cu instead?  It takes a (sequence, kv head)'s keys in one block, one round of blocks
+// after the other, and a key tile costs it the same whether its rows are 16 or 256: 2.0, 2.4, 3.3 us per 128 keys (head_dim 64,
+// 128, 256).  The kernel here spreads any amount of work over the whole card, at 0.42, 0.70, 1.83 ns per 16 rows x 16 keys.
+// They meet where the 16-row tiles of all sequences and heads number 700, 430, 225 per round.  (Measured for 1 - 16
+// sequences, 1 - 8 heads, 16 - 2048 rows a head: 8 heads, 8192 keys, head_dim 128: 512 rows 109 us here and 160 there, 1024
+// rows 197 and 160.)
+static bool ad_prompt(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group) {
+    const int64_t rows = (s->tokens * group + s->batch - 1) / s->batch;   // of a sequence and head, on average
+    const int64_t lists = (int64_t)s->batch * c->kv_heads, block = c->head_dim == 256 ? 128 : 256, sms = sm_count();
+    const int64_t rounds = (lists * ((rows + block - 1) / block) + sms - 1) / sms;
+    const int64_t meet = c->head_dim == 64 ? 700 : c->head_dim == 128 ? 430 : 225;
+    return rows > 16 && lists * ((rows + 15) / 16) > meet * rounds;
+}
+
 static int ad_teams(int D, int NT) { return sm_count() * ((D * NT <= 128 ? 12 : 8) / AD_WARPS); }
 
 template <int D, int BS, int NT, typename T>
@@ -742,6 +756,7 @@ extern "C" size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *
     if (kv4_check_cache(cache, 0) != MPSBNB_OK || kv4_check_seqs(seqs, cache) != MPSBNB_OK) return 0;
     if (heads <= 0 || heads % cache->kv_heads != 0 || seqs->batch == 0 || seqs->tokens == 0) return 0;
     const int nt = ad_nt(seqs, heads / cache->kv_heads);
+    if (ad_prompt(cache, seqs, heads / cache->kv_heads)) return 16;   // (not used)
     return (size_t)ad_teams(cache->head_dim, nt) * (2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float) + sizeof(AdJoin));
 }
 
@@ -769,7 +784,7 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.scale_log2 = scale * 1.4426950408889634f;
     static const float codes[2][16] = {MPSBNB_NF4_TABLE, MPSBNB_FP4_TABLE};
     for (int i = 0; i < 16; ++i) a.code[i] = codes[cache->quant_type][i] * attn4_code_scale(cache->quant_type);
-    if ((int64_t)seqs->new_tokens * group >= 128) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, (cudaStream_t)stream);
+    if (ad_prompt(cache, seqs, group)) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, (cudaStream_t)stream);
     const int nt = ad_nt(seqs, group);
     cudaStream_t st = (cudaStream_t)stream;
     const int dt = cache->dtype;

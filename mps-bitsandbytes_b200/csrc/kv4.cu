@@ -8,62 +8,75 @@ namespace mpsbnb {
 
 static __device__ int g_kv4_status = 0;
 
+template <typename T> __device__ __forceinline__ uint32_t pair_of(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pair_of<__half>(float lo, float hi) { const __half2 h = __floats2half2_rn(lo, hi); return *reinterpret_cast<const uint32_t *>(&h); }
+template <> __device__ __forceinline__ uint32_t pair_of<__nv_bfloat16>(float lo, float hi) { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t *>(&h); }
+
 // ------------------------------------------------------------------------------------------
 // Dequantise: out[b, place, h, :] = fl(code * absmax), zeros past the sequence's end.  Bound by the 2 bytes written per
-// element.  A thread owns 16 elements of K and of V (8 bytes of codes in, two 16-byte stores out each); the codebook
-// sits in shared memory once per lane, so a warp's 32 look-ups never meet in a bank.
+// element.  A warp takes a place, finds its page once and goes through the rows of all heads, K first; a lane owns 8 elements
+// (4 bytes of codes in, a 16-byte store out), so that a warp writes 512 consecutive bytes.  The codebook sits in shared memory
+// once per lane: a warp's 32 look-ups never meet in a bank.
 // ------------------------------------------------------------------------------------------
 template <typename T, int BS>
 __global__ void __launch_bounds__(256)
-kv4_dequantize_kernel(const Kv4Layer kv, const Kv4Seqs sq, int quant_type, int head_dim, int max_len, T *__restrict__ k,
+kv4_dequantize_kernel(const Kv4Layer kv, const Kv4Seqs sq, int quant_type, int cpr_shift, int max_len, T *__restrict__ k,
                       T *__restrict__ v) {
     __shared__ float tab[16 * 32];
     for (int i = threadIdx.x; i < 512; i += 256) tab[i] = kCode[quant_type][i >> 5];
     __syncthreads();
     const int lane = threadIdx.x & 31;
-    const int cpr = head_dim / 16;
-    const int64_t total = (int64_t)sq.batch * max_len * kv.kv_heads * cpr;
-    const int64_t stride = (int64_t)gridDim.x * 256;
-    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < total; c += stride) {
-        const int64_t r = c / cpr;
-        const int kc = (int)(c - r * cpr);
-        const int64_t bp = r / kv.kv_heads;
-        const int h = (int)(r - bp * kv.kv_heads);
-        const int b = (int)(bp / max_len), place = (int)(bp - (int64_t)b * max_len);
+    const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(tab) + lane * 4u;
+    // a row is cpr chunks of 8 elements (8, 16 or 32 lanes); the warp goes on by `step` rows, K's before V's
+    const int cpr = 1 << cpr_shift, step = 32 >> cpr_shift, kc = lane & (cpr - 1), rl = lane >> cpr_shift;
+    const int head_bytes = (1 << (kv.page_shift - 4)) * kv.group_bytes;
+    const int64_t places = (int64_t)sq.batch * max_len;
+    constexpr int U = 4;
+    for (int64_t bp = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); bp < places; bp += (int64_t)gridDim.x * 8) {
+        const int b = (int)(bp < 0x7fffffff ? (uint32_t)bp / (uint32_t)max_len : bp / max_len), place = (int)(bp - (int64_t)b * max_len);
         const int len = min(max(__ldg(sq.lens + b), 0), sq.capacity);
-        uint2 kw = make_uint2(0u, 0u), vw = make_uint2(0u, 0u);
-        float ks = 0.0f, vs = 0.0f;
         const bool live = place < len;
+        int page = 0;
+        bool bad = false;
         if (live) {
-            const int page = __ldg(sq.table + (int64_t)b * sq.table_ld + (place >> kv.page_shift));
-            if (page < 0 || page >= kv.num_pages) {
-                if (kc == 0) atomicExch(&g_kv4_status, KV4_BAD_PAGE);
-                ks = vs = __int_as_float(0x7fc00000);
-            } else {
-                const uint8_t *g = kv.group(page, h, place);
-                const int slot = place & (KV4_GROUP - 1);
-                const int so = kv.scale_off + 2 * (slot * (head_dim / BS) + kc * 16 / BS);
-                kw = __ldg(reinterpret_cast<const uint2 *>(g + slot * (head_dim / 2)) + kc);
-                vw = __ldg(reinterpret_cast<const uint2 *>(g + kv.half_bytes + slot * (head_dim / 2)) + kc);
-                ks = to_f32<T>(*reinterpret_cast<const T *>(g + so));
-                vs = to_f32<T>(*reinterpret_cast<const T *>(g + kv.half_bytes + so));
+            page = __ldg(sq.table + (int64_t)b * sq.table_ld + (place >> kv.page_shift));
+            bad = page < 0 || page >= kv.num_pages;
+            if (bad && lane == 0) atomicExch(&g_kv4_status, KV4_BAD_PAGE);
+        }
+        const int slot = place & (KV4_GROUP - 1);
+        const uint8_t *base = live && !bad ? kv.group(page, 0, place) + slot * (cpr * 4) + kc * 4 : nullptr;   // my codes of head 0's K
+        const int to_scale = kv.scale_off + 2 * ((slot * cpr + kc) * 8 / BS) - (slot * (cpr * 4) + kc * 4);      // from them to their absmax
+        const int64_t row0 = bp * kv.kv_heads;
+        for (int r0 = 0; r0 < 2 * kv.kv_heads; r0 += step * U) {
+            uint32_t w[U];
+            float s[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * step + rl;
+                w[u] = 0x77777777u; s[u] = bad ? __int_as_float(0x7fc00000) : 0.0f;   // (code 7 is not negative: zeros, not -0)
+                if (r < 2 * kv.kv_heads && base != nullptr) {
+                    const uint8_t *g = base + (r >= kv.kv_heads ? (int64_t)(r - kv.kv_heads) * head_bytes + kv.half_bytes : (int64_t)r * head_bytes);
+                    w[u] = __ldg(reinterpret_cast<const uint32_t *>(g));
+                    s[u] = to_f32<T>(*reinterpret_cast<const T *>(g + to_scale));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * step + rl;
+                if (r >= 2 * kv.kv_heads) break;
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float lo, hi;
+                    const uint32_t at_lo = j == 0 ? w[u] << 7 : w[u] >> (8 * j - 7), at_hi = j == 0 ? w[u] << 3 : w[u] >> (8 * j - 3);
+                    asm("ld.shared.f32 %0, [%1];" : "=f"(lo) : "r"((at_lo & 0x780u) + tab_lane));
+                    asm("ld.shared.f32 %0, [%1];" : "=f"(hi) : "r"((at_hi & 0x780u) + tab_lane));
+                    o[j] = pair_of<T>(__fmul_rn(lo, s[u]), __fmul_rn(hi, s[u]));
+                }
+                T *dst = r >= kv.kv_heads ? v + (((row0 + r - kv.kv_heads) << cpr_shift) + kc) * 8 : k + (((row0 + r) << cpr_shift) + kc) * 8;
+                __stcs(reinterpret_cast<uint4 *>(dst), make_uint4(o[0], o[1], o[2], o[3]));
             }
         }
-        auto put = [&](T *out, uint2 w, float s) {
-            uint32_t o[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t word = j < 4 ? w.x : w.y;
-                const float lo = tab[((word >> (8 * (j & 3))) & 15u) * 32 + lane], hi = tab[((word >> (8 * (j & 3) + 4)) & 15u) * 32 + lane];
-                T pr[2] = {from_f32<T>(live ? __fmul_rn(lo, s) : 0.0f), from_f32<T>(live ? __fmul_rn(hi, s) : 0.0f)};
-                o[j] = *reinterpret_cast<const uint32_t *>(pr);
-            }
-            uint4 *dst = reinterpret_cast<uint4 *>(out + r * head_dim + kc * 16);
-            __stcs(dst, make_uint4(o[0], o[1], o[2], o[3]));
-            __stcs(dst + 1, make_uint4(o[4], o[5], o[6], o[7]));
-        };
-        put(k, kw, ks);
-        put(v, vw, vs);
     }
 }
 
@@ -150,12 +163,12 @@ extern "C" int mpsbnb_kv4_dequantize(const mpsbnb_kv4_cache *cache, int layer, c
     if (k == nullptr || v == nullptr || !aligned16(k) || !aligned16(v)) return MPSBNB_ERR_INVALID_ARG;
     const Kv4Layer kv = kv4_layer(cache, layer);
     const Kv4Seqs sq = kv4_seqs(&s, cache);
-    const int64_t total = (int64_t)s.batch * max_len * cache->kv_heads * (cache->head_dim / 16);
-    const int64_t want = (total + 255) / 256, cap = (int64_t)sm_count() * 16;
+    const int cpr_shift = cache->head_dim == 64 ? 3 : cache->head_dim == 128 ? 4 : 5;
+    const int64_t want = ((int64_t)s.batch * max_len + 7) / 8, cap = (int64_t)sm_count() * 8;
     const int grid = (int)(want < cap ? want : cap);
     cudaStream_t st = (cudaStream_t)stream;
 #define LAUNCH_DEQUANT(T, BS) \
-    kv4_dequantize_kernel<T, BS><<<grid, 256, 0, st>>>(kv, sq, cache->quant_type, cache->head_dim, (int)max_len, (T *)k, (T *)v)
+    kv4_dequantize_kernel<T, BS><<<grid, 256, 0, st>>>(kv, sq, cache->quant_type, cpr_shift, (int)max_len, (T *)k, (T *)v)
     if (cache->dtype == MPSBNB_F16) { if (cache->blocksize == 32) LAUNCH_DEQUANT(__half, 32); else LAUNCH_DEQUANT(__half, 64); }
     else { if (cache->blocksize == 32) LAUNCH_DEQUANT(__nv_bfloat16, 32); else LAUNCH_DEQUANT(__nv_bfloat16, 64); }
 #undef LAUNCH_DEQUANT

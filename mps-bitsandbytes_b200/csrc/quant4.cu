@@ -12,6 +12,8 @@
 // the reference arithmetic for every (x, absmax) pair of fp16 and of bf16 by
 // oracle/oracle.c:o_prove_quantizer with block maxima in [1e-30, 1e30]; fp32 input and maxima
 // outside that range use IEEE division.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv4.cuh"
 
@@ -329,94 +331,101 @@ quantize4_stream_kernel(const T *__restrict__ A, IDX total, uint8_t *__restrict_
 
 // ------------------------------------------------------------------------------------------
 // Rows of keys and values into their places in the paged cache (kv4.cuh): the quantiser above with a scattered
-// destination.  A thread owns 8 elements (one 16-byte load where the rows allow it, one 32-bit store), bs / 8 lanes a
-// block; K and V are the two halves of the index range, so one launch stores a layer's new tokens.
+// destination, one launch for a layer's new tokens.  A warp takes a token, finds its place once and then goes through
+// the rows of all heads, K first: a lane owns 8 elements (one 16-byte load where the rows allow it, one 32-bit store), bs / 8
+// lanes a block, four loads per lane under way.  Codes by the streaming quantiser's search.
 // ------------------------------------------------------------------------------------------
 static __device__ int g_kv4_append_status = 0;
 
 template <typename T, int QT, int LPB>
 __global__ void __launch_bounds__(256)
 kv4_append_kernel(const Kv4Layer kv, const Kv4Seqs sq, const T *__restrict__ k, int64_t k_ts, int64_t k_hs,
-                  const T *__restrict__ v, int64_t v_ts, int64_t v_hs, int head_dim, int vec) {
-    __shared__ float2 nf4_tab[16];
-    if (QT == MPSBNB_NF4) {
-        if (threadIdx.x < 16) nf4_bucket_table_fill(nf4_tab, threadIdx.x);
-        __syncthreads();
-    }
-    const int cpr = head_dim / 8;                                  // chunks of a row: 8, 16 or 32, all in one warp
-    const int64_t rows = (int64_t)sq.tokens * kv.kv_heads, total = 2 * rows * cpr;
+                  const T *__restrict__ v, int64_t v_ts, int64_t v_hs, int cpr_shift, int vec) {
+    __shared__ __align__(16) float2 table[(QT == MPSBNB_NF4 ? NF4_B32_ENTRIES : FP4_B16_ENTRIES) * 32];
+    if (QT == MPSBNB_NF4) nf4_bucket32_fill(table, threadIdx.x, 256);
+    else fp4_bucket16_fill(table, threadIdx.x, 256);
+    __syncthreads();
     const int lane = threadIdx.x & 31;
-    const int64_t stride = (int64_t)gridDim.x * 256;
-    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c - lane < total; c += stride) {
-        const int64_t r = c / cpr;
-        const int kc = (int)(c - r * cpr);
-        const bool is_v = r >= rows;
-        const int64_t rr = is_v ? r - rows : r;
-        const int t = (int)(rr / kv.kv_heads), h = (int)(rr - (int64_t)t * kv.kv_heads);
-        bool live = c < total;
-        int place = 0, page = 0;
-        if (live) {                                                // where the token goes
-            int b, i, row, n, len;
-            if (sq.cu == nullptr) {
-                b = t / sq.new_tokens;
-            } else {
-                int lo = 0, hi = sq.batch;                         // last sequence that starts at or before t
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (__ldg(sq.cu + mid) <= t) lo = mid; else hi = mid;
-                }
-                b = lo;
+    const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(table) + (uint32_t)lane * 8u;
+    // a row is cpr chunks of 8 elements (8, 16 or 32 lanes); the warp goes on by `step` rows, K's before V's
+    const int cpr = 1 << cpr_shift, half_dim = cpr * 4, step = 32 >> cpr_shift, kc = lane & (cpr - 1), rl = lane >> cpr_shift;
+    const int head_bytes = (1 << (kv.page_shift - 4)) * kv.group_bytes;
+    constexpr int U = 4;
+    for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < sq.tokens; t += gridDim.x * 8) {
+        int b, row, n, len;
+        if (sq.cu == nullptr) {
+            b = t / sq.new_tokens;
+        } else {
+            int lo = 0, hi = sq.batch;                             // last sequence that starts at or before t
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (__ldg(sq.cu + mid) <= t) lo = mid; else hi = mid;
             }
-            sq.get(b, row, n, len);
-            i = t - row;
-            place = len - n + i;
-            live = i >= 0 && i < n && place >= 0;
-            if (live) {
-                page = __ldg(sq.table + (int64_t)b * sq.table_ld + (place >> kv.page_shift));
-                if (page < 0 || page >= kv.num_pages) {
-                    if (kc == 0) atomicExch(&g_kv4_append_status, KV4_BAD_PAGE);
-                    live = false;
-                }
-            }
+            b = lo;
         }
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (live) {
-            const T *src = (is_v ? v + (int64_t)t * v_ts + (int64_t)h * v_hs : k + (int64_t)t * k_ts + (int64_t)h * k_hs) + kc * 8;
-            if (vec) {
-                raw = __ldg(reinterpret_cast<const uint4 *>(src));
-            } else {
-                const uint16_t *s16 = reinterpret_cast<const uint16_t *>(src);
-                raw = make_uint4(s16[0] | (uint32_t)s16[1] << 16, s16[2] | (uint32_t)s16[3] << 16,
-                                 s16[4] | (uint32_t)s16[5] << 16, s16[6] | (uint32_t)s16[7] << 16);
-            }
+        sq.get(b, row, n, len);
+        const int i = t - row, place = len - n + i;
+        if (i < 0 || i >= n || place < 0) continue;                // (the whole warp: t is the warp's)
+        const int page = __ldg(sq.table + (int64_t)b * sq.table_ld + (place >> kv.page_shift));
+        if (page < 0 || page >= kv.num_pages) {
+            if (lane == 0) atomicExch(&g_kv4_append_status, KV4_BAD_PAGE);
+            continue;
         }
-        float x[8];
-        {
-            const T *hv = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(hv[j]);
-        }
-        // largest magnitude by its bits: a NaN orders above infinity and is not lost
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 1; o < LPB; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (!live) continue;
-        const float a = m >= 0x7f800000u ? __int_as_float(0x7fc00000) : fmaxf(__uint_as_float(m), 1e-8f);
-        uint32_t word = 0;
-        if (a > 1e-8f && a <= 1e30f) {                             // a 16-bit input's magnitude: the shortcut is proven exact
-            const float ri = __frcp_rn(a);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) word |= code_fast<QT>(block_div<true>(x[j], a, ri), nf4_tab) << (4 * j);
-        } else {                                                   // (a NaN block: any codes will do)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) word |= code_fast<QT>(block_div<false>(x[j], a, 0.f), nf4_tab) << (4 * j);
-        }
-        uint8_t *g = kv.group(page, h, place) + (is_v ? kv.half_bytes : 0);
         const int slot = place & (KV4_GROUP - 1);
-        reinterpret_cast<uint32_t *>(g + slot * (head_dim / 2))[kc] = word;
-        if ((kc & (LPB - 1)) == 0) reinterpret_cast<T *>(g + kv.scale_off)[slot * (cpr / LPB) + kc / LPB] = from_f32<T>(a);
+        uint8_t *base = kv.group(page, 0, place) + slot * half_dim + kc * 4;                       // my codes of head 0's K
+        const int to_scale = kv.scale_off + 2 * (slot * (cpr / LPB) + kc / LPB) - (slot * half_dim + kc * 4);   // from them to their absmax
+        const T *ks = k + (int64_t)t * k_ts + kc * 8, *vs = v + (int64_t)t * v_ts + kc * 8;
+        for (int r0 = 0; r0 < 2 * kv.kv_heads; r0 += step * U) {
+            uint4 raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * step + rl;
+                raw[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (r < 2 * kv.kv_heads) {
+                    const T *src = r >= kv.kv_heads ? vs + (r - kv.kv_heads) * v_hs : ks + r * k_hs;
+                    if (vec) {
+                        raw[u] = __ldg(reinterpret_cast<const uint4 *>(src));
+                    } else {
+                        const uint16_t *s16 = reinterpret_cast<const uint16_t *>(src);
+                        raw[u] = make_uint4(s16[0] | (uint32_t)s16[1] << 16, s16[2] | (uint32_t)s16[3] << 16,
+                                            s16[4] | (uint32_t)s16[5] << 16, s16[6] | (uint32_t)s16[7] << 16);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r0 + u * step >= 2 * kv.kv_heads) break;       // warp-uniform
+                const int r = r0 + u * step + rl;
+                // largest magnitude by its bits, two at a time: a NaN orders above infinity and is not lost
+                const uint32_t m2 = __vmaxu2(__vmaxu2(raw[u].x & 0x7fff7fffu, raw[u].y & 0x7fff7fffu), __vmaxu2(raw[u].z & 0x7fff7fffu, raw[u].w & 0x7fff7fffu));
+                uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+#pragma unroll
+                for (int o = 1; o < LPB; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const bool bad = m >= (sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);   // the block reads back as NaN; any codes will do
+                const uint16_t mb = (uint16_t)m;
+                const float a = bad ? 1.0f : fmaxf(to_f32<T>(*reinterpret_cast<const T *>(&mb)), 1e-8f);
+                float x[8];
+                const T *hv = reinterpret_cast<const T *>(&raw[u]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(hv[j]);
+                uint32_t word = 0;
+                if (bad) {
+                } else if (a > 1e-8f && a <= 1e30f) {              // a 16-bit input's magnitude: the shortcut is proven exact
+                    const float ri = __frcp_rn(a);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) word += code_unit<QT>(block_div<true>(x[j], a, ri), tab_lane) << (4 * j);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) word += code_unit<QT>(block_div<false>(x[j], a, 0.f), tab_lane) << (4 * j);
+                }
+                if (r < 2 * kv.kv_heads) {
+                    const bool is_v = r >= kv.kv_heads;
+                    uint8_t *g = base + (is_v ? (int64_t)(r - kv.kv_heads) * head_bytes + kv.half_bytes : (int64_t)r * head_bytes);
+                    *reinterpret_cast<uint32_t *>(g) = word;
+                    if ((kc & (LPB - 1)) == 0) *reinterpret_cast<T *>(g + to_scale) = from_f32<T>(bad ? __int_as_float(0x7fc00000) : a);
+                }
+            }
+        }
     }
 }
 
@@ -865,12 +874,13 @@ extern "C" int mpsbnb_kv4_append(const mpsbnb_kv4_cache *cache, int layer, const
     const Kv4Layer kv = kv4_layer(cache, layer);
     const Kv4Seqs sq = kv4_seqs(seqs, cache);
     const int vec = aligned16(k) && aligned16(v) && ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
-    const int64_t total = 2 * seqs->tokens * cache->kv_heads * (cache->head_dim / 8);
-    const int grid = grid_for(total, 256, 16);
+    const int cpr_shift = cache->head_dim == 64 ? 3 : cache->head_dim == 128 ? 4 : 5;
+    const int64_t want = (seqs->tokens + 7) / 8, cap = (int64_t)sm_count() * 8;
+    const int grid = (int)(want < cap ? want : cap);
     cudaStream_t st = (cudaStream_t)stream;
 #define LAUNCH_APPEND(T, QT, LPB)                                                                                   \
     kv4_append_kernel<T, QT, LPB><<<grid, 256, 0, st>>>(kv, sq, (const T *)k, k_token_stride, k_head_stride, (const T *)v, \
-                                                        v_token_stride, v_head_stride, cache->head_dim, vec)
+                                                        v_token_stride, v_head_stride, cpr_shift, vec)
 #define LAUNCH_APPEND_LPB(T, QT)                                                                                    \
     do {                                                                                                            \
         if (cache->blocksize == 32) LAUNCH_APPEND(T, QT, 4);                                                        \

@@ -180,13 +180,26 @@ CASES = [
     (128, 64, 64, "nf4", F16, 8, 2, [37, 64, 1], [37, 150, 90], True, None),   # short prompts
     (64, 64, 16, "nf4", BF16, 4, 4, [33, 16], [33, 500], True, 17),
     (128, 64, 64, "fp4", F16, 8, 2, [130], [1040], False, None),
-    (128, 64, 64, "nf4", BF16, 8, 2, [300, 129, 257, 2], [300, 700, 257, 900], True, None),   # prompts
-    (64, 64, 64, "nf4", F16, 12, 4, [260, 513], [260, 600], True, 200),
+    (128, 64, 64, "nf4", BF16, 8, 2, [300, 129, 257, 2], [300, 700, 257, 900], True, None),
     (256, 64, 64, "nf4", BF16, 6, 2, [200, 140], [333, 140], True, None),
-    (128, 32, 16, "fp4", F16, 5, 1, [301], [444], True, None),
-    (64, 32, 32, "nf4", BF16, 3, 1, [400], [400], False, None),
-    (256, 32, 128, "fp4", F16, 2, 1, [257, 300], [1000, 300], True, 129),
+    # prompts: 16-row tiles of all sequences and heads above 700, 430, 225 for head_dim 64, 128, 256
+    (128, 64, 64, "nf4", BF16, 32, 8, [300, 129, 257, 2], [300, 700, 257, 900], True, None),
+    (64, 64, 64, "nf4", F16, 24, 8, [260, 513], [260, 600], True, 200),
+    (256, 64, 64, "nf4", BF16, 24, 8, [200, 140], [333, 140], True, None),
+    (128, 32, 16, "fp4", F16, 40, 8, [201], [444], True, None),
+    (64, 32, 32, "nf4", BF16, 24, 8, [500], [500], False, None),
+    (256, 32, 128, "fp4", F16, 16, 8, [257, 300], [1000, 300], True, 129),
+    (128, 64, 128, "fp4", BF16, 56, 8, [37, 130, 128], [1037, 130, 1000], True, 1),
+    (128, 32, 64, "nf4", BF16, 12, 4, [513, 700], [515, 1500], True, 300),
+    (64, 64, 16, "fp4", BF16, 16, 16, [700, 1], [701, 5], True, None),
+    (256, 32, 64, "nf4", BF16, 8, 1, [511], [900], False, None),
+    (128, 64, 32, "nf4", F16, 8, 8, [900, 0, 1100], [900, 20, 1111], True, None),
 ]
+PROMPTS = [c for c in CASES if (lambda rows: len(c[7]) * c[6] * -(-rows // 16) > {64: 700, 128: 430, 256: 225}[c[0]])(sum(c[7]) * (c[5] // c[6]) / len(c[7]))]
+
+
+def test_both_kernels_are_covered():
+    assert len(PROMPTS) == 11 and len(CASES) - len(PROMPTS) == 17 and {c[:2] for c in PROMPTS} == {(d, b) for d in (64, 128, 256) for b in (32, 64)}
 
 
 def _problem(case, seed=0, k_size=1.0, v_size=1.0):
@@ -220,7 +233,7 @@ def test_attention(case):
     assert_device_ok()
 
 
-@pytest.mark.parametrize("head_dim,heads,kv_heads", [(64, 8, 2), (128, 8, 1), (256, 4, 2)])
+@pytest.mark.parametrize("head_dim,heads,kv_heads", [(64, 8, 2), (128, 8, 1), (256, 4, 2), (64, 48, 8), (128, 24, 4)])
 def test_many_sequences_of_all_kinds(head_dim, heads, kv_heads):
     """More blocks of rows than there are SMs, in an order that mixes sequences with one and with two row tiles, without new tokens,
     without keys, and shorter than their new tokens."""
@@ -241,13 +254,13 @@ def test_many_sequences_of_all_kinds(head_dim, heads, kv_heads):
     assert_device_ok()
 
 
-@pytest.mark.parametrize("heads,new", [(8, 6), (8, 200)])
-def test_rows_without_keys_are_zero_and_rows_past_the_last_sequence_stay(heads, new):
+@pytest.mark.parametrize("heads,kv_heads,new", [(8, 2, 6), (8, 2, 200), (48, 8, 200)])
+def test_rows_without_keys_are_zero_and_rows_past_the_last_sequence_stay(heads, kv_heads, new):
     import kv_util as U
     # lengths 0; shorter than the new tokens; none new; whole
     news, lens = [2, new, 0, 3, new], [0, 4, 30, 3, new + 100]
     starts = _starts(news)
-    cache = U.make_cache(5 * 5, 2, 128, seed=2)
+    cache = U.make_cache(5 * 5, kv_heads, 128, seed=2)
     table = U.random_table(5, 5, 25)
     q = torch.randn(starts[-1] + 4, heads, 128, device="cuda", dtype=F16)
     want, want_lse, bound = U.attention(q, cache, 0, table, lens, starts)
@@ -263,14 +276,14 @@ def test_rows_without_keys_are_zero_and_rows_past_the_last_sequence_stay(heads, 
     assert (fresh[n:] == 0).all() and torch.equal(fresh[:n], got[:n])
 
 
-@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("new,kv_heads", [(1, 2), (150, 2), (150, 8)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
-def test_what_lies_in_unseen_places_does_not_matter(dtype, new):
+def test_what_lies_in_unseen_places_does_not_matter(dtype, new, kv_heads):
     import kv_util as U
     lens, window = [200, 333], 90
-    cache = U.make_cache(13, 2, 128, dtype=dtype, seed=5)
+    cache = U.make_cache(13, kv_heads, 128, dtype=dtype, seed=5)
     table = U.random_table(2, 6, 13, seed=1)
-    q = torch.randn(2, new, 8, 128, device="cuda").to(dtype)
+    q = torch.randn(2, new, 4 * kv_heads, 128, device="cuda").to(dtype)
     clean = bnb.attention_4bit(q, cache, 0, table, _i32(lens), window=window)
     bad = torch.ones(13, 64, dtype=torch.bool, device="cuda")       # pages, places
     for b, length in enumerate(lens):
@@ -285,11 +298,11 @@ def test_what_lies_in_unseen_places_does_not_matter(dtype, new):
     assert_device_ok()
 
 
-@pytest.mark.parametrize("new", [1, 130])
+@pytest.mark.parametrize("new,kv_heads", [(1, 2), (130, 2), (130, 8)])
 @pytest.mark.parametrize("k_size,v_size,scale", [(1e-20, 1e-30, None), (0.05, 1e30, None), (30.0, 1e-3, 0.02), (1.0, 1.0, 0.0), (1.0, 1.0, -0.1)])
-def test_magnitudes_and_scales(new, k_size, v_size, scale):
+def test_magnitudes_and_scales(new, kv_heads, k_size, v_size, scale):
     import kv_util as U
-    case = (128, 64, 64, "nf4", BF16, 8, 2, [new, new], [400, 1100], True, None)
+    case = (128, 64, 64, "nf4", BF16, 4 * kv_heads, kv_heads, [new, new], [400, 1100], True, None)
     cache, table, starts, q = _problem(case, 3, k_size, v_size)
     # values of very different size beside one another, the first of them the largest by far
     cache.v_absmax[:, :, :, 0, 0] *= 2.0 ** 6
@@ -312,14 +325,14 @@ def test_small_and_large_fp16_queries(size):
     U.check(bnb.attention_4bit(q, cache, 1, table, _i32(case[8])), want, bound, F16)
 
 
-@pytest.mark.parametrize("new", [1, 140])
-def test_a_page_outside_the_cache_gives_nan_and_a_status(new):
+@pytest.mark.parametrize("new,kv_heads", [(1, 2), (140, 2), (140, 8)])
+def test_a_page_outside_the_cache_gives_nan_and_a_status(new, kv_heads):
     import ctypes as C
     import kv_util as U
     from mps_bitsandbytes_b200 import _native as N
-    cache = U.make_cache(9, 2, 128)
+    cache = U.make_cache(9, kv_heads, 128)
     table = U.random_table(3, 3, 9)
-    q = torch.randn(3, new, 8, 128, device="cuda", dtype=F16)
+    q = torch.randn(3, new, 4 * kv_heads, 128, device="cuda", dtype=F16)
     lens = _i32([150, 190, 150])
     clean = bnb.attention_4bit(q, cache, 0, table, lens)
     st = C.c_int(0)
@@ -335,7 +348,7 @@ def test_a_page_outside_the_cache_gives_nan_and_a_status(new):
         assert torch.isnan(k[1, 64:128]).all() and torch.isnan(v[1, 64:128]).all() and torch.isfinite(k[1, 128:]).all()
         assert N.lib().mpsbnb_device_status(C.byref(st), 1) == 0 and st.value == 401
         before = cache.data.clone()
-        x = torch.randn(3, 100, 2, 128, device="cuda", dtype=F16)
+        x = torch.randn(3, 100, kv_heads, 128, device="cuda", dtype=F16)
         bnb.append_kv_4bit(cache, 0, x, x, bad, lens)
         assert N.lib().mpsbnb_device_status(C.byref(st), 1) == 0 and st.value == 401
         assert torch.equal(cache.data[0, table[1, 1].item()], before[0, table[1, 1].item()])
@@ -383,7 +396,7 @@ def test_offsets_beyond_32_bits():
     lens = _i32([700, 513])
     want = bnb.attention_4bit(q, small, 0, _i32([[0, 1, 2], [3, 4, 5]]), lens)
     assert torch.equal(bnb.attention_4bit(q, cache, 2, table, lens), want)
-    q = torch.randn(2, 300, 16, 64, device="cuda", dtype=F16)
+    q = torch.randn(2, 400, 16, 64, device="cuda", dtype=F16)         # 16 lists of 50 row tiles: the prompt kernel
     want = bnb.attention_4bit(q, small, 0, _i32([[0, 1, 2], [3, 4, 5]]), lens)
     assert torch.equal(bnb.attention_4bit(q, cache, 2, table, lens), want)
     k, _ = bnb.dequantize_kv_4bit(cache, 2, table, lens, 700)
