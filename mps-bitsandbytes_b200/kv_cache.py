@@ -17,7 +17,6 @@ has a backward pass.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import heapq
 from typing import List, Optional, Sequence, Tuple, Union
@@ -206,7 +205,7 @@ class KVCache4bit(_PageBook):
         self.v_absmax = self.data[..., half + codes:].view(dtype).unflatten(-1, (_GROUP, nb))
         self._desc = N.Kv4Cache(self.data.data_ptr(), num_pages, num_layers, num_kv_heads, head_dim, page_size, blocksize,
                                 N.qt(quant_type), N.dt(dtype))
-        self._ref = C.byref(self._desc)
+        self._ref, self._index = C.byref(self._desc), device.index
 
     def _copy_pages(self, src: List[int], dst: List[int]) -> None:
         copy_kv_pages_4bit(self, src, dst)
@@ -237,10 +236,10 @@ def _check_cache(cache: KVCache4bit, layer: int, what: str):
 
 
 def _check_index(name: str, t: Tensor, dim: int, cache: KVCache4bit):
-    if t.dtype != torch.int32 or t.dim() != dim or t.device != cache.device:
+    if t.dtype is not torch.int32 or t.dim() != dim or t.get_device() != cache._index:
         raise ValueError(f"{name} must be int32 with {dim} dimension{'s' if dim > 1 else ''} on {cache.device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if (t.stride(-1) != 1 and t.shape[-1] > 1) or (dim == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if not t.is_contiguous() and ((t.stride(-1) != 1 and t.shape[-1] > 1) or (dim == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1])):
         raise ValueError(f"{name} must have distinct rows, contiguous along the last dimension")
 
 
@@ -269,32 +268,49 @@ def _seqs(cache: KVCache4bit, page_table: Tensor, seq_lens: Tensor, cu_seqlens: 
                      None if cu_seqlens is None else cu_seqlens.data_ptr(), tokens, width, batch, new)
 
 
-def _rows(name: str, t: Tensor, heads: Optional[int], cache: KVCache4bit) -> Tensor:
-    """[..., heads, head_dim] as [tokens, heads, head_dim] whose rows can be fetched in 16-byte pieces (a copy if not)."""
-    if t.device != cache.device:
+def _rows(name: str, t: Tensor, heads: Optional[int], cache: KVCache4bit):
+    """[..., heads, head_dim] as rows that can be fetched in 16-byte pieces: (the tensor, or a copy of it, that holds them,
+    tokens, heads, strides of a token and of a head)."""
+    if t.get_device() != cache._index:
         raise ValueError(f"{name} must be on {cache.device}, got {t.device}")
-    if t.dtype != cache.dtype:
+    if t.dtype is not cache.dtype:
         raise ValueError(f"{name} must have the cache's dtype {cache.dtype}, got {t.dtype}")
-    if t.dim() not in (3, 4) or t.shape[-1] != cache.head_dim or (heads is not None and t.shape[-2] != heads):
+    shape = t.shape
+    if len(shape) not in (3, 4) or shape[-1] != cache.head_dim or (heads is not None and shape[-2] != heads):
         raise ValueError(f"{name} must be [tokens, heads, {cache.head_dim}] or [batch, tokens, heads, {cache.head_dim}]"
-                         f"{f' with {heads} heads' if heads is not None else ''}, got {tuple(t.shape)}")
-    if torch.is_grad_enabled() and t.requires_grad:
+                         f"{f' with {heads} heads' if heads is not None else ''}, got {tuple(shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, but the 4-bit cache has no backward pass")
-    r = t.reshape(-1, *t.shape[-2:]) if t.dim() == 4 else t
-    if r.stride(2) != 1 or (r.stride(0) | r.stride(1)) & 7 or r.data_ptr() & 15:
-        r = r.contiguous()
-        if r.data_ptr() & 15:                       # contiguous already, but on an odd address
-            r = r.clone()
-    return r
+    stride = t.stride()
+    if len(shape) == 4:
+        tokens = shape[0] * shape[1]
+        # the tokens of all sequences at one distance (else a copy)
+        if shape[0] > 1 and shape[1] > 1 and stride[0] != shape[1] * stride[1]:
+            t = t.contiguous()
+            stride = t.stride()
+        token = stride[1] if shape[1] > 1 else stride[0]
+    else:
+        tokens, token = shape[0], stride[0]
+    head = stride[-2]
+    if stride[-1] != 1 or (token | head) & 7 or t.data_ptr() & 15:
+        t = t.contiguous()
+        if t.data_ptr() & 15:                       # contiguous already, but on an odd address
+            t = t.clone(memory_format=torch.contiguous_format)
+        head, token = cache.head_dim, shape[-2] * cache.head_dim
+    return t, tokens, shape[-2], token, head
 
 
-def _on(device: torch.device):
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def _stream(device: torch.device) -> int:
-    """The current stream's handle, without the Stream object that torch.cuda.current_stream() makes (3 us of a 20 us call)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _call(cache: KVCache4bit, what: str, entry, *args):
+    """Runs a C entry point on the cache's device and its current stream."""
+    index = cache._index
+    # (the stream's handle without the Stream object that torch.cuda.current_stream() makes: 3 us of a 20 us call)
+    if torch._C._cuda_getDevice() == index:
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        N.check(status, what)
 
 
 # ---------------------------------------------------------------------- operators
@@ -309,15 +325,13 @@ def append_kv_4bit(cache: KVCache4bit, layer: int, k: Tensor, v: Tensor, page_ta
     ``quantize_4bit``.  A page that is written must belong to one sequence only (``KVCache4bit.extend`` sees to it).
     """
     _check_cache(cache, layer, "append_kv_4bit")
-    kr = _rows("k", k, cache.num_kv_heads, cache)
-    vr = _rows("v", v, cache.num_kv_heads, cache)
+    kr, tokens, _, k_token, k_head = _rows("k", k, cache.num_kv_heads, cache)
+    vr, _, _, v_token, v_head = _rows("v", v, cache.num_kv_heads, cache)
     if k.shape != v.shape:
         raise ValueError(f"k and v must have the same shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    sq = _seqs(cache, page_table, seq_lens, cu_seqlens, kr.shape[0], None)
-    with _on(cache.device):
-        N.check(N.lib().mpsbnb_kv4_append(cache._ref, layer, C.byref(sq), kr.data_ptr(), kr.stride(0), kr.stride(1),
-                                          vr.data_ptr(), vr.stride(0), vr.stride(1),
-                                          _stream(cache.device)), "append_kv_4bit")
+    sq = _seqs(cache, page_table, seq_lens, cu_seqlens, tokens, None)
+    _call(cache, "append_kv_4bit", N.lib().mpsbnb_kv4_append, cache._ref, layer, sq, kr.data_ptr(), k_token, k_head,
+          vr.data_ptr(), v_token, v_head)
 
 
 def dequantize_kv_4bit(cache: KVCache4bit, layer: int, page_table: Tensor, seq_lens: Tensor,
@@ -332,9 +346,7 @@ def dequantize_kv_4bit(cache: KVCache4bit, layer: int, page_table: Tensor, seq_l
         raise ValueError(f"max_len must not be negative, got {max_len}")
     shape = (page_table.shape[0], int(max_len), cache.num_kv_heads, cache.head_dim)
     k, v = cache.k_absmax.new_empty(shape), cache.k_absmax.new_empty(shape)
-    with _on(cache.device):
-        N.check(N.lib().mpsbnb_kv4_dequantize(cache._ref, layer, C.byref(sq), max_len, k.data_ptr(), v.data_ptr(),
-                                              _stream(cache.device)), "dequantize_kv_4bit")
+    _call(cache, "dequantize_kv_4bit", N.lib().mpsbnb_kv4_dequantize, cache._ref, layer, sq, max_len, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -355,13 +367,12 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
     -inf; rows past ``cu_seqlens[-1]`` stay as they were in ``out``, and are zeros without it.
     """
     _check_cache(cache, layer, "attention_4bit")
-    qr = _rows("q", q, None, cache)
-    heads = qr.shape[1]
+    qr, tokens, heads, token, head = _rows("q", q, None, cache)
     if heads == 0 or heads % cache.num_kv_heads:
         raise ValueError(f"q has {heads} heads, which {cache.num_kv_heads} key/value heads do not divide")
     if window is not None and (window <= 0 or not causal):
         raise ValueError(f"window must be positive and needs causal=True, got {window}")
-    sq = _seqs(cache, page_table, seq_lens, cu_seqlens, qr.shape[0], max_seqlen)
+    sq = _seqs(cache, page_table, seq_lens, cu_seqlens, tokens, max_seqlen)
     if out is None:
         out = q.new_empty(q.shape) if cu_seqlens is None else q.new_zeros(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() & 15:
@@ -370,13 +381,11 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
     if return_lse:
         lse = torch.full(q.shape[:-1], float("-inf"), dtype=torch.float32, device=q.device)
     lib = N.lib()
-    with _on(cache.device):
-        nbytes = lib.mpsbnb_attention_4bit_workspace_bytes(cache._ref, C.byref(sq), heads)
-        ws = cache.data.new_empty(nbytes)
-        N.check(lib.mpsbnb_attention_4bit(
-            cache._ref, layer, C.byref(sq), qr.data_ptr(), qr.stride(0), qr.stride(1), heads, int(causal), int(window or 0),
-            float(cache.head_dim ** -0.5 if scale is None else scale), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            ws.data_ptr(), nbytes, _stream(cache.device)), "attention_4bit")
+    nbytes = lib.mpsbnb_attention_4bit_workspace_bytes(cache._ref, sq, heads)
+    ws = cache.data.new_empty(nbytes)
+    _call(cache, "attention_4bit", lib.mpsbnb_attention_4bit, cache._ref, layer, sq, qr.data_ptr(), token, head, heads,
+          1 if causal else 0, window or 0, cache.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+          None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -398,6 +407,4 @@ def copy_kv_pages_4bit(cache: KVCache4bit, src: Sequence[int], dst: Sequence[int
     if not targets.isdisjoint(src):
         raise ValueError("a page is both source and destination")
     array = C.c_int32 * len(src)
-    with _on(cache.device):
-        N.check(N.lib().mpsbnb_kv4_copy_pages(cache._ref, array(*src), array(*dst), len(src),
-                                              _stream(cache.device)), "copy_kv_pages_4bit")
+    _call(cache, "copy_kv_pages_4bit", N.lib().mpsbnb_kv4_copy_pages, cache._ref, array(*src), array(*dst), len(src))
