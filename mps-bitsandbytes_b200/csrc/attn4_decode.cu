@@ -188,8 +188,9 @@ template <class S> struct AdPiece {
     }
 };
 
-// units per team: equal, and worth a piece with a few tiles for each of the warps
-__device__ __forceinline__ int64_t ad_per(int64_t total, int teams, int cost) { return max(ad_div(total + teams - 1, teams), (int64_t)(cost + 4 * AD_WARPS)); }
+// Units per team: equal, and no fewer than give each warp two tiles and then some.  (What little work there is is best spread
+// thin: 32 heads of 200 keys take 15.4 us so, 17.4 with a piece's cost and a tile for each warp, 19.5 with four tiles.)
+__device__ __forceinline__ int64_t ad_per(int64_t total, int teams, int cost) { return max(ad_div(total + teams - 1, teams), (int64_t)(cost / 4 + 2 * AD_WARPS)); }
 
 // partial result of team c, slot s (0: its first piece, 1: its last): RT x D sums, then RT (maximum, sum) pairs
 template <int D, int RT> __device__ __forceinline__ float *ad_partial(float *ws, int64_t c, int s) {
@@ -218,7 +219,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     }
     const int cta_warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int in_team = cta_warp / AD_WARPS, warp = cta_warp % AD_WARPS;
-    const int teams = gridDim.x * S::TEAMS, team = blockIdx.x * S::TEAMS + in_team;
+    const int teams = gridDim.x * S::TEAMS, team = in_team * gridDim.x + blockIdx.x;   // little work spreads over the SMs
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + (S::END - 16 - AD_BASE));
     int64_t units = ad_units<S>(A, lane);                            // (its loads are under way while the table is made)
     pdl_launch_dependents();
