@@ -17,7 +17,8 @@
 //   warp 16         issues the MMAs: S_A, S_B, then per key tile O_A += P_A V, S_A(next), O_B += P_B V, S_B(next), on
 //                   into the next block of rows without a pause.
 //   warp 17         fetches the codes: one bulk copy per group of 16 tokens, two tiles ahead.
-//   warps 18, 19    bring the next rows of q as soon as the last products with the present ones have been issued.
+//   warps 18, 19    bring the next rows of q as soon as the last products with the present ones have been issued
+//                   (head_dim 256: warps 4-7, which have no second tile).
 // fp16 operands hold bf16 caches too: the absmax of a K tile (and, carried along, of the V tiles) is brought near 2^8 by
 // a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.
 #include <type_traits>
@@ -49,11 +50,12 @@ template <int D, int BS> struct ApSmem {
     static constexpr int PANELS = D / 64, PANEL = KT * 128, Q_PANEL = 128 * 128, BUF = PANELS * PANEL;
     static constexpr int GROUP = 2 * kv4_half_bytes(D, BS), CODES = KT / KV4_GROUP * GROUP;
     static constexpr int NBUF = D > 64 && BS == 32 ? 2 : 3;          // operand buffers (what fits)
+    static constexpr int Q_WARPS = TILES == 1 ? 4 : 2;               // that bring q
     static constexpr int Q = 0;
     static constexpr int RING = Q + TILES * PANELS * Q_PANEL;
     static constexpr int LUT = RING + NBUF * BUF;
     static constexpr int RAW = LUT + 256 * 128;
-    static constexpr int EXPO = RAW + 2 * CODES;                     // [2][TILES * 128] bytes: exponent that a bf16 row of q was brought down by
+    static constexpr int EXPO = RAW + 2 * CODES;                     // [2][TILES * 128] bytes: power of two that a bf16 row of q was divided by
     static constexpr int BAR = EXPO + 2 * TILES * 128;
     static constexpr int TOTAL = BAR + 336;
     // tensor memory columns
@@ -91,6 +93,16 @@ __device__ __forceinline__ void ap_tmem_st16(uint32_t taddr, const uint32_t (&r)
 __device__ __forceinline__ void ap_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+// 16 lanes (rows) of 32 columns as the products' own registers have them: of each eight columns lane l gets 2 (l % 4) and the
+// next, of row l / 4 and then of row l / 4 + 8
+__device__ __forceinline__ void ap_tmem_ld_rows(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
@@ -207,9 +219,9 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(raw_full(i), 1); mbar_init(raw_empty(i), AP_EXPANDERS);
             mbar_init(s_full(i), 1); mbar_init(p_full(i), 4); mbar_init(o_done(i), 1);
-            mbar_init(q_full(i), 2); mbar_init(q_empty(i), 1);
+            mbar_init(q_full(i), S::Q_WARPS); mbar_init(q_empty(i), 1);
         }
-        for (int i = 0; i < 4; ++i) { mbar_init(item_full(i), 1); mbar_init(item_empty(i), 4 * TILES + AP_EXPANDERS + 3); }   // (the issuer, two q warps)
+        for (int i = 0; i < 4; ++i) { mbar_init(item_full(i), 1); mbar_init(item_empty(i), 4 * TILES + AP_EXPANDERS + 1 + S::Q_WARPS); }   // (1: the issuer)
         *abort_flag = *never = 0;
         fence_mbar_init();
     }
@@ -244,6 +256,89 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
         return true;
     };
 #define AP_WAIT(b_, ph_, code_) if (!mbar_wait(b_, ph_, abort_flag)) { atomicExch(&g_attn4_prompt_status, code_); *abort_flag = 1; break; }
+
+    // ------------------------------------------------------------ q: 16 bytes per lane, LPR lanes a row
+    // Straight into the swizzled panels by asynchronous copies, all of a lane's under way at once; a bf16 row is then turned into fp16 where it lies.  Lane l finds where the
+    // warp's rows l, l + 32 lie and hands that to the lanes that copy them.
+    auto bring_q = [&](int part) {
+        constexpr int LPR = D / 8, ROWS = 32 / LPR, STEPS = 32 / ROWS;   // rows a step, steps for 32 rows
+        constexpr int MINE = 128 / S::Q_WARPS, PARTS = MINE / 32;    // rows of this warp, lanes' rows
+        const uint32_t negate = A.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale goes into q: maxima stay maxima
+        const int k = lane % LPR, my = lane / LPR, base = part * MINE;
+        int count[2] = {0, 0};
+        Item w;
+        while (!*abort_flag && next_item(w, false)) {
+            if (w.nk == 0) continue;
+            uint64_t src[TILES][PARTS];                              // 0: no such row
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int x = 0; x < PARTS; ++x) {
+                    const int r = w.r0 + t * 128 + base + x * 32 + lane, i = r / A.group, g = r - i * A.group;
+                    src[t][x] = r < w.rows ? reinterpret_cast<uint64_t>(reinterpret_cast<const T *>(A.q) + (int64_t)(w.row0 + i) * A.q_ts + (int64_t)(w.h * A.group + g) * A.q_hs) : 0;
+                }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                if (t >= w.tiles) break;
+                auto dest = [&](int rr) { return sb + S::Q + (t * S::PANELS + k / 8) * S::Q_PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4); };
+                AP_WAIT(q_empty(t), (count[t] & 1) ^ 1, 423);
+#pragma unroll
+                for (int x = 0; x < PARTS; ++x)
+#pragma unroll 16
+                    for (int s = 0; s < STEPS; ++s) {
+                        const uint64_t from = __shfl_sync(0xffffffffu, src[t][x], s * ROWS + my);
+                        // (no bytes read, 16 zeros written where there is no row)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dest(base + x * 32 + s * ROWS + my)),
+                                     "l"(from != 0 ? from + k * 16 : reinterpret_cast<uint64_t>(A.q)), "r"(from != 0 ? 16 : 0) : "memory");
+                    }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                if (BF || negate != 0) {
+                    // a row to a lane from here on: eight lanes' columns lie in eight different banks' places by the swizzle, and
+                    // nothing waits for a shuffle behind the expanders' look-ups
+                    __syncwarp();
+#pragma unroll 1
+                    for (int x = 0; x < PARTS; ++x) {
+                        const int rr = base + x * 32 + lane;
+                        const uint32_t row = sb + S::Q + t * S::PANELS * S::Q_PANEL + rr * 128;
+                        auto at = [&](int c) { return row + (c >> 3) * S::Q_PANEL + (((c & 7) ^ (rr & 7)) << 4); };
+                        auto load = [&](int c) {
+                            uint4 v;
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at(c)));
+                            return v;
+                        };
+                        uint32_t e2 = 0;
+                        if constexpr (BF) {
+                            uint32_t m2 = 0;                         // largest magnitudes of the even and odd channels
+#pragma unroll 8
+                            for (int c = 0; c < LPR; ++c) {
+                                const uint4 v = load(c);
+                                m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+                            }
+                            // Less an exponent that brings the row's largest to 2^15 (an infinity or a NaN stays one), two channels
+                            // at a time: fp16's bits are then bf16's, three places up.  Parts below 2^-29 of the largest go to
+                            // zero, or lose bits.
+                            const uint32_t e = max(30u, min(254u, max(m2 & 0xffffu, m2 >> 16) >> 7)) - 30;
+                            q_exp[(count[t] & 1) * (TILES * 128) + t * 128 + rr] = (uint8_t)(e + 15);   // of 2^(e - 112), as in fp32
+                            e2 = e * 0x00800080u;
+                        }
+#pragma unroll 4
+                        for (int c = 0; c < LPR; ++c) {
+                            const uint4 v = load(c);
+                            auto cv = [&](uint32_t y) {
+                                if constexpr (BF) return ((__vmaxu2(y & 0x7fff7fffu, e2) - e2) << 3) | ((y ^ negate) & 0x80008000u);
+                                else return y ^ negate;
+                            };
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at(c)), "r"(cv(v.x)), "r"(cv(v.y)), "r"(cv(v.z)), "r"(cv(v.w)));
+                        }
+                    }
+                }
+                ++count[t];
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full(t));
+            }
+        }
+    };
 
     if (warp >= AP_MMA) {
         ap_regs_down<AP_REGS_OTHER>();
@@ -291,77 +386,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
             // no copy may be in flight when the block ends (they are not, unless a wait has run out)
             for (int j = max(0, jj - 2); j < jj; ++j) mbar_wait(raw_full(j & 1), (j >> 1) & 1, never);
         } else if (warp >= AP_Q) {
-            // -------------------------------------------------------- q: 16 bytes per lane, LPR lanes a row
-            // Straight into the swizzled panels by asynchronous copies, all of a lane's under way at once (the rows were asked
-            // of L2 before); a bf16 row is then turned into fp16 where it lies, by the lanes that brought it.
-            constexpr int LPR = D / 8, ROWS = 32 / LPR, STEPS = 64 / ROWS;
-            const uint32_t negate = A.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale goes into q: maxima stay maxima
-            const int k = lane % LPR;
-            int count[2] = {0, 0};
-            Item w;
-            while (!*abort_flag && next_item(w, false)) {
-                if (w.nk == 0) continue;
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    if (t >= w.tiles) break;
-                    const int first_rr = (warp - AP_Q) * 64 + lane / LPR, first_r = w.r0 + t * 128 + first_rr;
-                    const int first_i = first_r / A.group, first_g = first_r - first_i * A.group;
-                    // every row of this lane: f(row of the tile, source or nullptr)
-                    auto each = [&](auto f) {
-                        int rr = first_rr, i = first_i, g = first_g;
-#pragma unroll 8
-                        for (int s = 0; s < STEPS; ++s, rr += ROWS) {
-                            f(rr, i < w.n ? reinterpret_cast<const T *>(A.q) + (int64_t)(w.row0 + i) * A.q_ts + (int64_t)(w.h * A.group + g) * A.q_hs + k * 8 : nullptr);
-                            g += ROWS;
-                            while (g >= A.group) { g -= A.group; ++i; }
-                        }
-                    };
-                    auto dest = [&](int rr) { return sb + S::Q + (t * S::PANELS + k / 8) * S::Q_PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4); };
-                    each([&](int, const T *src) { if (src != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(src)); });
-                    AP_WAIT(q_empty(t), (count[t] & 1) ^ 1, 423);
-                    each([&](int rr, const T *src) {
-                        if (src != nullptr) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dest(rr)), "l"(src));
-                        else asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dest(rr)), "r"(0u));
-                    });
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    if (BF || negate != 0) {
-                        constexpr int FLY = 8;                       // rows worked on side by side
-#pragma unroll 1
-                        for (int s0 = 0; s0 < STEPS; s0 += FLY) {
-                            uint4 x[FLY];
-                            uint32_t mx[FLY];
-#pragma unroll
-                            for (int y = 0; y < FLY; ++y) {
-                                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[y].x), "=r"(x[y].y), "=r"(x[y].z), "=r"(x[y].w) : "r"(dest(first_rr + (s0 + y) * ROWS)));
-                                // largest magnitude, two halves at a time
-                                const uint32_t m2 = __vmaxu2(__vmaxu2(x[y].x & 0x7fff7fffu, x[y].y & 0x7fff7fffu), __vmaxu2(x[y].z & 0x7fff7fffu, x[y].w & 0x7fff7fffu));
-                                mx[y] = max(m2 & 0xffffu, m2 >> 16);
-                            }
-                            if constexpr (BF) {
-#pragma unroll
-                                for (int o = 1; o < LPR; o <<= 1)
-#pragma unroll
-                                    for (int y = 0; y < FLY; ++y) mx[y] = max(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], o));
-                            }
-#pragma unroll
-                            for (int y = 0; y < FLY; ++y) {
-                                const int rr = first_rr + (s0 + y) * ROWS, e = max(1, min(253, (int)(mx[y] >> 7)));
-                                const float down = __int_as_float((254 - e) << 23);   // a row's largest comes to [1, 2)
-                                if (BF && k == 0) q_exp[(count[t] & 1) * (TILES * 128) + t * 128 + rr] = (uint8_t)e;
-                                auto cv = [&](uint32_t v) {
-                                    v ^= negate;
-                                    return BF ? ap_half2(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down) : v;
-                                };
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dest(rr)), "r"(cv(x[y].x)), "r"(cv(x[y].y)), "r"(cv(x[y].z)), "r"(cv(x[y].w)));
-                            }
-                        }
-                    }
-                    ++count[t];
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(q_full(t));
-                }
-            }
+            if constexpr (TILES == 2) bring_q(warp - AP_Q);
         } else if (elect_one()) {
             // -------------------------------------------------------- products
             const uint32_t idesc_s = umma_idesc_f16(0, 128, KT);
@@ -581,14 +606,18 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
                             if (odd && (sbits[it] & INF) == INF) s = 0.0f;
                         }
                         const __half2 s2 = __float2half2_rn(s);
-                        if (turn & 1) { uint32_t x = c[it][0]; c[it][0] = c[it][1]; c[it][1] = x; x = c[it][2]; c[it][2] = c[it][3]; c[it][3] = x; }
-                        if (turn & 2) { uint32_t x = c[it][0]; c[it][0] = c[it][2]; c[it][2] = x; x = c[it][1]; c[it][1] = c[it][3]; c[it][3] = x; }
+                        if (side == 0) {
+                            if (turn & 1) { uint32_t x = c[it][0]; c[it][0] = c[it][1]; c[it][1] = x; x = c[it][2]; c[it][2] = c[it][3]; c[it][3] = x; }
+                            if (turn & 2) { uint32_t x = c[it][0]; c[it][0] = c[it][2]; c[it][2] = x; x = c[it][1]; c[it][1] = c[it][3]; c[it][3] = x; }
+                        }
+                        // K: 16 bytes are the eight channels of a word.  V: one byte of each of the four words, so that column
+                        // 8 e + 2 i + (0, 1) of O is channel 8 i + 2 e + (0, 1) of 32.
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             uint32_t o[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const uint32_t p = ap_lut(lut, c[it][i], e);
+                                const uint32_t p = side == 0 ? ap_lut(lut, c[it][i], e) : ap_lut(lut, c[it][e], i ^ turn);
                                 const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&p), s2);
                                 o[e] = *reinterpret_cast<const uint32_t *>(&y);
                             }
@@ -608,7 +637,8 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
             }
         }
     } else if (TILES == 1 && warp >= 4) {
-        ap_regs_down<AP_REGS_OTHER>();                               // (no second row tile)
+        ap_regs_down<AP_REGS_OTHER>();
+        if constexpr (TILES == 1) bring_q(warp - 4);                 // (there is no second row tile)
     } else {
         ap_regs_up<AP_REGS_SOFTMAX>();
         // ------------------------------------------------------------ softmax: one row per thread
@@ -742,25 +772,38 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
             ap_unpack2(l2, la, lb);
             const float l = la + lb;
             const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l) * __int_as_float(max(1, ve - 8) << 23) * attn4_code_unscale(A.quant_type);
+            // Four lanes take 32 channels (64 bytes) of a row, eight rows at a time: with 16 bytes of 32 rows each, stores kept the
+            // load and store unit busy 4 times as long.  (The order that V's channels have in O makes a lane's eight neighbours.)
             const int64_t orow = live ? (int64_t)(w.row0 + i) * A.heads + w.h * A.group + g : -1;
-            T *dst = reinterpret_cast<T *>(A.out) + orow * D;
+            int64_t row4[4];
+            float inv4[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                row4[x] = __shfl_sync(0xffffffffu, orow, (lane >> 2) + 8 * x);
+                inv4[x] = __shfl_sync(0xffffffffu, inv, (lane >> 2) + 8 * x);
+            }
+            T *const dst = reinterpret_cast<T *>(A.out) + (lane & 3) * 8;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
-                uint32_t v[32];
+                uint32_t v[2][16];                                   // rows lane / 4 + 16 x (+ 8: the upper two of four)
                 if (w.nk > 0) {
-                    tmem_ld_32x32(t_o + c0, v);
+                    ap_tmem_ld_rows(t_o + c0, v[0]);
+                    ap_tmem_ld_rows(t_o + c0 + (16u << 16), v[1]);
                     tmem_ld_wait();
                 }
-                uint32_t y[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    T pr[2] = {from_f32<T>(0.0f), from_f32<T>(0.0f)};
-                    if (l != 0.0f) { pr[0] = from_f32<T>(__uint_as_float(v[2 * e]) * inv); pr[1] = from_f32<T>(__uint_as_float(v[2 * e + 1]) * inv); }
-                    y[e] = *reinterpret_cast<const uint32_t *>(pr);
-                }
-                if (orow >= 0) {
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t y[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4 *>(dst + c0 + 8 * e) = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+                    for (int e = 0; e < 4; ++e) {
+                        T pr[2] = {from_f32<T>(0.0f), from_f32<T>(0.0f)};
+                        if (inv4[x] != 0.0f) {
+                            pr[0] = from_f32<T>(__uint_as_float(v[x >> 1][4 * e + 2 * (x & 1)]) * inv4[x]);
+                            pr[1] = from_f32<T>(__uint_as_float(v[x >> 1][4 * e + 2 * (x & 1) + 1]) * inv4[x]);
+                        }
+                        y[e] = *reinterpret_cast<const uint32_t *>(pr);
+                    }
+                    if (row4[x] >= 0) *reinterpret_cast<uint4 *>(dst + row4[x] * D + c0) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             }
             tc_fence_before();                                       // O has been read before the next item's P is announced
