@@ -24,7 +24,6 @@
 #include <type_traits>
 
 #include "attn4.cuh"
-#include "ops.cuh"
 
 namespace mpsbnb {
 
@@ -192,19 +191,6 @@ template <class S> struct AdPiece {
 // thin: 32 heads of 200 keys take 15.4 us so, 17.4 with a piece's cost and a tile for each warp, 19.5 with four tiles.)
 __device__ __forceinline__ int64_t ad_per(int64_t total, int teams, int cost) { return max(ad_div(total + teams - 1, teams), (int64_t)(cost / 4 + 2 * AD_WARPS)); }
 
-// partial result of team c, slot s (0: its first piece, 1: its last): RT x D sums, then RT (maximum, sum) pairs
-template <int D, int RT> __device__ __forceinline__ float *ad_partial(float *ws, int64_t c, int s) {
-    return ws + (c * 2 + s) * (RT * (D + 2));
-}
-// behind the partials: what the team's last piece wants joined, if more teams share its (sequence, head, row tile)
-struct AdJoin {
-    int n, slot;                                 // parts, in the teams from this one on (0: nothing to join); the first's slot
-    int row0, rows, r, h;                        // the sequence's first row and number of (token, head) rows; row tile, kv head
-};
-template <int D, int RT> __device__ __forceinline__ AdJoin *ad_join(float *ws, int teams) {
-    return reinterpret_cast<AdJoin *>(ws + (int64_t)teams * 2 * RT * (D + 2));
-}
-
 template <int D, int BS, int NT, typename T>
 __global__ void __launch_bounds__((AdSmem<D, BS, NT>::THREADS), 1)
 attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
@@ -244,7 +230,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const int64_t per = ad_per(total, teams, S::COST), t0 = min(total, team * per), t1 = min(total, t0 + per);
     // what the teams leave for attn4_combine_kernel (a team's thread 0 writes both)
-    AdJoin *join = ad_join<D, RT>(A.ws, teams) + team;
+    Attn4Join *join = attn4_join<D, RT>(A.ws, teams) + team;
     if (warp == 0 && lane == 0) join->n = 0;
     Piece in;                                                        // piece the next copy belongs to
     if (t0 >= t1 || !in.start(A, units, t0, t1)) return;             // whole team; no barrier of the block follows
@@ -586,7 +572,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k; o[i][nt][j + 2] *= k; }
             }
         const bool whole = cur.a == 0 && cur.e == sq.nt;
-        float *part = ad_partial<D, RT>(A.ws, team, first_piece ? 0 : 1);
+        float *part = attn4_partial<D, RT>(A.ws, team, first_piece ? 0 : 1);
         if (cur.a == 0 && !whole && warp == 0 && lane == 0) {
             join->n = 1 + (int)((sq.nt - cur.e + per - 1) / per);
             join->slot = first_piece ? 0 : 1;
@@ -636,73 +622,28 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     } while (cur.next(A));
 }
 
-// Joins partial results: sum of 2^(m_i - M) O_i over sum of 2^(m_i - M) l_i.  A block is one row of what one team began and others
-// went on with; its warps share the parts, each with a running maximum of its own.
-constexpr int AD_JOIN_WARPS = 4;
-template <int D, int RT, typename T>
-__global__ void __launch_bounds__(AD_JOIN_WARPS * 32)
-attn4_combine_kernel(const __grid_constant__ Attn4Args A, int teams) {
-    __shared__ float red[AD_JOIN_WARPS][D + 2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c0 = blockIdx.x, row = blockIdx.y;
-    // every block waits, so that this kernel's end means the end of the one before it as well
-    pdl_grid_dependency_wait();
-    const AdJoin p = ad_join<D, RT>(A.ws, teams)[c0];
-    const int R = p.r * RT + row;
-    if (p.n == 0 || R >= p.rows) return;
-    float M = ATTN4_NONE, L = 0.0f, v[D / 32];
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) v[j] = 0.0f;
-#pragma unroll 4
-    for (int x = warp; x < p.n; x += AD_JOIN_WARPS) {
-        const float *q = ad_partial<D, RT>(A.ws, c0 + x, x == 0 ? p.slot : 0);
-        const float2 ml = *reinterpret_cast<const float2 *>(q + RT * D + 2 * row);
-        const float mn = fmaxf(M, ml.x), ko = ex2(M - mn), kn = ex2(ml.x - mn);
-        M = mn;
-        L = L * ko + ml.y * kn;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) v[j] = v[j] * ko + q[row * D + j * 32 + lane] * kn;
-    }
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) red[warp][j * 32 + lane] = v[j];
-    if (lane == 0) { red[warp][D] = M; red[warp][D + 1] = L; }
-    __syncthreads();
-    M = red[0][D];
-#pragma unroll
-    for (int w = 1; w < AD_JOIN_WARPS; ++w) M = fmaxf(M, red[w][D]);
-    float k[AD_JOIN_WARPS];
-    L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < AD_JOIN_WARPS; ++w) { k[w] = ex2(red[w][D] - M); L = fmaf(red[w][D + 1], k[w], L); }
-    const int i = R / A.group;
-    const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
-    const int64_t orow = (int64_t)(p.row0 + i) * A.heads + p.h * A.group + (R - i * A.group);
-    for (int d = threadIdx.x; d < D; d += AD_JOIN_WARPS * 32) {
-        float y = 0.0f;
-#pragma unroll
-        for (int w = 0; w < AD_JOIN_WARPS; ++w) y = fmaf(red[w][d], k[w], y);
-        reinterpret_cast<T *>(A.out)[orow * D + d] = from_f32<T>(y * inv);
-    }
-    if (A.lse != nullptr && threadIdx.x == 0) A.lse[orow] = L == 0.0f ? __int_as_float(0xff800000) : (M + __log2f(L)) * 0.69314718f;
-}
-
 // ------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------
 // 16 rows per tile where 8 do not hold a sequence's rows: the keys are then expanded half as often
 static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return (int64_t)s->new_tokens * group > 8 ? 2 : 1; }
 
-// The tensor-core kernel of attn4_prompt.cu instead?  It takes a (sequence, kv head)'s keys in one block, one round of blocks
-// after the other, and a key tile costs it the same whether its rows are 16 or 256: 2.0, 2.4, 3.3 us per 128 keys (head_dim 64,
-// 128, 256).  The kernel here spreads any amount of work over the whole card, at 0.42, 0.70, 1.83 ns per 16 rows x 16 keys.
-// They meet where the 16-row tiles of all sequences and heads number 700, 430, 225 per round.  (Measured for 1 - 16
-// sequences, 1 - 8 heads, 16 - 2048 rows a head: 8 heads, 8192 keys, head_dim 128: 512 rows 109 us here and 160 there, 1024
-// rows 197 and 160.)
-static bool ad_prompt(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group) {
+// The tensor-core kernel of attn4_prompt.cu instead?  A key tile costs it the same whether its rows are 16 or 256: 2.0, 2.4, 3.3 us
+// per 128 keys and block (head_dim 64, 128, 256).  The kernel here spreads any amount of work over the whole card, at 0.42, 0.70,
+// 1.83 ns per 16 rows x 16 keys.  They meet where the 16-row tiles of all sequences and heads number 700, 430, 225 per round of
+// blocks over the card.  (Measured for 1 - 16 sequences, 1 - 8 heads, 16 - 2048 rows a head.)
+// Few blocks of rows (under AD_SPLIT rounds) share out the keys as well, and then a part of a round counts as that.
+constexpr int AD_SPLIT = 2;
+enum AdKind { AD_TOKENS, AD_PROMPTS, AD_PROMPTS_SPLIT };
+static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group) {
     const int64_t rows = (s->tokens * group + s->batch - 1) / s->batch;   // of a sequence and head, on average
     const int64_t lists = (int64_t)s->batch * c->kv_heads, block = c->head_dim == 256 ? 128 : 256, sms = sm_count();
-    const int64_t rounds = (lists * ((rows + block - 1) / block) + sms - 1) / sms;
+    const int64_t blocks = lists * ((rows + block - 1) / block), tiles = lists * ((rows + 15) / 16);
     const int64_t meet = c->head_dim == 64 ? 700 : c->head_dim == 128 ? 430 : 225;
-    return rows > 16 && lists * ((rows + 15) / 16) > meet * rounds;
+    // (every block of the card looks through the (sequence, block of rows) pairs, 32 at a time)
+    const bool split = lists * (((int64_t)s->new_tokens * group + block - 1) / block) <= AD_SPLIT * sms;
+    if (rows <= 16 || tiles * sms <= meet * (split ? blocks : (blocks + sms - 1) / sms * sms)) return AD_TOKENS;
+    return split ? AD_PROMPTS_SPLIT : AD_PROMPTS;
 }
 
 static int ad_teams(int D, int NT) { return sm_count() * ((D * NT <= 128 ? 12 : 8) / AD_WARPS); }
@@ -721,17 +662,7 @@ static int ad_launch(const Attn4Args &a, cudaStream_t st) {
     attn4_decode_kernel<D, BS, NT, T><<<teams / S::TEAMS, S::THREADS, S::BYTES, st>>>(a);
     int rc = check_launch();
     if (rc != MPSBNB_OK) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(teams, S::RT);
-    cfg.blockDim = dim3(AD_JOIN_WARPS * 32);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    MPSBNB_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_combine_kernel<D, S::RT, T>, a, teams));
-    return check_launch();
+    return attn4_combine<D, S::RT, 1, T>(a, teams, st);
 }
 
 template <int D, int BS>
@@ -757,8 +688,9 @@ extern "C" size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *
     if (kv4_check_cache(cache, 0) != MPSBNB_OK || kv4_check_seqs(seqs, cache) != MPSBNB_OK) return 0;
     if (heads <= 0 || heads % cache->kv_heads != 0 || seqs->batch == 0 || seqs->tokens == 0) return 0;
     const int nt = ad_nt(seqs, heads / cache->kv_heads);
-    if (ad_prompt(cache, seqs, heads / cache->kv_heads)) return 16;   // (not used)
-    return (size_t)ad_teams(cache->head_dim, nt) * (2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float) + sizeof(AdJoin));
+    const AdKind kind = ad_kind(cache, seqs, heads / cache->kv_heads);
+    if (kind != AD_TOKENS) return kind == AD_PROMPTS ? 16 : attn4_prompt_ws(cache->head_dim);   // (16: not used)
+    return (size_t)ad_teams(cache->head_dim, nt) * (2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float) + sizeof(Attn4Join));
 }
 
 extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
@@ -785,7 +717,8 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.scale_log2 = scale * 1.4426950408889634f;
     static const float codes[2][16] = {MPSBNB_NF4_TABLE, MPSBNB_FP4_TABLE};
     for (int i = 0; i < 16; ++i) a.code[i] = codes[cache->quant_type][i] * attn4_code_scale(cache->quant_type);
-    if (ad_prompt(cache, seqs, group)) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, (cudaStream_t)stream);
+    const AdKind kind = ad_kind(cache, seqs, group);
+    if (kind != AD_TOKENS) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, kind == AD_PROMPTS_SPLIT, (cudaStream_t)stream);
     const int nt = ad_nt(seqs, group);
     cudaStream_t st = (cudaStream_t)stream;
     const int dt = cache->dtype;

@@ -24,7 +24,6 @@
 #include <type_traits>
 
 #include "attn4.cuh"
-#include "ops.cuh"
 
 namespace mpsbnb {
 
@@ -57,7 +56,7 @@ template <int D, int BS> struct ApSmem {
     static constexpr int RAW = LUT + 256 * 128;
     static constexpr int EXPO = RAW + 2 * CODES;                     // [2][TILES * 128] bytes: power of two that a bf16 row of q was divided by
     static constexpr int BAR = EXPO + 2 * TILES * 128;
-    static constexpr int TOTAL = BAR + 336;
+    static constexpr int TOTAL = BAR + 368;
     // tensor memory columns
     static constexpr int S_COL = 0, S_STEP = TILES == 2 ? 128 : 64, O_COL = 2 * S_STEP;
     static_assert(O_COL + TILES * D <= 512, "tensor memory");
@@ -137,9 +136,11 @@ template <int TILES, int KT> struct ApItem {
     int b, h, r0, rows, row0, n, len, first;
     int tiles;                                                       // 128-row tiles that hold rows
     int lo, hi, start, nk;                                           // keys any row sees: [lo, hi), from place `start` in nk tiles
+    int slot;                                                        // where the partial result goes; -1: the item is whole
 
-    __device__ __forceinline__ void set(const Attn4Args &A, int b_, int h_, int r0_) {
-        b = b_; h = h_; r0 = r0_;
+    // key tiles [a, e) of it
+    __device__ __forceinline__ void set(const Attn4Args &A, int b_, int h_, int r0_, int a, int e, int slot_) {
+        b = b_; h = h_; r0 = r0_; slot = slot_;
         A.sq.get(b, row0, n, len);
         rows = n * A.group;
         tiles = TILES == 2 && r0 + 128 < rows ? 2 : 1;
@@ -149,6 +150,9 @@ template <int TILES, int KT> struct ApItem {
         lo = A.window > 0 ? max(0, first + i_lo + 1 - A.window) : 0;
         start = lo & ~(KV4_GROUP - 1);
         nk = hi > lo ? (hi - start + KT - 1) / KT : 0;
+        nk = max(0, min(nk, e) - a);
+        start += a * KT;
+        hi = min(hi, start + nk * KT);
     }
 };
 
@@ -181,9 +185,83 @@ template <int STEP> struct ApList {
     }
 };
 
+// Few items: the key tiles of all, AP_COST more for each item, are cut into equal runs, one per block, in the order of the pairs
+// (block of rows, sequence) with a sequence's heads side by side.  Whole warp.
+constexpr int AP_COST = 4, AP_ALL = 0x7fffffff;
+template <int TILES, int KT> struct ApRun {
+    int pair, h, nt;                                                 // where we are; the item's key tiles (one dead one if there is no key)
+    int a, e;                                                        // tiles of the piece
+    int64_t left, per;                                               // units of the run behind the piece; units of every run
+    __device__ __forceinline__ static void place(const Attn4Args &A, int blocks, int pair, int &b, int &r0) {
+        const int level = pair / A.sq.batch;
+        b = pair - level * A.sq.batch;
+        r0 = (blocks - 1 - level) * TILES * 128;
+    }
+    __device__ __forceinline__ static int tiles(const Attn4Args &A, int blocks, int pair) {   // 0: no such item
+        if (pair >= blocks * A.sq.batch) return 0;
+        int b, r0;
+        ApItem<TILES, KT> w;
+        place(A, blocks, pair, b, r0);
+        w.set(A, b, 0, r0, 0, AP_ALL, 0);
+        return r0 < w.rows ? max(w.nk, 1) : 0;
+    }
+    __device__ __forceinline__ static int64_t units(const Attn4Args &A, int nt) { return nt > 0 ? (int64_t)(nt + AP_COST) * A.kv.kv_heads : 0; }
+    __device__ __forceinline__ bool begin(const Attn4Args &A, int blocks) {
+        const int lane = threadIdx.x & 31, pairs = blocks * A.sq.batch;
+        int64_t total = 0;
+        for (int p = lane; p < pairs; p += 32) total += units(A, tiles(A, blocks, p));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)(AP_COST + 4));
+        const int64_t t0 = min(total, blockIdx.x * per), t1 = min(total, t0 + per);
+        left = t1 - t0;
+        if (left == 0) return false;
+        int64_t base = 0, inc;
+        int mine;
+        for (int p0 = 0;; p0 += 32) {
+            mine = tiles(A, blocks, p0 + lane);
+            inc = units(A, mine);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += up;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, base + inc > t0);
+            if (hit != 0) {
+                const int l = __ffs(hit) - 1;
+                pair = p0 + l;
+                nt = __shfl_sync(0xffffffffu, mine, l);
+                base += __shfl_sync(0xffffffffu, inc, l) - units(A, nt);
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        h = (int)((t0 - base) / (nt + AP_COST));
+        take((int)(t0 - base - (int64_t)h * (nt + AP_COST)));
+        return e > 0 || next(A, blocks);
+    }
+    __device__ __forceinline__ void take(int from) {                 // the piece that begins `from` units into its item
+        const int to = (int)min((int64_t)(nt + AP_COST), from + left);
+        left -= to - from;
+        a = max(0, from - AP_COST);
+        e = max(0, to - AP_COST);
+    }
+    __device__ __forceinline__ bool next(const Attn4Args &A, int blocks) {
+        do {
+            if (left == 0) return false;
+            if (++h == A.kv.kv_heads) {
+                h = 0;
+                do nt = tiles(A, blocks, ++pair); while (nt == 0);   // (units are left: there is one)
+            }
+            take(0);
+        } while (e == 0);
+        return true;
+    }
+};
+
 template <int D, int BS, typename T>
 __global__ void __launch_bounds__(AP_THREADS, 1)
-attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
+attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) {
     using S = ApSmem<D, BS>;
     constexpr int TILES = S::TILES, KT = S::KT, NB = D / BS, SOFF = KV4_GROUP * (D / 2), HALF = kv4_half_bytes(D, BS);
     constexpr bool BF = !std::is_same<T, __half>::value;
@@ -209,9 +287,9 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
     volatile float *k_pow = reinterpret_cast<volatile float *>(smem + S::BAR + 176);     // [4]: power of two of a K tile
     volatile int *v_exp = reinterpret_cast<volatile int *>(smem + S::BAR + 192);         // [4]: V's exponent from a tile on
     volatile uint8_t *q_exp = smem + S::EXPO;
-    volatile int *queue = reinterpret_cast<volatile int *>(smem + S::BAR + 208);         // [4][4]: items (sequence, or -1; head; row)
-    auto item_full = [&](int s) { return bar + 272 + 8u * s; };      // [4] each
-    auto item_empty = [&](int s) { return bar + 304 + 8u * s; };
+    volatile int *queue = reinterpret_cast<volatile int *>(smem + S::BAR + 208);         // [4][6]: items (sequence, or -1; head; row; key tiles; slot)
+    auto item_full = [&](int s) { return bar + 304 + 8u * s; };      // [4] each
+    auto item_empty = [&](int s) { return bar + 336 + 8u * s; };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -247,12 +325,13 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
     auto next_item = [&](Item &w, bool one) -> bool {
         const int s = turn_ & 3;
         if (!mbar_wait(item_full(s), (turn_ >> 2) & 1, abort_flag)) { atomicExch(&g_attn4_prompt_status, 424); *abort_flag = 1; return false; }
-        const int b = queue[4 * s], h = queue[4 * s + 1], r0 = queue[4 * s + 2];
+        volatile int *it = queue + 6 * s;
+        const int b = it[0], h = it[1], r0 = it[2], a = it[3], e = it[4], slot = it[5];
         if (!one) __syncwarp();
         if (one || lane == 0) mbar_arrive(item_empty(s));
         ++turn_;
         if (b < 0) return false;
-        w.set(A, b, h, r0);
+        w.set(A, b, h, r0, a, e, slot);
         return true;
     };
 #define AP_WAIT(b_, ph_, code_) if (!mbar_wait(b_, ph_, abort_flag)) { atomicExch(&g_attn4_prompt_status, code_); *abort_flag = 1; break; }
@@ -346,19 +425,47 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
             // -------------------------------------------------------- codes
             int jj = 0;
             ApList<TILES * 128> list;
-            list.begin(A, blocks);
+            ApRun<TILES, KT> run;
+            Attn4Join *join = attn4_join<D, TILES * 128>(A.ws, gridDim.x) + blockIdx.x;
+            bool more = true;
+            if (split) {
+                if (lane == 0) join->n = 0;
+                __syncwarp();
+                more = run.begin(A, blocks);
+            } else {
+                list.begin(A, blocks);
+            }
             for (int turn = 0; !*abort_flag; ++turn) {
-                int b = -1, h = 0, r0 = 0;
-                if (!list.find(A, (int64_t)turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), b, h, r0)) b = -1;
+                int b = -1, h = 0, r0 = 0, first = 0, end = AP_ALL, slot = -1;
+                if (split) {
+                    if (more) {
+                        run.place(A, blocks, run.pair, b, r0);
+                        h = run.h; first = run.a; end = run.e;
+                        if (first > 0 || end < run.nt) {
+                            slot = turn == 0 ? 0 : 1;                // (a piece between the first and the last is whole)
+                            if (first == 0 && lane == 0) {
+                                int row0, n, len;
+                                A.sq.get(b, row0, n, len);
+                                join->slot = slot;
+                                join->row0 = row0; join->rows = n * A.group; join->r = r0 / (TILES * 128); join->h = h;
+                                join->n = 1 + (int)((run.nt - end + run.per - 1) / run.per);
+                            }
+                        }
+                        more = run.next(A, blocks);
+                    }
+                } else if (!list.find(A, (int64_t)turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), b, h, r0)) {
+                    b = -1;
+                }
                 const int qs = turn & 3;
                 AP_WAIT(item_empty(qs), ((turn >> 2) & 1) ^ 1, 425);
                 if (lane == 0) {
-                    queue[4 * qs] = b; queue[4 * qs + 1] = h; queue[4 * qs + 2] = r0;
+                    volatile int *it = queue + 6 * qs;
+                    it[0] = b; it[1] = h; it[2] = r0; it[3] = first; it[4] = end; it[5] = slot;
                     mbar_arrive(item_full(qs));
                 }
                 if (b < 0) break;
                 Item w;
-                w.set(A, b, h, r0);
+                w.set(A, b, h, r0, first, end, slot);
                 for (int j = 0; j < w.nk; ++j, ++jj) {
                     const int st = jj & 1;
                     AP_WAIT(raw_empty(st), ((jj >> 1) & 1) ^ 1, 411);
@@ -771,10 +878,13 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
             float la, lb;
             ap_unpack2(l2, la, lb);
             const float l = la + lb;
-            const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l) * __int_as_float(max(1, ve - 8) << 23) * attn4_code_unscale(A.quant_type);
+            // a partial result: sums as they are, and the reference
+            const float up = w.nk > 0 ? __int_as_float(max(1, ve - 8) << 23) * attn4_code_unscale(A.quant_type) : 0.0f;
+            const float inv = l == 0.0f ? 0.0f : w.slot < 0 ? __fdividef(1.0f, l) * up : up;
             // Four lanes take 32 channels (64 bytes) of a row, eight rows at a time: with 16 bytes of 32 rows each, stores kept the
             // load and store unit busy 4 times as long.  (The order that V's channels have in O makes a lane's eight neighbours.)
-            const int64_t orow = live ? (int64_t)(w.row0 + i) * A.heads + w.h * A.group + g : -1;
+            float *const part = attn4_partial<D, TILES * 128>(A.ws, blockIdx.x, max(w.slot, 0));
+            const int64_t orow = !live ? -1 : w.slot >= 0 ? t * 128 + rr : (int64_t)(w.row0 + i) * A.heads + w.h * A.group + g;
             int64_t row4[4];
             float inv4[4];
 #pragma unroll
@@ -793,21 +903,26 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
                 }
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    uint32_t y[4];
+                    if (row4[x] < 0) continue;
+                    float y[8];                                      // (a row without keys: whatever v holds)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        T pr[2] = {from_f32<T>(0.0f), from_f32<T>(0.0f)};
-                        if (inv4[x] != 0.0f) {
-                            pr[0] = from_f32<T>(__uint_as_float(v[x >> 1][4 * e + 2 * (x & 1)]) * inv4[x]);
-                            pr[1] = from_f32<T>(__uint_as_float(v[x >> 1][4 * e + 2 * (x & 1) + 1]) * inv4[x]);
-                        }
-                        y[e] = *reinterpret_cast<const uint32_t *>(pr);
+                    for (int e = 0; e < 8; ++e) y[e] = inv4[x] != 0.0f ? __uint_as_float(v[x >> 1][4 * (e >> 1) + 2 * (x & 1) + (e & 1)]) * inv4[x] : 0.0f;
+                    if (w.slot < 0) {
+                        T z[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) z[e] = from_f32<T>(y[e]);
+                        *reinterpret_cast<uint4 *>(dst + row4[x] * D + c0) = *reinterpret_cast<const uint4 *>(z);
+                    } else {
+                        float *to = part + row4[x] * D + c0 + (lane & 3) * 8;
+                        *reinterpret_cast<float4 *>(to) = make_float4(y[0], y[1], y[2], y[3]);
+                        *reinterpret_cast<float4 *>(to + 4) = make_float4(y[4], y[5], y[6], y[7]);
                     }
-                    if (row4[x] >= 0) *reinterpret_cast<uint4 *>(dst + row4[x] * D + c0) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             }
             tc_fence_before();                                       // O has been read before the next item's P is announced
-            if (orow >= 0 && A.lse != nullptr) A.lse[orow] = l == 0.0f ? __int_as_float(0xff800000) : (m - AP_LIFT + __log2f(l)) * 0.69314718f;
+            if (w.slot >= 0) {
+                if (live) *reinterpret_cast<float2 *>(part + TILES * 128 * D + 2 * orow) = make_float2(m - AP_LIFT, l);
+            } else if (live && A.lse != nullptr) A.lse[orow] = l == 0.0f ? __int_as_float(0xff800000) : (m - AP_LIFT + __log2f(l)) * 0.69314718f;
         }
     }
 #undef AP_WAIT
@@ -823,7 +938,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks) {
 // host side
 // ------------------------------------------------------------------------------------------
 template <int D, int BS, typename T>
-static int ap_launch(const Attn4Args &a, cudaStream_t st) {
+static int ap_launch(const Attn4Args &a, bool split, cudaStream_t st) {
     using S = ApSmem<D, BS>;
     constexpr int smem = S::TOTAL;
     static_assert(smem <= 227 * 1024, "shared memory of the prompt kernel");
@@ -841,12 +956,19 @@ static int ap_launch(const Attn4Args &a, cudaStream_t st) {
     // no more blocks than there can be items: a sequence's last block of rows may be partly filled
     const int64_t most = a.kv.kv_heads * (((int64_t)a.sq.tokens * a.group) / (S::TILES * 128) + a.sq.batch);
     const int sms = sm_count();
-    attn4_prompt_kernel<D, BS, T><<<(int)(most < sms ? most : sms), AP_THREADS, smem, st>>>(a, (int)blocks);
-    return check_launch();
+    const int grid = split || most > sms ? sms : (int)most;
+    attn4_prompt_kernel<D, BS, T><<<grid, AP_THREADS, smem, st>>>(a, (int)blocks, split);
+    const int rc = check_launch();
+    return rc != MPSBNB_OK || !split ? rc : attn4_combine<D, S::TILES * 128, ATTN4_JOIN_WARPS, T>(a, grid, st);
 }
 
-int attn4_prompt(const Attn4Args &a, int head_dim, int blocksize, int dtype, cudaStream_t st) {
-#define AP_PICK(D, BS) return dtype == MPSBNB_F16 ? ap_launch<D, BS, __half>(a, st) : ap_launch<D, BS, __nv_bfloat16>(a, st)
+size_t attn4_prompt_ws(int head_dim) {
+    const int rows = head_dim == 256 ? 128 : 256;
+    return (size_t)sm_count() * (2 * rows * (head_dim + 2) * sizeof(float) + sizeof(Attn4Join));
+}
+
+int attn4_prompt(const Attn4Args &a, int head_dim, int blocksize, int dtype, bool split, cudaStream_t st) {
+#define AP_PICK(D, BS) return dtype == MPSBNB_F16 ? ap_launch<D, BS, __half>(a, split, st) : ap_launch<D, BS, __nv_bfloat16>(a, split, st)
     if (blocksize == 32) {
         if (head_dim == 64) AP_PICK(64, 32);
         if (head_dim == 128) AP_PICK(128, 32);

@@ -174,6 +174,7 @@ CASES = [
     (64, 32, 128, "nf4", F16, 5, 1, [3], [2000], True, 1),
     (256, 64, 64, "nf4", F16, 4, 2, [1, 1], [513, 90], True, None),
     (256, 32, 32, "fp4", BF16, 16, 1, [1, 2], [700, 33], True, 100),
+    (256, 32, 32, "nf4", F16, 16, 2, [1, 2], [700, 333], True, None),
     (128, 32, 64, "nf4", BF16, 24, 2, [1, 1], [400, 41], True, None),          # 12 rows a head: 16-row tiles
     (128, 64, 64, "nf4", F16, 40, 1, [1], [1500], True, None),                 # 40 rows: three tiles
     (128, 64, 64, "nf4", F16, 7, 7, [5, 1, 0, 8], [5, 33, 20, 100], True, None),
@@ -194,12 +195,35 @@ CASES = [
     (64, 64, 16, "fp4", BF16, 16, 16, [700, 1], [701, 5], True, None),
     (256, 32, 64, "nf4", BF16, 8, 1, [511], [900], False, None),
     (128, 64, 32, "nf4", F16, 8, 8, [900, 0, 1100], [900, 20, 1111], True, None),
+    # ... and more blocks of rows than two rounds over the card
+    (128, 64, 64, "nf4", BF16, 64, 16, [100, 33, 256, 64, 1, 17, 0, 130, 70, 90] * 2, [177, 33, 400, 64, 5, 99, 50, 131, 700, 90] * 2, True, None),
+    (128, 32, 32, "fp4", F16, 32, 16, [140, 99] * 10, [200, 99] * 10, True, 70),
+    (64, 64, 16, "nf4", F16, 32, 16, [200, 301] * 7, [200, 310] * 7, False, None),
+    (64, 32, 64, "nf4", BF16, 16, 16, [513, 400, 300, 600] * 3, [513, 499, 300, 601] * 3, True, None),
+    (256, 64, 64, "fp4", BF16, 32, 16, [65, 129, 64] * 4, [190, 140, 64] * 4, True, None),
+    (256, 32, 16, "nf4", F16, 16, 16, [130, 260, 190, 129] * 2, [131, 300, 250, 129] * 2, True, 150),
+    # an item shared by many blocks
+    (128, 64, 64, "nf4", F16, 16, 1, [33], [20000], True, None),
+    (256, 64, 64, "nf4", BF16, 8, 1, [16, 40], [9000, 40], True, 5000),
+    (64, 32, 16, "fp4", BF16, 20, 1, [50, 1, 13], [50, 700, 8000], False, None),
 ]
-PROMPTS = [c for c in CASES if (lambda rows: len(c[7]) * c[6] * -(-rows // 16) > {64: 700, 128: 430, 256: 225}[c[0]])(sum(c[7]) * (c[5] // c[6]) / len(c[7]))]
 
 
-def test_both_kernels_are_covered():
-    assert len(PROMPTS) == 11 and len(CASES) - len(PROMPTS) == 17 and {c[:2] for c in PROMPTS} == {(d, b) for d in (64, 128, 256) for b in (32, 64)}
+def _kernel(case, sms):
+    """Which kernel the case's shape should go to: by 16-row tiles and blocks of 256 (128) rows of all sequences and heads."""
+    head_dim, new, kv_heads, group = case[0], case[7], case[6], case[5] // case[6]
+    rows, lists, block = -(-sum(new) * group // len(new)), len(new) * kv_heads, 128 if head_dim == 256 else 256
+    blocks, tiles, meet = lists * -(-rows // block), lists * -(-rows // 16), {64: 700, 128: 430, 256: 225}[head_dim]
+    split = lists * -(-max(new) * group // block) <= 2 * sms
+    if rows <= 16 or tiles * sms <= meet * (blocks if split else -(-blocks // sms) * sms):
+        return "tokens"
+    return "prompts, split" if split else "prompts"
+
+
+def test_all_kernels_are_covered():
+    kinds = [(_kernel(c, torch.cuda.get_device_properties(0).multi_processor_count), c[0], c[1]) for c in CASES]
+    assert set(kinds) == {(k, d, b) for k in ("tokens", "prompts", "prompts, split") for d in (64, 128, 256) for b in (32, 64)}
+    assert [sum(k[0] == x for k in kinds) for x in ("tokens", "prompts, split", "prompts")] == [12, 20, 6]
 
 
 def _problem(case, seed=0, k_size=1.0, v_size=1.0):
