@@ -629,20 +629,26 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
 static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return (int64_t)s->new_tokens * group > 8 ? 2 : 1; }
 
 // The tensor-core kernel of attn4_prompt.cu instead?  A key tile costs it the same whether its rows are 16 or 256: 2.0, 2.4, 3.3 us
-// per 128 keys and block (head_dim 64, 128, 256).  The kernel here spreads any amount of work over the whole card, at 0.42, 0.70,
-// 1.83 ns per 16 rows x 16 keys.  They meet where the 16-row tiles of all sequences and heads number 700, 430, 225 per round of
-// blocks over the card.  (Measured for 1 - 16 sequences, 1 - 8 heads, 16 - 2048 rows a head.)
-// Few blocks of rows (under AD_SPLIT rounds) share out the keys as well, and then a part of a round counts as that.
+// per 128 keys and block of rows on an SM (head_dim 64, 128, 256).  The kernel here spreads any amount of work over the whole card,
+// at 0.42, 0.70, 1.83 ns per 16 rows x 16 keys, and begins and ends sooner, by 15, 20, 6 us.  So prompts go there when
+// keys * (16-row tiles - 4.7, 2.9, 1.5 * blocks of rows) is above 570, 450, 50 thousand.  The keys are those that the table has room
+// for: what the lengths are is known on the device alone.  (Measured for 1 - 8 sequences, 1 and 8 heads, 20 - 4096 rows a head and
+// 1024 - 32768 keys.  8 heads, head_dim 128, here and there, us: 8192 keys of 64 rows 32 and 42, 256 rows 71 and 50, 1024 rows 210
+// and 71; 1024 keys of 256 rows 28 and 46, 4096 rows 153 and 50.)
+// Few blocks of rows (under AD_SPLIT rounds over the card) share out the keys as well; of many, a round begun counts as a whole one.
 constexpr int AD_SPLIT = 2;
 enum AdKind { AD_TOKENS, AD_PROMPTS, AD_PROMPTS_SPLIT };
-static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group) {
+static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group, int window) {
     const int64_t rows = (s->tokens * group + s->batch - 1) / s->batch;   // of a sequence and head, on average
     const int64_t lists = (int64_t)s->batch * c->kv_heads, block = c->head_dim == 256 ? 128 : 256, sms = sm_count();
     const int64_t blocks = lists * ((rows + block - 1) / block), tiles = lists * ((rows + 15) / 16);
-    const int64_t meet = c->head_dim == 64 ? 700 : c->head_dim == 128 ? 430 : 225;
     // (every block of the card looks through the (sequence, block of rows) pairs, 32 at a time)
     const bool split = lists * (((int64_t)s->new_tokens * group + block - 1) / block) <= AD_SPLIT * sms;
-    if (rows <= 16 || tiles * sms <= meet * (split ? blocks : (blocks + sms - 1) / sms * sms)) return AD_TOKENS;
+    double keys = (double)s->table_width * c->page_size;
+    if (window > 0 && keys > (double)window + s->new_tokens) keys = (double)window + s->new_tokens;
+    const int at = c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2;
+    const double meet[3] = {4.7, 2.9, 1.5}, sooner[3] = {570e3, 450e3, 50e3};
+    if (rows <= 16 || keys * (tiles - meet[at] * (split ? blocks : (blocks + sms - 1) / sms * sms)) <= sooner[at]) return AD_TOKENS;
     return split ? AD_PROMPTS_SPLIT : AD_PROMPTS;
 }
 
@@ -688,9 +694,10 @@ extern "C" size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *
     if (kv4_check_cache(cache, 0) != MPSBNB_OK || kv4_check_seqs(seqs, cache) != MPSBNB_OK) return 0;
     if (heads <= 0 || heads % cache->kv_heads != 0 || seqs->batch == 0 || seqs->tokens == 0) return 0;
     const int nt = ad_nt(seqs, heads / cache->kv_heads);
-    const AdKind kind = ad_kind(cache, seqs, heads / cache->kv_heads);
-    if (kind != AD_TOKENS) return kind == AD_PROMPTS ? 16 : attn4_prompt_ws(cache->head_dim);   // (16: not used)
-    return (size_t)ad_teams(cache->head_dim, nt) * (2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float) + sizeof(Attn4Join));
+    const size_t tokens = (size_t)ad_teams(cache->head_dim, nt) * (2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float) + sizeof(Attn4Join));
+    // (a window, not known here, may lead from the prompt kernel to the other, not back)
+    const size_t prompts = ad_kind(cache, seqs, heads / cache->kv_heads, 0) == AD_PROMPTS_SPLIT ? attn4_prompt_ws(cache->head_dim) : 0;
+    return tokens > prompts ? tokens : prompts;
 }
 
 extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
@@ -717,7 +724,7 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.scale_log2 = scale * 1.4426950408889634f;
     static const float codes[2][16] = {MPSBNB_NF4_TABLE, MPSBNB_FP4_TABLE};
     for (int i = 0; i < 16; ++i) a.code[i] = codes[cache->quant_type][i] * attn4_code_scale(cache->quant_type);
-    const AdKind kind = ad_kind(cache, seqs, group);
+    const AdKind kind = ad_kind(cache, seqs, group, window);
     if (kind != AD_TOKENS) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, kind == AD_PROMPTS_SPLIT, (cudaStream_t)stream);
     const int nt = ad_nt(seqs, group);
     cudaStream_t st = (cudaStream_t)stream;

@@ -27,6 +27,13 @@ def random_table(batch, width, pages, seed=0):
     return torch.randperm(pages, generator=gen)[:batch * width].view(batch, width).to(torch.int32).cuda()
 
 
+def widen(table, page):
+    """The table with room for 128 K places, of entries that no key needs: prompts then go to the prompt kernel."""
+    wide = torch.full((table.shape[0], max(table.shape[1], (1 << 17) // page)), -1, dtype=torch.int32, device=table.device)
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
 def rows_of(cache, layer, pages, first, last, name):
     """[last - first, kv heads, head_dim] in 64 bits: the values of places first .. last - 1."""
     place = torch.arange(first, last, device="cuda")

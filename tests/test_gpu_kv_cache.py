@@ -209,21 +209,24 @@ CASES = [
 ]
 
 
-def _kernel(case, sms):
-    """Which kernel the case's shape should go to: by 16-row tiles and blocks of 256 (128) rows of all sequences and heads."""
-    head_dim, new, kv_heads, group = case[0], case[7], case[6], case[5] // case[6]
+def _kernel(case, sms, places):
+    """Which kernel the case's shape should go to: by 16-row tiles and blocks of 256 (128) rows of all sequences and heads, and by the
+    places that the table has room for."""
+    head_dim, new, kv_heads, group, window = case[0], case[7], case[6], case[5] // case[6], case[10]
     rows, lists, block = -(-sum(new) * group // len(new)), len(new) * kv_heads, 128 if head_dim == 256 else 256
-    blocks, tiles, meet = lists * -(-rows // block), lists * -(-rows // 16), {64: 700, 128: 430, 256: 225}[head_dim]
+    blocks, tiles = lists * -(-rows // block), lists * -(-rows // 16)
+    meet, sooner = {64: (4.7, 570e3), 128: (2.9, 450e3), 256: (1.5, 50e3)}[head_dim]
     split = lists * -(-max(new) * group // block) <= 2 * sms
-    if rows <= 16 or tiles * sms <= meet * (blocks if split else -(-blocks // sms) * sms):
+    keys = min(places, window + max(new)) if window else places
+    if rows <= 16 or keys * (tiles - meet * (blocks if split else -(-blocks // sms) * sms)) <= sooner:
         return "tokens"
     return "prompts, split" if split else "prompts"
 
 
 def test_all_kernels_are_covered():
-    kinds = [(_kernel(c, torch.cuda.get_device_properties(0).multi_processor_count), c[0], c[1]) for c in CASES]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    kinds = [(_kernel(c, sms, 1 << 17), c[0], c[1]) for c in CASES] + [(_kernel(c, sms, max(c[8])), c[0], c[1]) for c in CASES]
     assert set(kinds) == {(k, d, b) for k in ("tokens", "prompts", "prompts, split") for d in (64, 128, 256) for b in (32, 64)}
-    assert [sum(k[0] == x for k in kinds) for x in ("tokens", "prompts, split", "prompts")] == [12, 20, 6]
 
 
 def _problem(case, seed=0, k_size=1.0, v_size=1.0):
@@ -244,16 +247,17 @@ def test_attention(case):
     cache, table, starts, q = _problem(case)
     new, lens, causal, window = case[7:]
     want, want_lse, bound = U.attention(q, cache, 1, table, lens, starts, causal, window)
-    got, lse = bnb.attention_4bit(q, cache, 1, table, _i32(lens), _i32(starts), max(new), causal, window, return_lse=True)
-    U.check(got, want, bound, case[4])
-    # scores are off by about 2^-11 of sum |q k| / sqrt(D) at most
-    err = 2.0 ** -11 * 16 + 2.0 ** -20 * want_lse.abs()
-    assert ((lse.double() - want_lse).abs() <= err).all()
-    again = bnb.attention_4bit(q, cache, 1, table, _i32(lens), _i32(starts), max(new), causal, window)
-    assert torch.equal(got, again)                                   # same bits each time
-    if len(set(new)) == 1:
-        even = bnb.attention_4bit(q.view(len(new), new[0], *q.shape[1:]), cache, 1, table, _i32(lens), causal=causal, window=window)
-        assert torch.equal(even.flatten(0, 1), got)
+    for table in (table, U.widen(table, case[2])):                   # prompts: both kernels
+        got, lse = bnb.attention_4bit(q, cache, 1, table, _i32(lens), _i32(starts), max(new), causal, window, return_lse=True)
+        U.check(got, want, bound, case[4])
+        # scores are off by about 2^-11 of sum |q k| / sqrt(D) at most
+        err = 2.0 ** -11 * 16 + 2.0 ** -20 * want_lse.abs()
+        assert ((lse.double() - want_lse).abs() <= err).all()
+        again = bnb.attention_4bit(q, cache, 1, table, _i32(lens), _i32(starts), max(new), causal, window)
+        assert torch.equal(got, again)                               # same bits each time
+        if len(set(new)) == 1:
+            even = bnb.attention_4bit(q.view(len(new), new[0], *q.shape[1:]), cache, 1, table, _i32(lens), causal=causal, window=window)
+            assert torch.equal(even.flatten(0, 1), got)
     assert_device_ok()
 
 
@@ -268,7 +272,7 @@ def test_many_sequences_of_all_kinds(head_dim, heads, kv_heads):
     lens = [rng.choice([0, n // 2, n, n, n + rng.randint(0, 60), rng.randint(0, 160)]) for n in news]
     starts = _starts(news)
     cache = U.make_cache(180 * 6, kv_heads, head_dim, 32, seed=6)
-    table = U.random_table(180, 6, 180 * 6)
+    table = U.widen(U.random_table(180, 6, 180 * 6), 32)
     q = torch.randn(starts[-1], heads, head_dim, device="cuda", dtype=F16)
     for window in (None, 23):
         want, want_lse, bound = U.attention(q, cache, 0, table, lens, starts, window=window)
@@ -285,7 +289,7 @@ def test_rows_without_keys_are_zero_and_rows_past_the_last_sequence_stay(heads, 
     news, lens = [2, new, 0, 3, new], [0, 4, 30, 3, new + 100]
     starts = _starts(news)
     cache = U.make_cache(5 * 5, kv_heads, 128, seed=2)
-    table = U.random_table(5, 5, 25)
+    table = U.widen(U.random_table(5, 5, 25), 64)
     q = torch.randn(starts[-1] + 4, heads, 128, device="cuda", dtype=F16)
     want, want_lse, bound = U.attention(q, cache, 0, table, lens, starts)
     out = torch.full_like(q, 7.0)
@@ -306,7 +310,7 @@ def test_what_lies_in_unseen_places_does_not_matter(dtype, new, kv_heads):
     import kv_util as U
     lens, window = [200, 333], 90
     cache = U.make_cache(13, kv_heads, 128, dtype=dtype, seed=5)
-    table = U.random_table(2, 6, 13, seed=1)
+    table = U.widen(U.random_table(2, 6, 13, seed=1), 64)
     q = torch.randn(2, new, 4 * kv_heads, 128, device="cuda").to(dtype)
     clean = bnb.attention_4bit(q, cache, 0, table, _i32(lens), window=window)
     bad = torch.ones(13, 64, dtype=torch.bool, device="cuda")       # pages, places
@@ -328,6 +332,7 @@ def test_magnitudes_and_scales(new, kv_heads, k_size, v_size, scale):
     import kv_util as U
     case = (128, 64, 64, "nf4", BF16, 4 * kv_heads, kv_heads, [new, new], [400, 1100], True, None)
     cache, table, starts, q = _problem(case, 3, k_size, v_size)
+    table = U.widen(table, 64)
     # values of very different size beside one another, the first of them the largest by far
     cache.v_absmax[:, :, :, 0, 0] *= 2.0 ** 6
     cache.v_absmax[:, :, :, 1:] *= 2.0 ** -6
@@ -355,7 +360,7 @@ def test_a_page_outside_the_cache_gives_nan_and_a_status(new, kv_heads):
     import kv_util as U
     from mps_bitsandbytes_b200 import _native as N
     cache = U.make_cache(9, kv_heads, 128)
-    table = U.random_table(3, 3, 9)
+    table = U.widen(U.random_table(3, 3, 9), 64)
     q = torch.randn(3, new, 4 * kv_heads, 128, device="cuda", dtype=F16)
     lens = _i32([150, 190, 150])
     clean = bnb.attention_4bit(q, cache, 0, table, lens)
@@ -421,8 +426,8 @@ def test_offsets_beyond_32_bits():
     want = bnb.attention_4bit(q, small, 0, _i32([[0, 1, 2], [3, 4, 5]]), lens)
     assert torch.equal(bnb.attention_4bit(q, cache, 2, table, lens), want)
     q = torch.randn(2, 400, 16, 64, device="cuda", dtype=F16)         # 16 lists of 50 row tiles: the prompt kernel
-    want = bnb.attention_4bit(q, small, 0, _i32([[0, 1, 2], [3, 4, 5]]), lens)
-    assert torch.equal(bnb.attention_4bit(q, cache, 2, table, lens), want)
+    want = bnb.attention_4bit(q, small, 0, U.widen(_i32([[0, 1, 2], [3, 4, 5]]), 256), lens)
+    assert torch.equal(bnb.attention_4bit(q, cache, 2, U.widen(table, 256), lens), want)
     k, _ = bnb.dequantize_kv_4bit(cache, 2, table, lens, 700)
     assert torch.equal(k, bnb.dequantize_kv_4bit(small, 0, _i32([[0, 1, 2], [3, 4, 5]]), lens, 700)[0])
     x = torch.randn(2, 9, 8, 64, device="cuda", dtype=F16)
@@ -433,11 +438,12 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(cache.data[:, 11000], cache.data[:, 11999]) and cache.data[2, 11000].any()
 
 
-def test_graph_replays_follow_lengths_and_two_graphs_do_not_share_workspaces():
+@pytest.mark.parametrize("new", [1, 45, 700])                        # each kernel
+def test_graph_replays_follow_lengths_and_two_graphs_do_not_share_workspaces(new):
     import kv_util as U
     cache = U.make_cache(33, 8, 128)
-    table = U.random_table(2, 16, 33)
-    q = [torch.randn(2, 1, 64, 128, device="cuda", dtype=F16) for _ in range(2)]
+    table = U.widen(U.random_table(2, 16, 33), 64)
+    q = [torch.randn(2, new, 64, 128, device="cuda", dtype=F16) for _ in range(2)]
     lens = [_i32([700, 40]), _i32([3, 1000])]
     eager = lambda i: bnb.attention_4bit(q[i], cache, 0, table, lens[i])
     side = torch.cuda.Stream()
@@ -466,11 +472,12 @@ def test_graph_replays_follow_lengths_and_two_graphs_do_not_share_workspaces():
     assert_device_ok()
 
 
-def test_calls_on_two_streams_at_once():
+@pytest.mark.parametrize("new", [1, 60, 3000])                       # each kernel
+def test_calls_on_two_streams_at_once(new):
     import kv_util as U
     cache = U.make_cache(65, 4, 128)
-    table = U.random_table(1, 64, 65)
-    qs = [torch.randn(1, 1, 32, 128, device="cuda", dtype=F16) for _ in range(2)]
+    table = U.widen(U.random_table(1, 64, 65), 64)
+    qs = [torch.randn(1, new, 32, 128, device="cuda", dtype=F16) for _ in range(2)]
     lens = [_i32([4000]), _i32([3333])]
     want = [bnb.attention_4bit(q, cache, 0, table, n) for q, n in zip(qs, lens)]
     torch.cuda.synchronize()
