@@ -70,7 +70,7 @@ attn4_combine_kernel(const __grid_constant__ Attn4Args A, int runs) {
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) v[j] = 0.0f;
 #pragma unroll 4
-    for (int x = ROWS == 1 ? warp : 0; x < p.n; x += ROWS == 1 ? ATTN4_JOIN_WARPS : 1) {
+    for (int x = ROWS == 1 ? warp : 0; x < min(p.n, runs - c0); x += ROWS == 1 ? ATTN4_JOIN_WARPS : 1) {
         const float *q = attn4_partial<D, RT>(A.ws, c0 + x, x == 0 ? p.slot : 0);
         const float2 ml = *reinterpret_cast<const float2 *>(q + RT * D + 2 * row);
         const float mn = fmaxf(M, ml.x), ko = ex2(M - mn), kn = ex2(ml.x - mn);

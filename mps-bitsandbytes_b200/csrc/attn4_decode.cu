@@ -21,6 +21,7 @@
 //    exceeds it by 2^8: one vote per tile instead of a reduction, and fp32 sums lose nothing by it.  The weight
 //    p * absmax goes to fp16; absmax is taken times a power of two that is lowered, in the same vote, when it exceeds 2^7.
 //    bf16 queries are brought to fp16 by a power of two per row: exact, but for parts below 2^-24 of the row's largest.
+#include <cmath>
 #include <type_traits>
 
 #include "attn4.cuh"
@@ -132,12 +133,14 @@ template <class S> struct AdPiece {
     int a, e;                                    // key tiles of the piece, relative to s.tlo
     int64_t left;                                // units of the run after this piece
 
-    // first piece of the run [t0, t1) of the whole list (false: the run holds none of its tiles); whole warp.
+    // first piece of the run [t0, t1) of the whole list (false: the run holds none of its tiles); whole warp.  (The ends of the
+    // walk are checked: lengths that change under a running kernel must not lead it outside.)
     // w: units of sequence `lane`
     __device__ __forceinline__ bool start(const Attn4Args &A, int64_t w, int64_t t0, int64_t t1) {
         const int lane = threadIdx.x & 31;
         int64_t base = 0;
         for (int b0 = 0;; b0 += 32) {
+            if (b0 >= A.sq.batch) return false;
             if (b0 > 0) w = ad_units<S>(A, b0 + lane);
             int64_t inc = w;
 #pragma unroll
@@ -178,7 +181,10 @@ template <class S> struct AdPiece {
                 r = 0;
                 if (++h == A.kv.kv_heads) {
                     h = 0;
-                    do { ++b; s.get<S>(A, b); } while (s.nt == 0);
+                    do {
+                        if (++b >= A.sq.batch) return false;
+                        s.get<S>(A, b);
+                    } while (s.nt == 0);
                 }
             }
             take(0);
@@ -706,7 +712,7 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     int rc = kv4_check_cache(cache, layer);
     if (rc == MPSBNB_OK) rc = kv4_check_seqs(seqs, cache);
     if (rc != MPSBNB_OK) return rc;
-    if (heads <= 0 || heads % cache->kv_heads != 0 || window < 0 || (window > 0 && !causal)) return MPSBNB_ERR_INVALID_ARG;
+    if (heads <= 0 || heads % cache->kv_heads != 0 || window < 0 || (window > 0 && !causal) || !(fabsf(scale) < INFINITY)) return MPSBNB_ERR_INVALID_ARG;
     if (q_token_stride < 0 || q_head_stride < 0) return MPSBNB_ERR_INVALID_ARG;
     if (seqs->batch == 0 || seqs->tokens == 0 || seqs->new_tokens == 0) return MPSBNB_OK;
     if (q == nullptr || out == nullptr) return MPSBNB_ERR_INVALID_ARG;

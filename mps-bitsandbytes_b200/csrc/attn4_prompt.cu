@@ -219,6 +219,7 @@ template <int TILES, int KT> struct ApRun {
         int64_t base = 0, inc;
         int mine;
         for (int p0 = 0;; p0 += 32) {
+            if (p0 >= pairs) return false;                           // (lengths that change under a running kernel)
             mine = tiles(A, blocks, p0 + lane);
             inc = units(A, mine);
 #pragma unroll
@@ -251,7 +252,10 @@ template <int TILES, int KT> struct ApRun {
             if (left == 0) return false;
             if (++h == A.kv.kv_heads) {
                 h = 0;
-                do nt = tiles(A, blocks, ++pair); while (nt == 0);   // (units are left: there is one)
+                do {
+                    if (++pair >= blocks * A.sq.batch) return false;
+                    nt = tiles(A, blocks, pair);
+                } while (nt == 0);
             }
             take(0);
         } while (e == 0);

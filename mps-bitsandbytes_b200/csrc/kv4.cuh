@@ -78,8 +78,8 @@ inline int kv4_check_seqs(const mpsbnb_kv4_seqs *s, const mpsbnb_kv4_cache *c) {
     if (s->batch == 0) return MPSBNB_OK;
     if (s->seq_lens == nullptr || (s->table_width > 0 && (s->page_table == nullptr || s->table_ld < s->table_width))) return MPSBNB_ERR_INVALID_ARG;
     if (s->cu_seqlens == nullptr && (int64_t)s->batch * s->new_tokens != s->tokens) return MPSBNB_ERR_INVALID_ARG;
-    // places and rows are 32-bit numbers in the kernels (a sequence of 2^30 tokens, 2^31 rows)
-    if ((int64_t)s->table_width * c->page_size > (1ll << 30) || s->tokens > 0x7fffffffll) return MPSBNB_ERR_TOO_LARGE;
+    // places and rows are 32-bit numbers in the kernels, with room for a step beyond the last
+    if ((int64_t)s->table_width * c->page_size > (1ll << 30) || s->tokens > (1ll << 30)) return MPSBNB_ERR_TOO_LARGE;
     return MPSBNB_OK;
 }
 

@@ -377,6 +377,9 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
         out = q.new_empty(q.shape) if cu_seqlens is None else q.new_zeros(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}, 16-byte aligned")
+    elif out.untyped_storage().data_ptr() == qr.untyped_storage().data_ptr():
+        qr = qr.clone(memory_format=torch.contiguous_format)   # rows of q are read after others' outputs have been written
+        token, head = heads * cache.head_dim, cache.head_dim
     lse = None
     if return_lse:
         lse = torch.full(q.shape[:-1], float("-inf"), dtype=torch.float32, device=q.device)
@@ -384,7 +387,7 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
     nbytes = lib.mpsbnb_attention_4bit_workspace_bytes(cache._ref, sq, heads)
     ws = cache.data.new_empty(nbytes)
     _call(cache, "attention_4bit", lib.mpsbnb_attention_4bit, cache._ref, layer, sq, qr.data_ptr(), token, head, heads,
-          1 if causal else 0, window or 0, cache.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+          1 if causal else 0, 0 if window is None else min(window, 1 << 30), cache.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
           None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 

@@ -414,6 +414,23 @@ def test_strided_queries_and_tables():
     assert torch.equal(bnb.attention_4bit(wide_rows[..., :64], cache, 0, big, lens), want)
 
 
+@pytest.mark.parametrize("new", [1, 70])
+def test_output_over_the_queries_and_windows_of_any_size(new):
+    import kv_util as U
+    cache = U.make_cache(24, 2, 128, seed=4)
+    table = U.widen(U.random_table(3, 8, 24), 64)
+    q = torch.randn(3, new, 32, 128, device="cuda", dtype=F16)
+    lens = _i32([500, 70, 333])
+    want = bnb.attention_4bit(q, cache, 0, table, lens)
+    for window in (1 << 20, 1 << 30, 1 << 31, (1 << 32) + 1):
+        assert torch.equal(bnb.attention_4bit(q, cache, 0, table, lens, window=window), want)
+    with pytest.raises(RuntimeError, match="attention_4bit failed"):
+        bnb.attention_4bit(q, cache, 0, table, lens, scale=math.nan)
+    for _ in range(3):
+        x = q.clone()
+        assert bnb.attention_4bit(x, cache, 0, table, lens, out=x) is x and torch.equal(x, want)
+
+
 def test_offsets_beyond_32_bits():
     import kv_util as U
     # a page is 2 * 256 * 36 * 8 bytes (147 KB); 3 layers of 12000 pages: 5.3 GB
