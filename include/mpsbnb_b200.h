@@ -450,7 +450,7 @@ typedef struct mpsbnb_kv4_cache {
  * row of the page table can hold) in the pages page_table[b * table_ld + 0 ...].  Its new tokens are rows
  * cu_seqlens[b] ... cu_seqlens[b + 1] - 1 of the call's [tokens, ...] tensors, or rows b * new_tokens ... with
  * cu_seqlens NULL; they take the last places of the sequence.  new_tokens is the largest number of new tokens of a
- * sequence (more are not looked at).  All tables are int32 on the device. */
+ * sequence (more are not looked at).  All tables are int32 on the device; they must not change while a call reads them. */
 typedef struct mpsbnb_kv4_seqs {
     const int32_t *page_table;
     int64_t table_ld;
@@ -487,8 +487,14 @@ int mpsbnb_kv4_copy_pages(const mpsbnb_kv4_cache *cache, const int32_t *src, con
  * (window must then be 0).  A row that sees no key gives zeros and lse = -inf.  Rows past cu_seqlens[batch] are left
  * as they were.  A row that sees a page outside the cache gives NaN (device status 401).
  *   q    [tokens, heads, head_dim] in the cache's dtype, strides in elements (multiples of 8), head_dim contiguous
- *   out  [tokens, heads, head_dim] contiguous, in the cache's dtype; q and out 16-byte aligned;  lse  NULL or fp32 [tokens, heads], natural log
- * Scores, softmax statistics and sums are fp32; probabilities and codes enter the products as fp16.
+ *   out  [tokens, heads, head_dim] contiguous, in the cache's dtype, not over q; q and out 16-byte aligned
+ *   lse  NULL or fp32 [tokens, heads], natural log
+ *   scale  finite
+ * Scores, softmax statistics and sums are fp32.  fp16 products: single tokens round the 16 code values and the weights
+ * probability * absmax, prompts code * absmax (keys and values) and the probabilities.
+ * A key whose absmax is not finite makes the rows that see it NaN; a value's makes NaN of its block's channels in those rows
+ * (single tokens) or of the rows (prompts).  Which of two kernels runs - and with it the rounding - depends on the numbers of rows,
+ * heads and sequences and on table_width, the room for keys: never on the lengths, so a captured graph follows them.
  * workspace: mpsbnb_attention_4bit_workspace_bytes() bytes, 16-byte aligned, used by this call only while it runs. */
 size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads);
 int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,

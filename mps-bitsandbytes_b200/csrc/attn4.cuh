@@ -51,7 +51,8 @@ template <int D, int RT> __device__ __forceinline__ Attn4Join *attn4_join(float 
     return reinterpret_cast<Attn4Join *>(ws + (int64_t)runs * 2 * RT * (D + 2));
 }
 
-// Joins partial results: sum of 2^(m_i - M) O_i over sum of 2^(m_i - M) l_i.  A block takes ROWS rows of what one run began and
+// Joins partial results: sum of 2^(m_i - M) O_i over sum of 2^(m_i - M) l_i.  Bound by the partials' bytes and by its launch: 444
+// runs of single tokens (8 rows of 128, 4 MB) 4 us behind the other kernel, 148 of prompts (256 rows, 39 MB) 14.  A block takes ROWS rows of what one run began and
 // others went on with: one, whose parts its warps share, each with a running reference of its own (single tokens: up to hundreds
 // of parts), or one for each warp (prompts: many rows, few parts).
 constexpr int ATTN4_JOIN_WARPS = 4;

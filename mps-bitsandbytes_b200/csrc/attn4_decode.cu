@@ -1,8 +1,13 @@
 // Attention over the paged 4-bit cache for few query rows per sequence (single tokens, drafts) - and, row tile by row
 // tile, for any number of them.  out = softmax(scale q K^T) V, K = code * absmax, V = code * absmax.
 //
-// Bound: HBM, for the cached bytes (head_dim / 2 + 2 head_dim / blocksize per token, head and side) are read once and
-// the arithmetic per byte is small; what stands in the way is turning 4-bit codes into operands at that rate.
+// Floor: HBM, for the cached bytes (head_dim / 2 + 2 head_dim / blocksize per token, head and side) are read once and
+// the arithmetic per byte is small.  Bound: turning 4-bit codes into operands at that rate.  64 sequences of up to 16384 places
+// (8 kv heads of 128, 8 query heads each: 545 MB) take 151 us, 3.6 TB/s, 0.55 of what a copy reaches; 57 % of the issue slots and 61 %
+// of the load pipe are then in use (326 instructions and 128 look-ups a lane for 16 tokens), the tensor pipe at 22 %.  Tried for it:
+// 8 warps a block (+20 %) and 16 (=) for 12; codes straight from global memory instead of the ring (+10 %); the next tile's
+// scores under this one's values (=); all look-ups of a block before its products (=).
+// Little work is bound by latency: 15 - 20 us for two launches, however short the sequences are.
 //
 //  * Work is a list of (sequence, kv head, row tile, key tile), cut into equal runs, one per team of four warps,
 //    whatever the sequences' lengths are: the lengths are read on the device, so a captured graph follows them.
@@ -19,7 +24,10 @@
 //    with the rounding of the 16 code values to fp16 only.
 //  * Softmax: probabilities are 2^(x - m) with a reference m that follows the running maximum only when a score
 //    exceeds it by 2^8: one vote per tile instead of a reduction, and fp32 sums lose nothing by it.  The weight
-//    p * absmax goes to fp16; absmax is taken times a power of two that is lowered, in the same vote, when it exceeds 2^7.
+//    p * absmax goes to fp16 (off by 2^-11 at most, 2.1e-4 in the root mean square; a second fp16 for the rest would cost a third
+//    more products and conversions): an output is off by 2.9e-4 - 3.6e-4 of its size, where its own rounding to fp16 makes 2.1e-4;
+//    in bf16 nothing is to be seen of it.  absmax is taken times a power of two that is lowered, in the same vote, when it
+//    exceeds 2^7.
 //    bf16 queries are brought to fp16 by a power of two per row: exact, but for parts below 2^-24 of the row's largest.
 #include <cmath>
 #include <type_traits>

@@ -1,7 +1,13 @@
 // Attention over the paged 4-bit cache for many query rows per sequence (prompts): out = softmax(scale q K^T) V on the
 // 5th-generation tensor cores, K and V expanded from their codes into operand tiles in shared memory.
 //
-// Bound: the tensor pipe (4 rows keys head_dim operations) and, close behind, the exponentials (16 a clock and SM).
+// Floor: the tensor pipe (4 rows keys head_dim operations) and, level with it at head_dim 128, the exponentials (16 a clock
+// and SM).  A tile of 256 rows and 128 keys: 2050 clocks for the products, 2050 for the powers, 3200 of shared memory (look-ups of
+// codes 1000, expanded operands written 500 and read by the products 1500 - 1700); it takes about 4400.  64 heads on 8 of 128,
+// 4096 tokens, causal: 344 us, 0.8 PFLOP/s of what the mask leaves, tensor pipe 40 - 44 % busy.
+// Without the expanders' arithmetic it takes 303 us, without the softmax's 231, without both 198: what is left is products and
+// hand-overs, and each of the two adds to them through shared memory and issue slots rather than by being waited for - P announced by
+// halves, so that its first products begin early, changed nothing (344 us).
 //
 // A block takes 256 rows (or the last 128) of one (sequence, kv head) at a time, long ones first; a row is a (new token,
 // head of the group) pair, so all heads of a group share each expanded tile.  Two 128-row tiles A and B alternate: while
@@ -19,6 +25,11 @@
 //   warp 17         fetches the codes: one bulk copy per group of 16 tokens, two tiles ahead.
 //   warps 18, 19    bring the next rows of q as soon as the last products with the present ones have been issued
 //                   (head_dim 256: warps 4-7, which have no second tile).
+// Where few blocks of rows would leave SMs idle, a block takes an equal run of all their key tiles instead, and partial results are
+// joined (attn4.cuh): 8 heads of 1024 rows over 8192 keys 71 us, of 4096 rows over 32768 keys 583.
+// Rounding: code * absmax of K and of V and the powers P go to fp16 once each, 2.1e-4 in the root mean square; an fp16 output is then
+// off by 4.8e-4 of its size, half a step of its type (its own rounding: 2.1e-4 on average); a bf16 output shows nothing of it.
+// Products in TF32 would halve the rate and double the operands.
 // fp16 operands hold bf16 caches too: the absmax of a K tile (and, carried along, of the V tiles) is brought near 2^8 by
 // a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.
 #include <type_traits>
@@ -187,6 +198,7 @@ template <int STEP> struct ApList {
 
 // Few items: the key tiles of all, AP_COST more for each item, are cut into equal runs, one per block, in the order of the pairs
 // (block of rows, sequence) with a sequence's heads side by side.  Whole warp.
+// (An item's rows of q and its end take as long as 4 tiles or so: 10 us.)
 constexpr int AP_COST = 4, AP_ALL = 0x7fffffff;
 template <int TILES, int KT> struct ApRun {
     int pair, h, nt;                                                 // where we are; the item's key tiles (one dead one if there is no key)

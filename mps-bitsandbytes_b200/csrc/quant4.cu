@@ -333,7 +333,9 @@ quantize4_stream_kernel(const T *__restrict__ A, IDX total, uint8_t *__restrict_
 // Rows of keys and values into their places in the paged cache (kv4.cuh): the quantiser above with a scattered
 // destination, one launch for a layer's new tokens.  A warp takes a token, finds its place once and then goes through
 // the rows of all heads, K first: a lane owns 8 elements (one 16-byte load where the rows allow it, one 32-bit store), bs / 8
-// lanes a block, four loads per lane under way.  Codes by the streaming quantiser's search.
+// lanes a block, four loads per lane under way.  Codes by the streaming quantiser's search.  Floor: the rows' bytes.  Bound:
+// instruction issue, 72 % of the slots (8 divisions and 8 searches per lane and load).  28 900 tokens of 8 heads of 128, FP4 from bf16:
+// 81 us for 150 MB in and out, 1.8 TB/s.  (The division is exact: codes are to be quantize_4bit's.)
 // ------------------------------------------------------------------------------------------
 static __device__ int g_kv4_append_status = 0;
 
