@@ -332,28 +332,64 @@ quantize4_stream_kernel(const T *__restrict__ A, IDX total, uint8_t *__restrict_
 // ------------------------------------------------------------------------------------------
 // Rows of keys and values into their places in the paged cache (kv4.cuh): the quantiser above with a scattered
 // destination, one launch for a layer's new tokens.  A warp takes a token, finds its place once and then goes through
-// the rows of all heads, K first: a lane owns 8 elements (one 16-byte load where the rows allow it, one 32-bit store), bs / 8
-// lanes a block, four loads per lane under way.  Codes by the streaming quantiser's search.  Floor: the rows' bytes.  Bound:
-// instruction issue, 72 % of the slots (8 divisions and 8 searches per lane and load).  28 900 tokens of 8 heads of 128, FP4 from bf16:
-// 81 us for 150 MB in and out, 1.8 TB/s.  (The division is exact: codes are to be quantize_4bit's.)
+// the heads' rows of K and of V: a lane owns 8 elements (one 16-byte load where the rows allow it, one 32-bit store), bs / 8
+// lanes a block, four loads per lane under way.
+// The codes are quantize_4bit's without its division.  x and the block's a are 16-bit numbers, so there are few quotients x / a near a
+// threshold: x * fl(1 / a) lies on the side of it that x / a lies on, with NF4's thresholds as they are and with FP4's, which
+// x / a can equal, taken 2^-16 larger in magnitude.  oracle/oracle.c:o_prove_kv4_thresholds tries every x and a.
+// Floor: the rows' bytes.  Bound: instruction issue, 76 % of the slots.  28 900 tokens of 8 heads of 128, FP4 from bf16: 62 us for
+// 150 MB in and out, 2.4 TB/s.  64 registers a thread: with 80 or 48 it takes 70 and 75.
 // ------------------------------------------------------------------------------------------
 static __device__ int g_kv4_append_status = 0;
 
+// 33 buckets of width 1/16 from -1 on, each with one threshold at most, once per lane: {threshold, code up to it, code above it}
+struct Kv4Bucket { float th; uint32_t below, above, pad; };
+template <int QT> __device__ __forceinline__ void kv4_bucket_fill(Kv4Bucket *tab, int tid, int nthreads) {
+    constexpr int N = QT == MPSBNB_NF4 ? 15 : 14;
+    constexpr float up = 1.0f + 0x1p-16f;
+    const float nf4[15] = {NF4_T0, NF4_T1, NF4_T2, NF4_T3, NF4_T4, NF4_T5, NF4_T6, NF4_T7, NF4_T8, NF4_T9, NF4_T10, NF4_T11, NF4_T12, NF4_T13, NF4_T14};
+    const float fp4[14] = {-FP4_T6 * up, -FP4_T5 * up, -FP4_T4 * up, -FP4_T3 * up, -FP4_T2 * up, -FP4_T1 * up, -FP4_T0 * up,
+                           FP4_T0 * up, FP4_T1 * up, FP4_T2 * up, FP4_T3 * up, FP4_T4 * up, FP4_T5 * up, FP4_T6 * up};
+    for (int i = tid; i < 33 * 32; i += nthreads) {
+        const int g = i >> 5, b = g < 32 ? g : 31;
+        const float lo = -1.0f + (float)b * 0.0625f, hi = -1.0f + (float)(b + 1) * 0.0625f;   // exact
+        int below = 0;
+        float th = NF4_INF;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float t = QT == MPSBNB_NF4 ? nf4[j] : fp4[j % 14];
+            if (t < lo) ++below;
+            else if (t < hi) th = t;
+        }
+        // FP4: the values' order is -7 .. -1, 0, 1 .. 7 in steps of the magnitude's code
+        auto code = [](int n) { return (uint32_t)(QT == MPSBNB_NF4 ? n : n < 7 ? 8 + (7 - n) : n - 7); };
+        tab[i] = {th, code(below), code(min(below + 1, 15 - (QT != MPSBNB_NF4))), 0u};
+    }
+}
+// v in [-1, 1]; tab_lane: shared address of the table + 16 lane
+__device__ __forceinline__ uint32_t kv4_code(float v, uint32_t tab_lane) {
+    const uint32_t bits = __float_as_uint(__fmaf_rz(v, 16.0f, 8388624.0f));
+    float th; uint32_t below, above, pad;
+    // bits = 0x4B000000 + bucket: shifted left by 9 the constant part leaves the 32-bit word, so no mask is needed
+    asm("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=f"(th), "=r"(below), "=r"(above), "=r"(pad) : "r"(tab_lane + (bits << 9)));
+    return v > th ? above : below;
+}
+
 template <typename T, int QT, int LPB>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 kv4_append_kernel(const Kv4Layer kv, const Kv4Seqs sq, const T *__restrict__ k, int64_t k_ts, int64_t k_hs,
-                  const T *__restrict__ v, int64_t v_ts, int64_t v_hs, int cpr_shift, int vec) {
-    __shared__ __align__(16) float2 table[(QT == MPSBNB_NF4 ? NF4_B32_ENTRIES : FP4_B16_ENTRIES) * 32];
-    if (QT == MPSBNB_NF4) nf4_bucket32_fill(table, threadIdx.x, 256);
-    else fp4_bucket16_fill(table, threadIdx.x, 256);
+                  const T *__restrict__ v, int64_t v_ts, int64_t v_hs, int cpr_shift, int vec, int parts) {
+    __shared__ __align__(16) Kv4Bucket table[33 * 32];
+    kv4_bucket_fill<QT>(table, threadIdx.x, 256);
     __syncthreads();
     const int lane = threadIdx.x & 31;
-    const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(table) + (uint32_t)lane * 8u;
-    // a row is cpr chunks of 8 elements (8, 16 or 32 lanes); the warp goes on by `step` rows, K's before V's
+    const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(table) + (uint32_t)lane * 16u;
+    // a row is cpr chunks of 8 elements (8, 16 or 32 lanes); the warp goes on by `step` heads
     const int cpr = 1 << cpr_shift, half_dim = cpr * 4, step = 32 >> cpr_shift, kc = lane & (cpr - 1), rl = lane >> cpr_shift;
-    const int head_bytes = (1 << (kv.page_shift - 4)) * kv.group_bytes;
+    const int64_t head_bytes = (int64_t)(1 << (kv.page_shift - 4)) * kv.group_bytes;
     constexpr int U = 4;
-    for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < sq.tokens; t += gridDim.x * 8) {
+    // the page that token t goes to (-1: none) and its place
+    auto find = [&](int t, int &place) {
         int b, row, n, len;
         if (sq.cu == nullptr) {
             b = t / sq.new_tokens;
@@ -366,65 +402,92 @@ kv4_append_kernel(const Kv4Layer kv, const Kv4Seqs sq, const T *__restrict__ k, 
             b = lo;
         }
         sq.get(b, row, n, len);
-        const int i = t - row, place = len - n + i;
-        if (i < 0 || i >= n || place < 0) continue;                // (the whole warp: t is the warp's)
+        const int i = t - row;
+        place = len - n + i;
+        if (i < 0 || i >= n || place < 0) return -1;
         const int page = __ldg(sq.table + (int64_t)b * sq.table_ld + (place >> kv.page_shift));
-        if (page < 0 || page >= kv.num_pages) {
-            if (lane == 0) atomicExch(&g_kv4_append_status, KV4_BAD_PAGE);
+        if (page >= 0 && page < kv.num_pages) return page;
+        if (lane == 0) atomicExch(&g_kv4_append_status, KV4_BAD_PAGE);
+        return -1;
+    };
+    const int first = blockIdx.x * 8 + (threadIdx.x >> 5), warps = gridDim.x * 8, items = sq.tokens * parts;
+    const bool few = kv.kv_heads < step;
+    const int passes = few ? (2 * kv.kv_heads + step - 1) / step : 2, chunks = (kv.kv_heads + step * U - 1) / (step * U);
+    int next_place = 0, next_page = first < items ? find(first / parts, next_place) : -1;
+    for (int item = first; item < items; item += warps) {
+        const int place = next_place, page = next_page, t = item / parts, part = item - t * parts;
+        bool ahead = item + warps < items;                         // the next item's place is looked for while this one's rows come
+        if (page < 0) {                                            // (the whole warp: t is the warp's)
+            if (ahead) next_page = find((item + warps) / parts, next_place);
             continue;
         }
         const int slot = place & (KV4_GROUP - 1);
-        uint8_t *base = kv.group(page, 0, place) + slot * half_dim + kc * 4;                       // my codes of head 0's K
+        uint8_t *const base = kv.group(page, 0, place) + slot * half_dim + kc * 4;                               // my codes of the first head's K
         const int to_scale = kv.scale_off + 2 * (slot * (cpr / LPB) + kc / LPB) - (slot * half_dim + kc * 4);   // from them to their absmax
-        const T *ks = k + (int64_t)t * k_ts + kc * 8, *vs = v + (int64_t)t * v_ts + kc * 8;
-        for (int r0 = 0; r0 < 2 * kv.kv_heads; r0 += step * U) {
-            uint4 raw[U];
+#pragma unroll 1
+        for (int pass = parts > 1 ? part / chunks : 0, end = parts > 1 ? pass + 1 : passes; pass < end; ++pass) {
+            // K's heads, then V's; of few heads both side by side
+            int side = pass, h = rl, left = kv.kv_heads - rl;        // left: heads of mine from here on; rows: the warp's
+            if (few) {
+                const int r = pass * step + rl;
+                side = r >= kv.kv_heads;
+                h = side ? r - kv.kv_heads : r;
+                left = r < 2 * kv.kv_heads;
+            }
+            const int skip = parts > 1 ? part % chunks * (step * U) : 0;
+            left -= skip;
+            h += skip;
+            const int64_t hs = side ? v_hs : k_hs;
+            const T *src = (side ? v + (int64_t)t * v_ts : k + (int64_t)t * k_ts) + h * hs + kc * 8;
+            uint8_t *dst = base + h * head_bytes + (side ? kv.half_bytes : 0);
+#pragma unroll 1
+            for (int rows = few ? 1 : parts > 1 ? min(kv.kv_heads - skip, step * U) : kv.kv_heads; rows > 0; rows -= step * U, left -= step * U, src += step * U * hs, dst += step * U * head_bytes) {
+                uint4 raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * step + rl;
-                raw[u] = make_uint4(0u, 0u, 0u, 0u);
-                if (r < 2 * kv.kv_heads) {
-                    const T *src = r >= kv.kv_heads ? vs + (r - kv.kv_heads) * v_hs : ks + r * k_hs;
-                    if (vec) {
-                        raw[u] = __ldg(reinterpret_cast<const uint4 *>(src));
-                    } else {
-                        const uint16_t *s16 = reinterpret_cast<const uint16_t *>(src);
-                        raw[u] = make_uint4(s16[0] | (uint32_t)s16[1] << 16, s16[2] | (uint32_t)s16[3] << 16,
-                                            s16[4] | (uint32_t)s16[5] << 16, s16[6] | (uint32_t)s16[7] << 16);
+                for (int u = 0; u < U; ++u) {
+                    raw[u] = make_uint4(0u, 0u, 0u, 0u);
+                    if (u * step < left) {
+                        const T *at = src + u * (step * hs);
+                        if (vec) {
+                            raw[u] = __ldg(reinterpret_cast<const uint4 *>(at));
+                        } else {
+                            const uint16_t *s16 = reinterpret_cast<const uint16_t *>(at);
+                            raw[u] = make_uint4(s16[0] | (uint32_t)s16[1] << 16, s16[2] | (uint32_t)s16[3] << 16,
+                                                s16[4] | (uint32_t)s16[5] << 16, s16[6] | (uint32_t)s16[7] << 16);
+                        }
                     }
                 }
-            }
+                if (ahead) { next_page = find((item + warps) / parts, next_place); ahead = false; }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (r0 + u * step >= 2 * kv.kv_heads) break;       // warp-uniform
-                const int r = r0 + u * step + rl;
-                // largest magnitude by its bits, two at a time: a NaN orders above infinity and is not lost
-                const uint32_t m2 = __vmaxu2(__vmaxu2(raw[u].x & 0x7fff7fffu, raw[u].y & 0x7fff7fffu), __vmaxu2(raw[u].z & 0x7fff7fffu, raw[u].w & 0x7fff7fffu));
-                uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+                for (int u = 0; u < U; ++u) {
+                    if (u * step >= rows) break;                   // warp-uniform
+                    // largest magnitude by its bits, two at a time: a NaN orders above infinity and is not lost
+                    const uint32_t m2 = __vmaxu2(__vmaxu2(raw[u].x & 0x7fff7fffu, raw[u].y & 0x7fff7fffu), __vmaxu2(raw[u].z & 0x7fff7fffu, raw[u].w & 0x7fff7fffu));
+                    uint32_t m = max(m2 & 0xffffu, m2 >> 16);
 #pragma unroll
-                for (int o = 1; o < LPB; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const bool bad = m >= (sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);   // the block reads back as NaN; any codes will do
-                const uint16_t mb = (uint16_t)m;
-                const float a = bad ? 1.0f : fmaxf(to_f32<T>(*reinterpret_cast<const T *>(&mb)), 1e-8f);
-                float x[8];
-                const T *hv = reinterpret_cast<const T *>(&raw[u]);
+                    for (int o = 1; o < LPB; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    const bool bad = m >= (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);   // the block reads back as NaN; any codes will do
+                    const uint16_t mb = (uint16_t)m;
+                    const float a = bad ? 1.0f : fmaxf(to_f32<T>(*reinterpret_cast<const T *>(&mb)), 1e-8f);
+                    float x[8];
+                    const T *hv = reinterpret_cast<const T *>(&raw[u]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(hv[j]);
-                uint32_t word = 0;
-                if (bad) {
-                } else if (a > 1e-8f && a <= 1e30f) {              // a 16-bit input's magnitude: the shortcut is proven exact
-                    const float ri = __frcp_rn(a);
+                    for (int j = 0; j < 8; ++j) x[j] = to_f32<T>(hv[j]);
+                    uint32_t word = 0;
+                    if (bad) {
+                    } else if (a > 1e-8f && a <= 1e30f) {          // a is the largest of the 16-bit numbers x, and 1 / a a normal number
+                        const float ri = __frcp_rn(a);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) word += code_unit<QT>(block_div<true>(x[j], a, ri), tab_lane) << (4 * j);
-                } else {
+                        for (int j = 0; j < 8; ++j) word += kv4_code(__fmul_rn(x[j], ri), tab_lane) << (4 * j);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) word += code_unit<QT>(block_div<false>(x[j], a, 0.f), tab_lane) << (4 * j);
-                }
-                if (r < 2 * kv.kv_heads) {
-                    const bool is_v = r >= kv.kv_heads;
-                    uint8_t *g = base + (is_v ? (int64_t)(r - kv.kv_heads) * head_bytes + kv.half_bytes : (int64_t)r * head_bytes);
-                    *reinterpret_cast<uint32_t *>(g) = word;
-                    if ((kc & (LPB - 1)) == 0) *reinterpret_cast<T *>(g + to_scale) = from_f32<T>(bad ? __int_as_float(0x7fc00000) : a);
+                        for (int j = 0; j < 8; ++j) word += code_of<QT>(block_div<false>(x[j], a, 0.f)) << (4 * j);
+                    }
+                    if (u * step < left) {
+                        uint8_t *g = dst + u * (step * head_bytes);
+                        *reinterpret_cast<uint32_t *>(g) = word;
+                        if ((kc & (LPB - 1)) == 0) *reinterpret_cast<T *>(g + to_scale) = from_f32<T>(bad ? __int_as_float(0x7fc00000) : a);
+                    }
                 }
             }
         }
@@ -877,12 +940,17 @@ extern "C" int mpsbnb_kv4_append(const mpsbnb_kv4_cache *cache, int layer, const
     const Kv4Seqs sq = kv4_seqs(seqs, cache);
     const int vec = aligned16(k) && aligned16(v) && ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
     const int cpr_shift = cache->head_dim == 64 ? 3 : cache->head_dim == 128 ? 4 : 5;
-    const int64_t want = (seqs->tokens + 7) / 8, cap = (int64_t)sm_count() * 8;
+    // Few tokens: a warp takes four loads' worth of a token's heads, not all of them (32 tokens of 32 heads of 128: 10 us
+    // for 25)
+    const int step = 32 >> cpr_shift, chunks = (cache->kv_heads + step * 4 - 1) / (step * 4);
+    const int units = cache->kv_heads < step ? (2 * cache->kv_heads + step - 1) / step : 2 * chunks;
+    const int parts = seqs->tokens * units <= (int64_t)sm_count() * 32 ? units : 1;
+    const int64_t want = (seqs->tokens * parts + 7) / 8, cap = (int64_t)sm_count() * 4;
     const int grid = (int)(want < cap ? want : cap);
     cudaStream_t st = (cudaStream_t)stream;
 #define LAUNCH_APPEND(T, QT, LPB)                                                                                   \
     kv4_append_kernel<T, QT, LPB><<<grid, 256, 0, st>>>(kv, sq, (const T *)k, k_token_stride, k_head_stride, (const T *)v, \
-                                                        v_token_stride, v_head_stride, cpr_shift, vec)
+                                                        v_token_stride, v_head_stride, cpr_shift, vec, parts)
 #define LAUNCH_APPEND_LPB(T, QT)                                                                                    \
     do {                                                                                                            \
         if (cache->blocksize == 32) LAUNCH_APPEND(T, QT, 4);                                                        \

@@ -216,6 +216,38 @@ int64_t o_prove_quantizer(int qt, int is_bf16, int64_t a_stride, float a_min, fl
     return bad;
 }
 
+/* As above for the cache's quantiser, which takes q = x * r as it is and moves FP4's thresholds (those that x / a can
+ * equal) away from zero by 2^-16 of themselves: the code is the number of signed thresholds below q. */
+int64_t o_prove_kv4_thresholds(int qt, int is_bf16, int64_t a_stride, float a_min, float a_max) {
+    float t[15];
+    if (qt == 0) o_nf4_thresholds(t); else o_fp4_thresholds(t);
+    float th[15];
+    int n = 0;
+    if (qt == 0) for (; n < 15; ++n) th[n] = t[n];
+    else {
+        for (int i = 6; i >= 0; --i) th[n++] = -t[i] * (1.0f + 0x1p-16f);
+        for (int i = 0; i < 7; ++i) th[n++] = t[i] * (1.0f + 0x1p-16f);
+    }
+    const float *code = code_of(qt);
+    int64_t bad = 0;
+#pragma omp parallel for schedule(dynamic, 64) reduction(+ : bad)
+    for (int64_t ai = 1; ai < 0x8000; ai += a_stride) {
+        float a = widen16((uint32_t)ai, is_bf16);
+        if (!(a > 0.0f) || isinf(a) || isnan(a) || a < a_min || a > a_max) continue;
+        float r = 1.0f / a;
+        for (uint32_t xi = 0; xi < 0x10000; ++xi) {
+            float x = widen16(xi, is_bf16);
+            if (isnan(x) || fabsf(x) > a) continue;
+            float q = x * r;
+            int c = 0;
+            for (int i = 0; i < n; ++i) c += q > th[i];
+            if (qt != 0) c = c < 7 ? 15 - c : c - 7;
+            bad += fabsf(q) > 1.0f || c != nearest16(x / a, code);   /* (the buckets are those of [-1, 1]) */
+        }
+    }
+    return bad;
+}
+
 /* Threshold search vs 16-way search on every float in +-window ulps around every
  * threshold and on n_random floats in [-1, 1]; returns the number of disagreements. */
 int64_t o_prove_thresholds(int qt, int window, int64_t n_random) {

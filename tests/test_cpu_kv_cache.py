@@ -243,3 +243,13 @@ def test_operators_want_a_cache():
         bnb.dequantize_kv_4bit(x, 0, None, None)
     with pytest.raises(TypeError, match="takes a KVCache4bit"):
         bnb.copy_kv_pages_4bit(x, [0], [1])
+
+
+@pytest.mark.parametrize("qt,bf16", [(0, 0), (1, 0), (0, 1), (1, 1)])
+def test_codes_by_the_reciprocal_are_those_of_the_division(qt, bf16):
+    """Every third absmax of the 16-bit types in the range where the cache's quantiser multiplies by 1 / absmax, with every x up
+    to it (a stride of 1 also returns 0)."""
+    from oracle import oracle_c
+    fn = oracle_c.lib().o_prove_kv4_thresholds
+    fn.restype, fn.argtypes = C.c_int64, [C.c_int, C.c_int, C.c_int64, C.c_float, C.c_float]
+    assert fn(qt, bf16, 3, 1.0001e-8, 1e30) == 0
