@@ -128,6 +128,16 @@ template <class S> __device__ __forceinline__ int64_t ad_units(const Attn4Args &
     s.get<S>(a, b);
     return s.units<S>(a);
 }
+// sum over the lanes up to this one
+__device__ __forceinline__ int64_t ad_scan(int64_t x) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += up;
+    }
+    return x;
+}
 // n / d for n >= 0, d > 0, in 32 bits where they do
 __device__ __forceinline__ int64_t ad_div(int64_t n, int64_t d) {
     return n < 0x7fffffffll && d < 0x7fffffffll ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
@@ -143,18 +153,15 @@ template <class S> struct AdPiece {
 
     // first piece of the run [t0, t1) of the whole list (false: the run holds none of its tiles); whole warp.  (The ends of the
     // walk are checked: lengths that change under a running kernel must not lead it outside.)
-    // w: units of sequence `lane`
-    __device__ __forceinline__ bool start(const Attn4Args &A, int64_t w, int64_t t0, int64_t t1) {
+    // w, inc: units of sequence `lane`, and of the sequences up to it
+    __device__ __forceinline__ bool start(const Attn4Args &A, int64_t w, int64_t inc, int64_t t0, int64_t t1) {
         const int lane = threadIdx.x & 31;
         int64_t base = 0;
         for (int b0 = 0;; b0 += 32) {
             if (b0 >= A.sq.batch) return false;
-            if (b0 > 0) w = ad_units<S>(A, b0 + lane);
-            int64_t inc = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += up;
+            if (b0 > 0) {
+                w = ad_units<S>(A, b0 + lane);
+                inc = ad_scan(w);
             }
             const uint32_t hit = __ballot_sync(0xffffffffu, base + inc > t0);
             if (hit != 0) {
@@ -221,33 +228,41 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     const int in_team = cta_warp / AD_WARPS, warp = cta_warp % AD_WARPS;
     const int teams = gridDim.x * S::TEAMS, team = in_team * gridDim.x + blockIdx.x;   // little work spreads over the SMs
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + (S::END - 16 - AD_BASE));
-    int64_t units = ad_units<S>(A, lane);                            // (its loads are under way while the table is made)
+    // little work is a chain of small loads: those of the lengths, and of the page table into L2, are under way while the table is made
+    const int64_t units = ad_units<S>(A, lane);
+    if (cta_warp == 0 && lane < A.sq.batch && A.sq.capacity > 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(A.sq.table + (int64_t)lane * A.sq.table_ld));
     pdl_launch_dependents();
 
     // ------------------------------------------------------------ table, barriers
-    {
-        const float mine = A.code[lane & 15];
-        for (int b = cta_warp; b < 256; b += S::WARPS) {
-            const float lo = __shfl_sync(0xffffffffu, mine, b & 15), hi = __shfl_sync(0xffffffffu, mine, b >> 4);
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(AD_LUT + (uint32_t)(b * 256 + lane * 4)), "r"(ad_half2(lo, hi)) : "memory");
-        }
-        if (threadIdx.x < S::WARPS * S::STAGES) mbar_init(S::BAR + 8 * threadIdx.x, G);
-        if (threadIdx.x == 0) *abort_flag = 0;
-        fence_mbar_init();
+    if (threadIdx.x < 256) {
+        // a byte to a thread: its pair 32 times, 16 bytes at a time and each lane beginning elsewhere (no two in a bank)
+        const uint32_t pair = ad_half2(A.code[threadIdx.x & 15], A.code[threadIdx.x >> 4]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(AD_LUT + threadIdx.x * 256 + ((i + lane) & 7) * 16), "r"(pair) : "memory");
     }
-    __syncthreads();
+    if (threadIdx.x < S::WARPS * S::STAGES) mbar_init(S::BAR + 8 * threadIdx.x, G);
+    if (threadIdx.x == 0) *abort_flag = 0;
+    fence_mbar_init();
 
     // ------------------------------------------------------------ my team's run
-    int64_t total = units;
-    for (int b = 32 + lane; b < A.sq.batch; b += 32) total += ad_units<S>(A, b);
+    const int64_t inc = ad_scan(units);
+    int64_t total = __shfl_sync(0xffffffffu, inc, 31);
+    if (A.sq.batch > 32) {
+        int64_t more = 0;
+        for (int b = 32 + lane; b < A.sq.batch; b += 32) more += ad_units<S>(A, b);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+        total += more;
+    }
     const int64_t per = ad_per(total, teams, S::COST), t0 = min(total, team * per), t1 = min(total, t0 + per);
     // what the teams leave for attn4_combine_kernel (a team's thread 0 writes both)
     Attn4Join *join = attn4_join<D, RT>(A.ws, teams) + team;
     if (warp == 0 && lane == 0) join->n = 0;
     Piece in;                                                        // piece the next copy belongs to
-    if (t0 >= t1 || !in.start(A, units, t0, t1)) return;             // whole team; no barrier of the block follows
+    const bool some = t0 < t1 && in.start(A, units, inc, t0, t1);
+    __syncthreads();
+    if (!some) return;                                               // whole team; no barrier of the block follows
     Piece cur = in;                                                  // piece being worked on
     auto team_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(in_team + 1), "n"(AD_WARPS * 32) : "memory"); };
     const uint32_t lut = AD_LUT + lane * 4;
