@@ -7,7 +7,7 @@
 // of the load pipe are then in use (326 instructions and 128 look-ups a lane for 16 tokens), the tensor pipe at 22 %.  Tried for it:
 // 8 warps a block (+20 %) and 16 (=) for 12; codes straight from global memory instead of the ring (+10 %); the next tile's
 // scores under this one's values (=); all look-ups of a block before its products (=).
-// Little work is bound by latency: 15 - 20 us for two launches, however short the sequences are.
+// Little work is bound by latency: 14 us for two launches, however short the sequences are (32 heads of 200 keys).
 //
 //  * Work is a list of (sequence, kv head, row tile, key tile), cut into equal runs, one per team of four warps,
 //    whatever the sequences' lengths are: the lengths are read on the device, so a captured graph follows them.

@@ -345,7 +345,8 @@ def dequantize_kv_4bit(cache: KVCache4bit, layer: int, page_table: Tensor, seq_l
     if max_len < 0:
         raise ValueError(f"max_len must not be negative, got {max_len}")
     shape = (page_table.shape[0], int(max_len), cache.num_kv_heads, cache.head_dim)
-    k, v = cache.k_absmax.new_empty(shape), cache.k_absmax.new_empty(shape)
+    k = cache.k_absmax.new_empty(shape)
+    v = torch.empty_like(k)
     _call(cache, "dequantize_kv_4bit", N.lib().mpsbnb_kv4_dequantize, cache._ref, layer, sq, max_len, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -374,7 +375,8 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
         raise ValueError(f"window must be positive and needs causal=True, got {window}")
     sq = _seqs(cache, page_table, seq_lens, cu_seqlens, tokens, max_seqlen)
     if out is None:
-        out = q.new_empty(q.shape) if cu_seqlens is None else q.new_zeros(q.shape)
+        like = torch.empty_like if cu_seqlens is None else torch.zeros_like
+        out = like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}, 16-byte aligned")
     elif out.untyped_storage().data_ptr() == qr.untyped_storage().data_ptr():
