@@ -17,6 +17,7 @@ struct Attn4Args {
     int32_t heads, group;                        // group: query heads per key/value head
     int32_t causal, window;
     int32_t quant_type;
+    int32_t rows_lo, rows_hi;                    // the kernel's sequences: those of more than rows_lo and up to rows_hi rows a head
     float scale_log2;                            // scale * log2(e): scores are kept as powers of two
     float code[16];                              // the codebook times attn4_code_scale()
 };

@@ -114,6 +114,7 @@ struct AdSeq {
     int rts;                                     // row tiles
     template <class S> __device__ __forceinline__ void get(const Attn4Args &a, int b) {
         a.sq.get(b, row0, n, len);
+        if (n * a.group > a.rows_hi) n = 0;
         const int low = a.window > 0 ? max(0, len - n - a.window + 1) : 0;
         tlo = low / S::TOK;
         nt = n > 0 ? max((len + S::TOK - 1) / S::TOK - tlo, 1) : 0;
@@ -667,12 +668,16 @@ static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return (int64_t)s->new_t
 // Few blocks of rows (under AD_SPLIT rounds over the card) share out the keys as well; of many, a round begun counts as a whole one.
 constexpr int AD_SPLIT = 2;
 enum AdKind { AD_TOKENS, AD_PROMPTS, AD_PROMPTS_SPLIT };
+static bool ad_split(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group) {
+    const int64_t block = c->head_dim == 256 ? 128 : 256;
+    // (every block of the card looks through the (sequence, block of rows) pairs, 32 at a time)
+    return (int64_t)s->batch * c->kv_heads * (((int64_t)s->new_tokens * group + block - 1) / block) <= AD_SPLIT * (int64_t)sm_count();
+}
 static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group, int window) {
     const int64_t rows = (s->tokens * group + s->batch - 1) / s->batch;   // of a sequence and head, on average
     const int64_t lists = (int64_t)s->batch * c->kv_heads, block = c->head_dim == 256 ? 128 : 256, sms = sm_count();
     const int64_t blocks = lists * ((rows + block - 1) / block), tiles = lists * ((rows + 15) / 16);
-    // (every block of the card looks through the (sequence, block of rows) pairs, 32 at a time)
-    const bool split = lists * (((int64_t)s->new_tokens * group + block - 1) / block) <= AD_SPLIT * sms;
+    const bool split = ad_split(c, s, group);
     double keys = (double)s->table_width * c->page_size;
     if (window > 0 && keys > (double)window + s->new_tokens) keys = (double)window + s->new_tokens;
     const int at = c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2;
@@ -680,6 +685,18 @@ static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int g
     if (rows <= 16 || keys * (tiles - meet[at] * (split ? blocks : (blocks + sms - 1) / sms * sms)) <= sooner[at]) return AD_TOKENS;
     return split ? AD_PROMPTS_SPLIT : AD_PROMPTS;
 }
+
+// Prompts among single tokens, as a server batches them: both kernels, each for its sequences.  It may be so where the longest has
+// four times the average's rows and alone would go to the prompt kernel.  (256 sequences over 4096 keys, one with 2048 new tokens, 32
+// heads on 8: 459 us; by the prompt kernel alone 1170, as two calls 156 and 276.)
+static bool ad_mixed(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group, int window) {
+    if (s->cu_seqlens == nullptr || 4 * s->tokens > (int64_t)s->batch * s->new_tokens) return false;
+    mpsbnb_kv4_seqs one = *s;
+    one.batch = 1; one.tokens = s->new_tokens;
+    return ad_kind(c, &one, group, window) != AD_TOKENS;
+}
+// rows a head up to which a sequence of a mixed call counts as single tokens: where the kernels' times per key meet
+static int ad_few_rows(int D) { return D == 64 ? 80 : D == 128 ? 48 : 32; }
 
 static int ad_teams(int D, int NT) { return sm_count() * ((D * NT <= 128 ? 12 : 8) / AD_WARPS); }
 
@@ -719,14 +736,17 @@ int attn4_decode_status_fetch(int *out, bool reset) {
 
 using namespace mpsbnb;
 
+static size_t ad_tokens_ws(int D, int nt) {
+    return ((size_t)ad_teams(D, nt) * (2 * (8 * nt) * (D + 2) * sizeof(float) + sizeof(Attn4Join)) + 15) & ~(size_t)15;
+}
+
 extern "C" size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads) {
     if (kv4_check_cache(cache, 0) != MPSBNB_OK || kv4_check_seqs(seqs, cache) != MPSBNB_OK) return 0;
     if (heads <= 0 || heads % cache->kv_heads != 0 || seqs->batch == 0 || seqs->tokens == 0) return 0;
-    const int nt = ad_nt(seqs, heads / cache->kv_heads);
-    const size_t tokens = (size_t)ad_teams(cache->head_dim, nt) * (2 * (8 * nt) * (cache->head_dim + 2) * sizeof(float) + sizeof(Attn4Join));
-    // (a window, not known here, may lead from the prompt kernel to the other, not back)
-    const size_t prompts = ad_kind(cache, seqs, heads / cache->kv_heads, 0) == AD_PROMPTS_SPLIT ? attn4_prompt_ws(cache->head_dim) : 0;
-    return tokens > prompts ? tokens : prompts;
+    const int group = heads / cache->kv_heads, nt = ad_nt(seqs, group), few = group > 8 ? 2 : 1;
+    const size_t any = ad_tokens_ws(cache->head_dim, nt), mixed = ad_tokens_ws(cache->head_dim, few), tokens = any > mixed ? any : mixed;
+    // (a window, not known here, may take the prompt kernel out, not bring it in)
+    return tokens + (ad_kind(cache, seqs, group, 0) == AD_PROMPTS_SPLIT || ad_mixed(cache, seqs, group, 0) ? attn4_prompt_ws(cache->head_dim) : 0);
 }
 
 extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
@@ -753,10 +773,21 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.scale_log2 = scale * 1.4426950408889634f;
     static const float codes[2][16] = {MPSBNB_NF4_TABLE, MPSBNB_FP4_TABLE};
     for (int i = 0; i < 16; ++i) a.code[i] = codes[cache->quant_type][i] * attn4_code_scale(cache->quant_type);
-    const AdKind kind = ad_kind(cache, seqs, group, window);
-    if (kind != AD_TOKENS) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, kind == AD_PROMPTS_SPLIT, (cudaStream_t)stream);
-    const int nt = ad_nt(seqs, group);
+    a.rows_lo = 0; a.rows_hi = 0x7fffffff;
     cudaStream_t st = (cudaStream_t)stream;
+    int nt = ad_nt(seqs, group);
+    if (ad_mixed(cache, seqs, group, window)) {
+        nt = group > 8 ? 2 : 1;
+        a.rows_lo = ad_few_rows(cache->head_dim);
+        a.ws = (float *)((char *)workspace + ad_tokens_ws(cache->head_dim, nt));
+        rc = attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, ad_split(cache, seqs, group), st);
+        if (rc != MPSBNB_OK) return rc;
+        a.rows_hi = a.rows_lo; a.rows_lo = 0;
+        a.ws = (float *)workspace;
+    } else {
+        const AdKind kind = ad_kind(cache, seqs, group, window);
+        if (kind != AD_TOKENS) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, kind == AD_PROMPTS_SPLIT, st);
+    }
     const int dt = cache->dtype;
     if (cache->blocksize == 32) {
         if (cache->head_dim == 64) return ad_launch_t<64, 32>(a, dt, nt, st);

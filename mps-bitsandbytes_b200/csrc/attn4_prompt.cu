@@ -177,7 +177,7 @@ template <int STEP> struct ApList {
         const int b = chunk * 32 + (threadIdx.x & 31);
         int row0, n = 0, len;
         if (b < A.sq.batch) A.sq.get(b, row0, n, len);
-        has = __ballot_sync(0xffffffffu, (int64_t)n * A.group > (int64_t)level * STEP);
+        has = __ballot_sync(0xffffffffu, (int64_t)n * A.group > max((int64_t)level * STEP, (int64_t)A.rows_lo));
     }
     __device__ __forceinline__ void begin(const Attn4Args &A, int blocks) { level = blocks - 1; chunk = 0; before = 0; look(A); }
     // item j, at or behind the one found last; false: there are not so many
@@ -215,7 +215,7 @@ template <int TILES, int KT> struct ApRun {
         ApItem<TILES, KT> w;
         place(A, blocks, pair, b, r0);
         w.set(A, b, 0, r0, 0, AP_ALL, 0);
-        return r0 < w.rows ? max(w.nk, 1) : 0;
+        return r0 < w.rows && w.rows > A.rows_lo ? max(w.nk, 1) : 0;
     }
     __device__ __forceinline__ static int64_t units(const Attn4Args &A, int nt) { return nt > 0 ? (int64_t)(nt + AP_COST) * A.kv.kv_heads : 0; }
     __device__ __forceinline__ bool begin(const Attn4Args &A, int blocks) {

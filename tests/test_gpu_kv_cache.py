@@ -206,6 +206,11 @@ CASES = [
     (128, 64, 64, "nf4", F16, 16, 1, [33], [20000], True, None),
     (256, 64, 64, "nf4", BF16, 8, 1, [16, 40], [9000, 40], True, 5000),
     (64, 32, 16, "fp4", BF16, 20, 1, [50, 1, 13], [50, 700, 8000], False, None),
+    # prompts among single tokens and drafts: both kernels in a call (the first: keys shared out; the last: more pairs than that looks through)
+    (128, 64, 64, "nf4", BF16, 32, 8, [1, 1, 400, 3, 1, 0, 1, 13], [700, 20, 555, 90, 1000, 40, 3, 13], True, None),
+    (256, 32, 32, "fp4", F16, 8, 2, [1, 2, 1, 1, 300, 1, 1, 9, 1], [300, 20, 77, 90, 500, 1, 640, 200, 33], True, 90),
+    (64, 64, 16, "nf4", F16, 48, 8, [2, 1, 1, 1, 1, 900, 14, 1, 1, 1] * 4, [70, 500, 33, 1, 90, 900, 400, 64, 65, 17] * 4, True, None),
+    (128, 32, 64, "nf4", F16, 40, 4, [1] * 40 + [700, 11, 5] + [1] * 40, list(range(1, 41)) + [900, 11, 600] + list(range(40, 400, 9)), True, None),
 ]
 
 
