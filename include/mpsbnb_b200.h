@@ -493,8 +493,9 @@ int mpsbnb_kv4_copy_pages(const mpsbnb_kv4_cache *cache, const int32_t *src, con
  * Scores, softmax statistics and sums are fp32.  fp16 products: single tokens round the 16 code values and the weights
  * probability * absmax, prompts code * absmax (keys and values) and the probabilities.
  * A key whose absmax is not finite makes the rows that see it NaN; a value's makes NaN of its block's channels in those rows
- * (single tokens) or of the rows (prompts).  Which of two kernels runs (both, where prompts and single tokens are mixed) - and with it the rounding - depends on the numbers of rows,
- * heads and sequences and on table_width, the room for keys: never on the lengths, so a captured graph follows them.
+ * (single tokens) or of the rows (prompts).  Which of two kernels runs (both, where prompts and single tokens are mixed) -
+ * and with it the rounding - depends on the numbers of rows, heads and sequences, on the window and on table_width, the room
+ * for keys: never on the lengths, so a captured graph follows them.
  * workspace: mpsbnb_attention_4bit_workspace_bytes() bytes, 16-byte aligned, used by this call only while it runs. */
 size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads);
 int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
