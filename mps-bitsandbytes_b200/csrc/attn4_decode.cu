@@ -26,8 +26,9 @@
 //    exceeds it by 2^8: one vote per tile instead of a reduction, and fp32 sums lose nothing by it.  The weight
 //    p * absmax goes to fp16 (off by 2^-11 at most, 2.1e-4 in the root mean square; a second fp16 for the rest would cost a third
 //    more products and conversions): an output is off by 2.9e-4 - 3.6e-4 of its size, where its own rounding to fp16 makes 2.1e-4;
-//    in bf16 nothing is to be seen of it.  absmax is taken times a power of two that is lowered, in the same vote, when it
-//    exceeds 2^7.
+//    in bf16 nothing is to be seen of it.  absmax is taken times a power of two that brings a tile's to [2^-4, 2^7]; the same
+//    vote sees when they leave that.  A tile that has more between its smallest and its largest takes a power of two for each row
+//    and block, after that row's largest weight: what other rows see, or what has next to no weight, costs a row no bits.
 //    bf16 queries are brought to fp16 by a power of two per row: exact, but for parts below 2^-24 of the row's largest.
 #include <cmath>
 #include <type_traits>
@@ -43,6 +44,8 @@ static __device__ int g_attn4_status = 0;
 constexpr int AD_WARPS = 4;                                          // of a team: the warps that share a run of tiles
 // What a (sequence, head, row tile) counts besides its tokens, in tokens: q, the joining of the warps
 constexpr int AD_COST_TOKENS = 512;
+// An absmax up to 1e-8 (as bf16 has it) is the quantiser's floor, or 0 in fp16: its block is nothing beside others.
+constexpr uint32_t AD_ABOVE_FLOOR = 0x322c0001u;
 constexpr uint32_t AD_LUT = 65536;                                   // shared-window address of the table
 constexpr uint32_t AD_BASE = 1024;                                   // ... and of the dynamic shared memory
 
@@ -450,7 +453,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 }
             }
             // absmax of the values, token tok (+ 8) of group x
-            float sv[G][2][NB], sm = 0.0f;
+            float sv[G][2][NB], sm = 0.0f, sn = __int_as_float(0x7f800000);
 #pragma unroll
             for (int x = 0; x < G; ++x) {
                 ad_scales<T, NB>(kb + x * S::GROUP + HALF + SOFF + tok * NB * 2, sv[x][0]);
@@ -483,7 +486,12 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
 #pragma unroll
             for (int x = 0; x < G; ++x)
 #pragma unroll
-                for (int blk = 0; blk < NB; ++blk) sm = fmaxf(sm, fmaxf(sv[x][0][blk], sv[x][1][blk]));
+                for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        sm = fmaxf(sm, sv[x][y][blk]);
+                        sn = fminf(sn, sv[x][y][blk]);
+                    }
             float p[G][NT][4], top = -1.0f;
 #pragma unroll
             for (int x = 0; x < G; ++x)
@@ -494,37 +502,142 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                         p[x][nt][j] = fmaf(s[x][nt][j], f[nt][j & 1], -m[nt][j & 1]);
                         top = fmaxf(top, p[x][nt][j]);
                     }
-            // p and absmax * up stay under 2^8 and 2^7, their product is at home in fp16
-            if (__any_sync(0xffffffffu, top > 8.0f || sm * up > 128.0f)) {
+            // lane (g, c): channels blk * BS + g * (BS / 8) + 0 .. BS / 8 - 1 of the tokens c, c + 4, c + 8, c + 12 of group x, those
+            // of two tokens in a byte: ev the even channels, od the odd ones
+            auto codes_of = [&](int x, int blk, uint32_t (&ev)[2], uint32_t (&od)[2]) {
+                uint32_t w[4];
 #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, d));
-                float ku = 1.0f;
-                if (sm * up > 128.0f) {                              // the largest comes to [16, 32)
-                    const int e = max(5, (int)(__float_as_uint(fminf(sm, 3.4e38f)) >> 23));
-                    const float un = __int_as_float((258 - e) << 23);   // 2^(131 - e)
-                    ku = un * __frcp_rn(up);                         // (0 where the difference leaves fp32)
-                    up = un;
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t va = kb + x * S::GROUP + HALF + (c + 4 * i) * (D / 2) + blk * (BS / 2) + g * (BS / 16);
+                    if constexpr (BS == 64) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(va));
+                    else { uint16_t h; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(va)); w[i] = h; }
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int y = 0; y < 2; ++y) {
+                    ev[y] = (w[2 * y] & 0x0F0F0F0Fu) | ((w[2 * y + 1] << 4) & 0xF0F0F0F0u);
+                    od[y] = ((w[2 * y] >> 4) & 0x0F0F0F0Fu) | (w[2 * y + 1] & 0xF0F0F0F0u);
+                }
+            };
+            auto weights = [&](const float (&pr)[4], int x, int blk, int nt, float (&wt)[4]) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float mx = fmaxf(s[0][nt][j], s[0][nt][j + 2]);
-                        if (G == 2) mx = fmaxf(mx, fmaxf(s[G - 1][nt][j], s[G - 1][nt][j + 2]));
-                        mx *= f[nt][j];
+                for (int j = 0; j < 4; ++j) wt[j] = pr[j] * (sv[x][j >> 1][blk] * up);
+                if (seen != 0xffffffffu) {                           // a value that is not finite is no matter of rows that do not see it
 #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                        const float mn = mx > m[nt][j] + 8.0f ? mx : m[nt][j], k = ex2(m[nt][j] - mn);
-                        m[nt][j] = mn;
-                        l[nt][j] *= k;
+                    for (int j = 0; j < 4; ++j) if (!(seen >> ((x * NT + nt) * 4 + j) & 1u)) wt[j] = 0.0f;
+                }
+            };
+            // p stays under 2^8 and absmax * up in [2^-4, 2^7]: their product is at home in fp16
+            auto least = [&]() { return __int_as_float((250 << 23) - __float_as_int(up)); };   // 2^-4 / up
+            const bool high = top > 8.0f || sm * up > 128.0f;
+            if (__any_sync(0xffffffffu, high || sn < least())) {
+                uint32_t sl = 0xffffffffu;                           // the least above the floor, as bits from there on
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k * ku; o[i][nt][j + 2] *= k * ku; }
+                for (int x = 0; x < G; ++x)
 #pragma unroll
-                        for (int x = 0; x < G; ++x) {
-                            p[x][nt][j] = fmaf(s[x][nt][j], f[nt][j], -mn);
-                            p[x][nt][j + 2] = fmaf(s[x][nt][j + 2], f[nt][j], -mn);
-                        }
+                    for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) sl = min(sl, __float_as_uint(sv[x][y][blk]) - AD_ABOVE_FLOOR);
+                sl = __reduce_min_sync(0xffffffffu, sl);
+                auto low = [&]() { return sl < (uint32_t)max(0, (int)(__float_as_uint(least()) - AD_ABOVE_FLOOR)); };
+                if (__any_sync(0xffffffffu, high || low())) {
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, d));
+                    float ku = 1.0f;
+                    // the largest comes to [16, 32); up is held in [2^-40, 2^100], where the sums are in no danger
+                    const float un = __int_as_float(max(87, min(227, 258 - (int)(__float_as_uint(fminf(sm, 3.4e38f)) >> 23))) << 23);
+                    if (sm * up > 128.0f) {
+                        ku = un * __frcp_rn(up);                     // (0 where the difference leaves fp32)
+                        up = un;
+                    } else if (low() && un > up) {                   // up again, if the sums allow it
+                        float most = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(o[i][nt][j]));
+#pragma unroll
+                        for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                        const float more = un * __frcp_rn(up);
+                        if (most * more < 0x1p100f) { ku = more; up = un; }
                     }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            float mx = fmaxf(s[0][nt][j], s[0][nt][j + 2]);
+                            if (G == 2) mx = fmaxf(mx, fmaxf(s[G - 1][nt][j], s[G - 1][nt][j + 2]));
+                            mx *= f[nt][j];
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                            const float mn = mx > m[nt][j] + 8.0f ? mx : m[nt][j], k = ex2(m[nt][j] - mn);
+                            m[nt][j] = mn;
+                            l[nt][j] *= k;
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k * ku; o[i][nt][j + 2] *= k * ku; }
+#pragma unroll
+                            for (int x = 0; x < G; ++x) {
+                                p[x][nt][j] = fmaf(s[x][nt][j], f[nt][j], -mn);
+                                p[x][nt][j + 2] = fmaf(s[x][nt][j + 2], f[nt][j], -mn);
+                            }
+                        }
+                    if (sm * up > 128.0f || low()) {
+                        // The tile's absmax do not fit in there: each column's largest weight of a block to [16, 32), the products
+                        // apart and back into up's unit.  To what follows the tile's values are zeros.
+#pragma unroll
+                        for (int blk = 0; blk < NB; ++blk) {
+                            uint32_t b0[G][NT], b1[G][NT], ev[G][2], od[G][2];
+                            float back[NT][2];
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                float wt[G][4], mul[2];
+#pragma unroll
+                                for (int x = 0; x < G; ++x) {
+                                    const float pr[4] = {ex2(p[x][nt][0]), ex2(p[x][nt][1]), ex2(p[x][nt][2]), ex2(p[x][nt][3])};
+                                    weights(pr, x, blk, nt, wt[x]);
+                                }
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    float wm = fmaxf(fmaxf(wt[0][j], wt[0][j + 2]), fmaxf(wt[G - 1][j], wt[G - 1][j + 2]));
+#pragma unroll
+                                    for (int d = 4; d < 32; d <<= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, d));
+                                    const int e = max(5, min(250, (int)(__float_as_uint(wm) >> 23)));
+                                    mul[j] = __int_as_float((258 - e) << 23);            // 2^(131 - e)
+                                    back[nt][j] = __int_as_float((e - 4) << 23);         // 2^(e - 131)
+                                }
+#pragma unroll
+                                for (int x = 0; x < G; ++x) {
+                                    b0[x][nt] = ad_transpose(ad_half2(wt[x][0] * mul[0], wt[x][1] * mul[1]));
+                                    b1[x][nt] = ad_transpose(ad_half2(wt[x][2] * mul[0], wt[x][3] * mul[1]));
+                                }
+                            }
+#pragma unroll
+                            for (int x = 0; x < G; ++x) codes_of(x, blk, ev[x], od[x]);
+#pragma unroll
+                            for (int j = 0; j < MB; ++j) {
+                                float t[NT][4];
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) t[nt][i] = 0.0f;
+#pragma unroll
+                                for (int x = 0; x < G; ++x) {
+                                    const uint32_t a0 = ad_lut(lut, ev[x][0], j), a1 = ad_lut(lut, od[x][0], j), a2 = ad_lut(lut, ev[x][1], j), a3 = ad_lut(lut, od[x][1], j);
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt) ad_mma(t[nt], a0, a1, a2, a3, b0[x][nt], b1[x][nt]);
+                                }
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) o[blk * MB + j][nt][i] = fmaf(t[nt][i], back[nt][i & 1], o[blk * MB + j][nt][i]);
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < G; ++x)
+#pragma unroll
+                            for (int blk = 0; blk < NB; ++blk) sv[x][0][blk] = sv[x][1][blk] = 0.0f;
+                    }
+                }
             }
 #pragma unroll
             for (int x = 0; x < G; ++x)
@@ -537,42 +650,25 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                     }
             // O^T += V^T P^T
 #pragma unroll
-            for (int x = 0; x < G; ++x) {
-                const uint32_t vb = kb + x * S::GROUP + HALF;
+            for (int x = 0; x < G; ++x)
 #pragma unroll
                 for (int blk = 0; blk < NB; ++blk) {
-                    const float s0 = sv[x][0][blk] * up, s1 = sv[x][1][blk] * up;
-                    uint32_t b0[NT], b1[NT];
+                    uint32_t b0[NT], b1[NT], ev[2], od[2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float wt[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) wt[j] = p[x][nt][j] * (j < 2 ? s0 : s1);
-                        if (seen != 0xffffffffu) {                   // a value that is not finite is no matter of rows that do not see it
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) if (!(seen >> ((x * NT + nt) * 4 + j) & 1u)) wt[j] = 0.0f;
-                        }
+                        weights(p[x][nt], x, blk, nt, wt);
                         b0[nt] = ad_transpose(ad_half2(wt[0], wt[1]));
                         b1[nt] = ad_transpose(ad_half2(wt[2], wt[3]));
                     }
-                    // lane (g, c): channels blk * BS + g * (BS / 8) + 0 .. BS / 8 - 1 of the tokens c, c + 4, c + 8, c + 12
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t va = vb + (c + 4 * i) * (D / 2) + blk * (BS / 2) + g * (BS / 16);
-                        if constexpr (BS == 64) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(va));
-                        else { uint16_t h; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(va)); w[i] = h; }
-                    }
-                    const uint32_t ev0 = (w[0] & 0x0F0F0F0Fu) | ((w[1] << 4) & 0xF0F0F0F0u), od0 = ((w[0] >> 4) & 0x0F0F0F0Fu) | (w[1] & 0xF0F0F0F0u);
-                    const uint32_t ev1 = (w[2] & 0x0F0F0F0Fu) | ((w[3] << 4) & 0xF0F0F0F0u), od1 = ((w[2] >> 4) & 0x0F0F0F0Fu) | (w[3] & 0xF0F0F0F0u);
+                    codes_of(x, blk, ev, od);
 #pragma unroll
                     for (int j = 0; j < MB; ++j) {
-                        const uint32_t a0 = ad_lut(lut, ev0, j), a1 = ad_lut(lut, od0, j), a2 = ad_lut(lut, ev1, j), a3 = ad_lut(lut, od1, j);
+                        const uint32_t a0 = ad_lut(lut, ev[0], j), a1 = ad_lut(lut, od[0], j), a2 = ad_lut(lut, ev[1], j), a3 = ad_lut(lut, od[1], j);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) ad_mma(o[blk * MB + j][nt], a0, a1, a2, a3, b0[nt], b1[nt]);
                     }
                 }
-            }
             if (++got == S::STAGES) { got = 0; phase ^= 1; }
             __syncwarp();                                            // every lane has read the stage
             issue();

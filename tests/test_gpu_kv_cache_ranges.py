@@ -1,0 +1,137 @@
+"""Attention over the 4-bit cache where keys and values of very different magnitudes lie side by side: what a row does not
+see, or gives next to no weight, must cost it nothing of its precision."""
+import math
+
+import pytest
+import torch
+
+import mps_bitsandbytes_b200 as bnb
+from gpu_util import assert_device_ok
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+HALF_STEP = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def reference(q, cache, layer, table, length, window=None):
+    """(out, limit) in 64 bits of one sequence's last rows q [n, heads, head_dim], causal.  ``limit`` counts what a row sees and
+    nothing else, a = a block's absmax:
+
+    an element of K or V goes into its product with two fp16 roundings at most, of 2^-11 of itself each, or of 2^-25 where it is
+    subnormal under a power of two that brings each block's absmax to 2^-14 at least: 2^-11 a.  bf16 queries: 2^-25 of the row's largest,
+    times sum |k|.  So a score is off by e = scale sum_d (|q_d| (2^-10 |k_d| + 2^-11 a) + 2^-25 max|q| |k_d|) and a probability by a factor
+    within exp(+-2 max e).  A weight is off by 2^-11 of itself, or by 2^-25 (and by no more than itself) where the key's a is 2^-4 at
+    least and the row's largest power of two is 1 at least: 2^-21 a of the row's largest probability.  fp32 sums: n 2^-23, and
+    2^-18 for scores and powers.
+    """
+    import kv_util as U
+    n, H, D = q.shape
+    group = H // cache.num_kv_heads
+    k, v = (U.rows_of(cache, layer, table, 0, length, x) for x in "kv")
+    place = torch.arange(length, device="cuda")
+    page = table.long()[place // cache.page_size], place % cache.page_size
+    ka, va = (getattr(cache, x + "_absmax")[layer][page[0], :, page[1] // 16, page[1] % 16].double().repeat_interleave(cache.blocksize, -1) for x in "kv")
+    pos = torch.arange(length - n, length, device="cuda")[:, None]
+    seen = place[None] <= pos
+    if window:
+        seen &= place[None] > pos - window
+    out, limit = torch.zeros(n, H, D, dtype=torch.float64, device="cuda"), torch.zeros(n, H, D, dtype=torch.float64, device="cuda")
+    for h in range(H):
+        x, g = q[:, h].double(), h // group
+        s = (x @ k[:, g].T * D ** -0.5).masked_fill(~seen, -math.inf)
+        p = torch.softmax(s, -1)
+        e = D ** -0.5 * (x.abs() @ (2.0 ** -10 * k[:, g].abs() + 2.0 ** -11 * ka[:, g]).T + 2.0 ** -25 * x.abs().amax(-1, keepdim=True) * k[:, g].abs().sum(-1)[None])
+        # (probabilities beyond the row's own resolution do not count)
+        e = e.masked_fill(~seen | (p < 2.0 ** -40), 0.0).amax(-1, keepdim=True)
+        size = p @ v[:, g].abs()
+        out[:, h] = p @ v[:, g]
+        limit[:, h] = (size * (torch.expm1(2 * e) + 3 * 2.0 ** -11 + length * 2.0 ** -23 + 2.0 ** -18) + p @ va[:, g] * 2.0 ** -11
+                       + torch.minimum(p, 2.0 ** -21 * p.amax(-1, keepdim=True)) @ va[:, g])
+    return out, limit + HALF_STEP[q.dtype] * (out.abs() + limit) + 2.0 ** -25
+
+
+def close(got, want, limit):
+    worst = ((got.double() - want).abs() / limit).max().item()
+    assert torch.isfinite(got).all() and worst <= 1.0, f"off by {worst:.3g} of the limit"
+
+
+def _cache(head_dim, blocksize, dtype, length, kv_heads, gen, quant="nf4"):
+    cache = bnb.KVCache4bit(1, -(-length // 32), kv_heads, head_dim, page_size=32, blocksize=blocksize, quant_type=quant, dtype=dtype)
+    table = torch.randperm(cache.num_pages, generator=torch.Generator().manual_seed(length)).to(torch.int32)[None].cuda()
+    k, v = (torch.randn(length, kv_heads, head_dim, generator=gen, device="cuda") for _ in range(2))
+    return cache, table, k, v
+
+
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("head_dim,blocksize,heads,kv_heads,new,length", [
+    (128, 64, 2, 2, 4, 100), (128, 64, 8, 2, 4, 97), (64, 32, 6, 2, 8, 333), (256, 64, 2, 1, 5, 70), (256, 32, 12, 1, 5, 64), (128, 32, 16, 1, 2, 35), (64, 64, 1, 1, 3, 40)])
+@pytest.mark.parametrize("dtype,large", [(BF16, 1e10), (BF16, 1e25), (F16, 6e4)])
+def test_a_drafted_token_of_any_magnitude_leaves_the_rows_before_it_alone(dtype, large, head_dim, blocksize, heads, kv_heads, new, length, side):
+    gen = torch.Generator(device="cuda").manual_seed(length)
+    cache, table, k, v = _cache(head_dim, blocksize, dtype, length, kv_heads, gen)
+    if dtype == F16:
+        k, v = k * 2.0 ** -12, v * 2.0 ** -12
+    x = k if side == "k" else v
+    x[-1] = large * torch.sign(x[-1])
+    lens = _i32([length])
+    bnb.append_kv_4bit(cache, 0, k.to(dtype), v.to(dtype), table, lens)
+    q = torch.randn(new, heads, head_dim, generator=gen, device="cuda").to(dtype)
+    got = bnb.attention_4bit(q[None], cache, 0, table, lens)[0]
+    want, limit = reference(q, cache, 0, table[0], length)
+    close(got[:-1], want[:-1], limit[:-1])
+    if side == "v":
+        close(got, want, limit)
+    assert_device_ok()
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,blocksize", [(2, 2, 128, 64), (12, 1, 64, 32), (4, 1, 256, 64)])
+@pytest.mark.parametrize("dtype,sizes", [(BF16, (1e10, 1.0)), (BF16, (1.0, 1e-6)), (BF16, (1e20, 1e-6)), (F16, (6e4, 1e-3))])
+def test_values_of_any_magnitude_that_have_next_to_no_weight(dtype, sizes, heads, kv_heads, head_dim, blocksize):
+    """Every eighth key is far larger than the others, and so far from the queries that its weight vanishes."""
+    length = 200
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    cache, table, k, v = _cache(head_dim, blocksize, dtype, length, kv_heads, gen)
+    far = torch.arange(length, device="cuda") % 8 == 3
+    k, v = k * 0.05, v * sizes[1]
+    k[far], v[far] = -4.0, v[far] * (sizes[0] / sizes[1])
+    v = v.clamp(-sizes[0], sizes[0])
+    lens = _i32([length])
+    bnb.append_kv_4bit(cache, 0, k.to(dtype), v.to(dtype), table, lens)
+    q = (4.0 + 0.5 * torch.randn(1, heads, head_dim, generator=gen, device="cuda")).to(dtype)
+    got = bnb.attention_4bit(q, cache, 0, table, lens)
+    want, limit = reference(q, cache, 0, table[0], length)
+    assert limit.max() < 0.1 * sizes[1]                              # (the large ones do count for nothing)
+    close(got, want, limit)
+
+
+@pytest.mark.parametrize("dtype,sizes", [(BF16, (1e12, 1e-6)), (F16, (6e4, 1e-4))])
+@pytest.mark.parametrize("head_dim,blocksize,heads", [(128, 64, 1), (128, 32, 12), (64, 32, 3), (256, 32, 2)])
+def test_blocks_of_a_row_of_any_magnitude(dtype, sizes, head_dim, blocksize, heads):
+    """The last block of every value is far smaller than the first ones: its channels are as exact as theirs."""
+    length = 150
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    cache, table, k, v = _cache(head_dim, blocksize, dtype, length, 1, gen, "fp4")
+    v = v.clamp(-1, 1) * sizes[0]
+    v[..., -blocksize:] *= sizes[1] / sizes[0]
+    v[3::5] *= 2.0 ** -3
+    lens = _i32([length])
+    bnb.append_kv_4bit(cache, 0, k.to(dtype), v.to(dtype), table, lens)
+    q = torch.randn(1, heads, head_dim, generator=gen, device="cuda").to(dtype)
+    close(bnb.attention_4bit(q, cache, 0, table, lens), *reference(q, cache, 0, table[0], length))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_blocks_of_zeros_beside_others(dtype):
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    cache, table, k, v = _cache(128, 32, dtype, 120, 2, gen)
+    k[..., 96:], v[..., 96:], k[::7], v[::5] = 0, 0, 0, 0
+    lens = _i32([120])
+    bnb.append_kv_4bit(cache, 0, k.to(dtype), v.to(dtype), table, lens)
+    q = torch.randn(3, 8, 128, generator=gen, device="cuda").to(dtype)
+    got = bnb.attention_4bit(q[None], cache, 0, table, lens)[0]
+    close(got, *reference(q, cache, 0, table[0], 120))
+    assert (got[..., 96:].abs() < 1e-7).all()
