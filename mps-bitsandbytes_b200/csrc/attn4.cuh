@@ -14,6 +14,8 @@ struct Attn4Args {
     void *out;
     float *lse;
     float *ws;                                   // partial results
+    uint32_t *wide;                              // [SMs], bit b % 32: sequence b's magnitudes are too far apart for the prompt kernel
+    int32_t wide_n, redo;                        // redo: those sequences and no others
     int32_t heads, group;                        // group: query heads per key/value head
     int32_t causal, window;
     int32_t quant_type;
@@ -126,8 +128,8 @@ template <int D, int RT, int ROWS, typename T> static int attn4_combine(const At
     return check_launch();
 }
 
-// attn4_prompt.cu.  split: its blocks share out the keys evenly and leave partial results
-int attn4_prompt(const Attn4Args &a, int head_dim, int blocksize, int dtype, bool split, cudaStream_t st);
+// attn4_prompt.cu.  split: its blocks share out the keys evenly and leave partial results.  grid: how many wrote their word of `wide`
+int attn4_prompt(const Attn4Args &a, int head_dim, int blocksize, int dtype, bool split, cudaStream_t st, int *grid);
 size_t attn4_prompt_ws(int head_dim);            // bytes of workspace when split
 
 }  // namespace mpsbnb

@@ -69,7 +69,7 @@ template <int D, int BS, int NT> struct AdSmem {
     static constexpr uint32_t RED = RING1 + (WARPS - WARPS0) * STAGES * STAGE;
     static constexpr uint32_t STAT = RED + WARPS * RT * RED_LD * 4;  // (maximum, sum) of every warp and row
     static constexpr uint32_t BAR = STAT + WARPS * RT * 8;
-    static constexpr uint32_t END = BAR + WARPS * STAGES * 8 + 16;
+    static constexpr uint32_t REDO = BAR + WARPS * STAGES * 8 + 4, END = REDO + 12;   // (the word before it: abort flag)
     static constexpr int BYTES = END - AD_BASE;
     static_assert(BYTES <= 227 * 1024, "shared memory of the decode kernel");
     static_assert(GROUP % 16 == 0, "bulk copies go by 16 bytes");
@@ -117,7 +117,12 @@ struct AdSeq {
     int rts;                                     // row tiles
     template <class S> __device__ __forceinline__ void get(const Attn4Args &a, int b) {
         a.sq.get(b, row0, n, len);
-        if (n * a.group > a.rows_hi) n = 0;
+        if (n * a.group > a.rows_hi || n * a.group <= a.rows_lo) n = 0;
+        if (a.redo) {
+            uint32_t mask;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(mask) : "r"(S::REDO) : "memory");
+            if (!(mask >> (b & 31) & 1u)) n = 0;
+        }
         const int low = a.window > 0 ? max(0, len - n - a.window + 1) : 0;
         tlo = low / S::TOK;
         nt = n > 0 ? max((len + S::TOK - 1) / S::TOK - tlo, 1) : 0;
@@ -182,13 +187,14 @@ template <class S> struct AdPiece {
         h = sub / s.rts;
         r = sub - h * s.rts;
         left = t1 - t0;
-        take((int)(off - (int64_t)sub * units));
+        take(A, (int)(off - (int64_t)sub * units));
         return e > 0 || next(A);
     }
     // the piece that begins `from` units into its (sequence, head, row tile)
-    __device__ __forceinline__ void take(int from) {
-        const int to = (int)min((int64_t)(s.nt + S::COST), from + left);
+    __device__ __forceinline__ void take(const Attn4Args &A, int from) {
+        int to = (int)min((int64_t)(s.nt + S::COST), from + left);
         left -= to - from;
+        if (A.redo) to = from == 0 ? s.nt + S::COST : 0;             // nothing is cut: whole ones, in the runs that they begin in
         a = max(0, from - S::COST);
         e = max(0, to - S::COST);
     }
@@ -206,7 +212,7 @@ template <class S> struct AdPiece {
                     } while (s.nt == 0);
                 }
             }
-            take(0);
+            take(A, 0);
         } while (e == 0);
         return true;
     }
@@ -224,6 +230,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     constexpr int NB = D / BS, MT = D / 16, MB = BS / 16, RT = S::RT, G = S::G;   // MB: k steps, and channel tiles, per block
     constexpr int HALF = kv4_half_bytes(D, BS), SOFF = KV4_GROUP * (D / 2);
     extern __shared__ __align__(128) unsigned char smem[];
+    if (A.redo) pdl_grid_dependency_wait();                          // (before any return: this kernel's end means the ends of those before)
     if (smem_u32(smem) != AD_BASE) {                                 // the layout counts on it
         if (threadIdx.x == 0) atomicExch(&g_attn4_status, 403);
         return;
@@ -232,6 +239,14 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     const int in_team = cta_warp / AD_WARPS, warp = cta_warp % AD_WARPS;
     const int teams = gridDim.x * S::TEAMS, team = in_team * gridDim.x + blockIdx.x;   // little work spreads over the SMs
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + (S::END - 16 - AD_BASE));
+    if (A.redo) {                                                    // (mostly there is nothing to do)
+        if (__syncthreads_or(threadIdx.x < A.wide_n && __ldcg(A.wide + threadIdx.x) != 0) == 0) return;
+        uint32_t mask = 0;
+        for (int i = lane; i < A.wide_n; i += 32) mask |= __ldcg(A.wide + i);
+        mask = __reduce_or_sync(0xffffffffu, mask);
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(S::REDO), "r"(mask) : "memory");
+        __syncwarp();
+    }
     // little work is a chain of small loads: those of the lengths, and of the page table into L2, are under way while the table is made
     const int64_t units = ad_units<S>(A, lane);
     if (cta_warp == 0 && lane < A.sq.batch && A.sq.capacity > 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(A.sq.table + (int64_t)lane * A.sq.table_ld));
@@ -262,7 +277,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     const int64_t per = ad_per(total, teams, S::COST), t0 = min(total, team * per), t1 = min(total, t0 + per);
     // what the teams leave for attn4_combine_kernel (a team's thread 0 writes both)
     Attn4Join *join = attn4_join<D, RT>(A.ws, teams) + team;
-    if (warp == 0 && lane == 0) join->n = 0;
+    if (!A.redo && warp == 0 && lane == 0) join->n = 0;
     Piece in;                                                        // piece the next copy belongs to
     const bool some = t0 < t1 && in.start(A, units, inc, t0, t1);
     __syncthreads();
@@ -807,9 +822,19 @@ static int ad_launch(const Attn4Args &a, cudaStream_t st) {
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     const int teams = ad_teams(D, NT);
-    attn4_decode_kernel<D, BS, NT, T><<<teams / S::TEAMS, S::THREADS, S::BYTES, st>>>(a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(teams / S::TEAMS);
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = a.redo ? 1 : 0;
+    MPSBNB_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_decode_kernel<D, BS, NT, T>, a));
     int rc = check_launch();
-    if (rc != MPSBNB_OK) return rc;
+    if (rc != MPSBNB_OK || a.redo) return rc;
     return attn4_combine<D, S::RT, 1, T>(a, teams, st);
 }
 
@@ -832,17 +857,47 @@ int attn4_decode_status_fetch(int *out, bool reset) {
 
 using namespace mpsbnb;
 
+// bytes of workspace: partial results of the kernel here, then - where prompts may go to the other one - a word for each of its blocks
+// and its partial results
+static size_t ad_wide_ws() { return ((size_t)sm_count() * sizeof(uint32_t) + 15) & ~(size_t)15; }
 static size_t ad_tokens_ws(int D, int nt) {
     return ((size_t)ad_teams(D, nt) * (2 * (8 * nt) * (D + 2) * sizeof(float) + sizeof(Attn4Join)) + 15) & ~(size_t)15;
+}
+
+static size_t ad_tokens_ws(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group) {
+    const size_t any = ad_tokens_ws(c->head_dim, ad_nt(s, group)), mixed = ad_tokens_ws(c->head_dim, group > 8 ? 2 : 1);
+    return any > mixed ? any : mixed;
+}
+static int ad_run(const Attn4Args &a, const mpsbnb_kv4_cache *c, int nt, cudaStream_t st) {
+    if (c->blocksize == 32) {
+        if (c->head_dim == 64) return ad_launch_t<64, 32>(a, c->dtype, nt, st);
+        if (c->head_dim == 128) return ad_launch_t<128, 32>(a, c->dtype, nt, st);
+        return ad_launch_t<256, 32>(a, c->dtype, nt, st);
+    }
+    if (c->head_dim == 64) return ad_launch_t<64, 64>(a, c->dtype, nt, st);
+    if (c->head_dim == 128) return ad_launch_t<128, 64>(a, c->dtype, nt, st);
+    return ad_launch_t<256, 64>(a, c->dtype, nt, st);
+}
+// the prompt kernel, and behind it the one here for what that does not take (16 rows per tile: there are many)
+static int ad_prompt(Attn4Args a, const mpsbnb_kv4_cache *c, bool split, cudaStream_t st) {
+    float *const ws = a.ws;
+    a.ws = reinterpret_cast<float *>(reinterpret_cast<char *>(a.wide) + ad_wide_ws());
+    const int rc = attn4_prompt(a, c->head_dim, c->blocksize, c->dtype, split, st, &a.wide_n);
+    if (rc != MPSBNB_OK) return rc;
+    a.ws = ws;
+    a.redo = 1;
+    return ad_run(a, c, 2, st);
 }
 
 extern "C" size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads) {
     if (kv4_check_cache(cache, 0) != MPSBNB_OK || kv4_check_seqs(seqs, cache) != MPSBNB_OK) return 0;
     if (heads <= 0 || heads % cache->kv_heads != 0 || seqs->batch == 0 || seqs->tokens == 0) return 0;
-    const int group = heads / cache->kv_heads, nt = ad_nt(seqs, group), few = group > 8 ? 2 : 1;
-    const size_t any = ad_tokens_ws(cache->head_dim, nt), mixed = ad_tokens_ws(cache->head_dim, few), tokens = any > mixed ? any : mixed;
+    const int group = heads / cache->kv_heads;
     // (a window, not known here, may take the prompt kernel out, not bring it in)
-    return tokens + (ad_kind(cache, seqs, group, 0) == AD_PROMPTS_SPLIT || ad_mixed(cache, seqs, group, 0) ? attn4_prompt_ws(cache->head_dim) : 0);
+    const AdKind kind = ad_kind(cache, seqs, group, 0);
+    const bool mixed = ad_mixed(cache, seqs, group, 0);
+    return ad_tokens_ws(cache, seqs, group) + (kind != AD_TOKENS || mixed ? ad_wide_ws() : 0) +
+           (kind == AD_PROMPTS_SPLIT || mixed ? attn4_prompt_ws(cache->head_dim) : 0);
 }
 
 extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
@@ -870,27 +925,19 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     static const float codes[2][16] = {MPSBNB_NF4_TABLE, MPSBNB_FP4_TABLE};
     for (int i = 0; i < 16; ++i) a.code[i] = codes[cache->quant_type][i] * attn4_code_scale(cache->quant_type);
     a.rows_lo = 0; a.rows_hi = 0x7fffffff;
+    a.wide = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(workspace) + ad_tokens_ws(cache, seqs, group));
+    a.wide_n = a.redo = 0;
     cudaStream_t st = (cudaStream_t)stream;
     int nt = ad_nt(seqs, group);
     if (ad_mixed(cache, seqs, group, window)) {
         nt = group > 8 ? 2 : 1;
         a.rows_lo = ad_few_rows(cache->head_dim);
-        a.ws = (float *)((char *)workspace + ad_tokens_ws(cache->head_dim, nt));
-        rc = attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, ad_split(cache, seqs, group), st);
+        rc = ad_prompt(a, cache, ad_split(cache, seqs, group), st);
         if (rc != MPSBNB_OK) return rc;
         a.rows_hi = a.rows_lo; a.rows_lo = 0;
-        a.ws = (float *)workspace;
     } else {
         const AdKind kind = ad_kind(cache, seqs, group, window);
-        if (kind != AD_TOKENS) return attn4_prompt(a, cache->head_dim, cache->blocksize, cache->dtype, kind == AD_PROMPTS_SPLIT, st);
+        if (kind != AD_TOKENS) return ad_prompt(a, cache, kind == AD_PROMPTS_SPLIT, st);
     }
-    const int dt = cache->dtype;
-    if (cache->blocksize == 32) {
-        if (cache->head_dim == 64) return ad_launch_t<64, 32>(a, dt, nt, st);
-        if (cache->head_dim == 128) return ad_launch_t<128, 32>(a, dt, nt, st);
-        return ad_launch_t<256, 32>(a, dt, nt, st);
-    }
-    if (cache->head_dim == 64) return ad_launch_t<64, 64>(a, dt, nt, st);
-    if (cache->head_dim == 128) return ad_launch_t<128, 64>(a, dt, nt, st);
-    return ad_launch_t<256, 64>(a, dt, nt, st);
+    return ad_run(a, cache, nt, st);
 }

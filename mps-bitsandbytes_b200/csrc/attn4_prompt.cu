@@ -31,7 +31,9 @@
 // off by 4.8e-4 of its size, half a step of its type (its own rounding: 2.1e-4 on average); a bf16 output shows nothing of it.
 // Products in TF32 would halve the rate and double the operands.
 // fp16 operands hold bf16 caches too: the absmax of a K tile (and, carried along, of the V tiles) is brought near 2^8 by
-// a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.
+// a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.  Blocks of elements that this
+// leaves under 2^-14, of which fp16 keeps too few bits, are noticed: their sequence is done again by attn4_decode_kernel, which
+// takes any magnitudes side by side.
 #include <type_traits>
 
 #include "attn4.cuh"
@@ -281,7 +283,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
     using S = ApSmem<D, BS>;
     constexpr int TILES = S::TILES, KT = S::KT, NB = D / BS, SOFF = KV4_GROUP * (D / 2), HALF = kv4_half_bytes(D, BS);
     constexpr bool BF = !std::is_same<T, __half>::value;
-    constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
+    constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u, FLOOR = BF ? 0x322cu : 0u;   // of 16-bit absmax; FLOOR: the quantiser's 1e-8
     using Item = ApItem<TILES, KT>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t sb = smem_u32(smem), bar = sb + S::BAR;
@@ -300,6 +302,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
     auto q_empty = [&](int t) { return bar + 144 + 8u * t; };
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + S::BAR + 160);
     volatile uint32_t *abort_flag = tmem_slot + 1, *never = tmem_slot + 2;               // never: stays 0
+    uint32_t *wide = reinterpret_cast<uint32_t *>(smem + S::BAR + 172);
     volatile float *k_pow = reinterpret_cast<volatile float *>(smem + S::BAR + 176);     // [4]: power of two of a K tile
     volatile int *v_exp = reinterpret_cast<volatile int *>(smem + S::BAR + 192);         // [4]: V's exponent from a tile on
     volatile uint8_t *q_exp = smem + S::EXPO;
@@ -316,7 +319,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
             mbar_init(q_full(i), S::Q_WARPS); mbar_init(q_empty(i), 1);
         }
         for (int i = 0; i < 4; ++i) { mbar_init(item_full(i), 1); mbar_init(item_empty(i), 4 * TILES + AP_EXPANDERS + 1 + S::Q_WARPS); }   // (1: the issuer)
-        *abort_flag = *never = 0;
+        *abort_flag = *never = *wide = 0;
         fence_mbar_init();
     }
     if (warp == AP_MMA) {
@@ -707,13 +710,25 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
                         asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sbits[it]) : "r"(src + sc0));
                     }
                     AP_WAIT(buf_empty(slot), ring_phase ^ 1, 418);
+                    float sc[PER], low = __int_as_float(0x7f800000);
+#pragma unroll
+                    for (int it = 0; it < PER; ++it) {
+                        sc[it] = to_f32<T>(*reinterpret_cast<const T *>(&sbits[it])) * (side == 0 ? down_k : down_v);
+                        low = fminf(low, sc[it]);
+                    }
+                    if (low < 0x1p-14f) {
+#pragma unroll
+                        for (int it = 0; it < PER; ++it) {
+                            const int place = place0 + tok + it * STEP;
+                            if (sc[it] < 0x1p-14f && sbits[it] > FLOOR && place >= w.lo && place < w.hi) atomicOr(wide, 1u << (w.b & 31));
+                        }
+                    }
                     if (side == 0 && w0 == 0 && lane == 0) { k_pow[jj & 3] = __int_as_float((ek - 8) << 23); v_exp[jj & 3] = v_cur; }
                     const uint32_t tile = sb + S::RING + slot * S::BUF;
 #pragma unroll
                     for (int it = 0; it < PER; ++it) {
-                        float s = to_f32<T>(*reinterpret_cast<const T *>(&sbits[it]));
+                        float s = sc[it];
                         if (side == 0) {
-                            s *= down_k;
                             if (odd) {                               // it has to reach the rows that see it and no others: through its key
 #pragma unroll
                                 for (int e = 0; e < NB; ++e) {
@@ -723,7 +738,6 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
                                 }
                             }
                         } else {
-                            s *= down_v;
                             const int place = place0 + tok + it * STEP;
                             if (part && (place < w.lo || place >= w.hi)) s = 0.0f;
                             if (odd && (sbits[it] & INF) == INF) s = 0.0f;
@@ -944,6 +958,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
 #undef AP_WAIT
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) A.wide[blockIdx.x] = *wide;
     if (warp == AP_MMA) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -954,7 +969,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
 // host side
 // ------------------------------------------------------------------------------------------
 template <int D, int BS, typename T>
-static int ap_launch(const Attn4Args &a, bool split, cudaStream_t st) {
+static int ap_launch(const Attn4Args &a, bool split, cudaStream_t st, int *grid_out) {
     using S = ApSmem<D, BS>;
     constexpr int smem = S::TOTAL;
     static_assert(smem <= 227 * 1024, "shared memory of the prompt kernel");
@@ -973,6 +988,7 @@ static int ap_launch(const Attn4Args &a, bool split, cudaStream_t st) {
     const int64_t most = a.kv.kv_heads * (((int64_t)a.sq.tokens * a.group) / (S::TILES * 128) + a.sq.batch);
     const int sms = sm_count();
     const int grid = split || most > sms ? sms : (int)most;
+    *grid_out = grid;
     attn4_prompt_kernel<D, BS, T><<<grid, AP_THREADS, smem, st>>>(a, (int)blocks, split);
     const int rc = check_launch();
     return rc != MPSBNB_OK || !split ? rc : attn4_combine<D, S::TILES * 128, ATTN4_JOIN_WARPS, T>(a, grid, st);
@@ -983,8 +999,8 @@ size_t attn4_prompt_ws(int head_dim) {
     return (size_t)sm_count() * (2 * rows * (head_dim + 2) * sizeof(float) + sizeof(Attn4Join));
 }
 
-int attn4_prompt(const Attn4Args &a, int head_dim, int blocksize, int dtype, bool split, cudaStream_t st) {
-#define AP_PICK(D, BS) return dtype == MPSBNB_F16 ? ap_launch<D, BS, __half>(a, split, st) : ap_launch<D, BS, __nv_bfloat16>(a, split, st)
+int attn4_prompt(const Attn4Args &a, int head_dim, int blocksize, int dtype, bool split, cudaStream_t st, int *grid) {
+#define AP_PICK(D, BS) return dtype == MPSBNB_F16 ? ap_launch<D, BS, __half>(a, split, st, grid) : ap_launch<D, BS, __nv_bfloat16>(a, split, st, grid)
     if (blocksize == 32) {
         if (head_dim == 64) AP_PICK(64, 32);
         if (head_dim == 128) AP_PICK(128, 32);

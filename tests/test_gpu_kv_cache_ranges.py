@@ -135,3 +135,106 @@ def test_blocks_of_zeros_beside_others(dtype):
     got = bnb.attention_4bit(q[None], cache, 0, table, lens)[0]
     close(got, *reference(q, cache, 0, table[0], 120))
     assert (got[..., 96:].abs() < 1e-7).all()
+
+
+#  heads, kv heads, new tokens of each sequence: keys shared out; not; prompts among single tokens
+PROMPTS = [(32, 8, [150, 300, 129]), (64, 16, [100, 33, 256, 64, 1, 17, 130, 70, 90] * 2), (32, 8, [1, 1, 400, 3, 1, 2, 1, 13])]
+
+
+def _prompts(head_dim, blocksize, dtype, heads, kv_heads, new, before, gen, change):
+    """A cache of the sequences' keys and values, change(k, v, b) made to those of each, and what an attention call takes."""
+    import kv_util as U
+    page = 32
+    lens = [n + before for n in new]
+    width = -(-max(lens) // page)
+    cache = bnb.KVCache4bit(1, len(new) * width, kv_heads, head_dim, page_size=page, blocksize=blocksize, dtype=dtype)
+    table = U.widen(U.random_table(len(new), width, len(new) * width), page)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    rows = [0]
+    for n in lens:
+        rows.append(rows[-1] + n)
+    k, v = (torch.randn(rows[-1], kv_heads, head_dim, generator=gen, device="cuda") for _ in range(2))
+    for b in range(len(new)):
+        change(k[rows[b]:rows[b + 1]], v[rows[b]:rows[b + 1]], b)
+    bnb.append_kv_4bit(cache, 0, k.to(dtype), v.to(dtype), table, _i32(lens), _i32(rows))
+    q = torch.randn(starts[-1], heads, head_dim, generator=gen, device="cuda").to(dtype)
+    return cache, table, lens, starts, q
+
+
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("heads,kv_heads,new", PROMPTS, ids=["shared out", "whole", "mixed"])
+@pytest.mark.parametrize("head_dim,blocksize,dtype,large", [(128, 64, BF16, 1e10), (128, 32, F16, 6e4), (64, 64, BF16, 1e25), (256, 64, BF16, 1e10)])
+def test_a_prompts_token_of_any_magnitude_leaves_the_rows_before_it_alone(head_dim, blocksize, dtype, large, heads, kv_heads, new, side):
+    gen = torch.Generator(device="cuda").manual_seed(head_dim)
+    at = {b: n // 2 for b, n in enumerate(new) if n > 30 and b % 4 != 1}   # (of the new tokens)
+
+    def change(k, v, b):
+        if dtype == F16:
+            k.mul_(2.0 ** -12), v.mul_(2.0 ** -12)
+        if b in at:
+            x = (k if side == "k" else v)[20 + at[b]]
+            x.copy_(large * torch.sign(x))
+    cache, table, lens, starts, q = _prompts(head_dim, blocksize, dtype, heads, kv_heads, new, 20, gen, change)
+    got, lse = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), max(new), return_lse=True)
+    again, lse2 = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), max(new), return_lse=True)
+    for b, n in enumerate(new):
+        rows = slice(starts[b], starts[b + 1])
+        want, limit = reference(q[rows], cache, 0, table[b], lens[b])
+        some = at.get(b, n) if side == "k" else n                    # (scores of 1e10 know no limit)
+        close(got[rows][:some], want[:some], limit[:some])
+        assert torch.equal(got[rows][:some], again[rows][:some]) and torch.equal(lse[rows][:some], lse2[rows][:some]) and torch.isfinite(lse[rows][:some]).all()
+    assert_device_ok()
+
+
+@pytest.mark.parametrize("heads,kv_heads,new", PROMPTS, ids=["shared out", "whole", "mixed"])
+@pytest.mark.parametrize("head_dim,blocksize,dtype,sizes", [(128, 64, F16, (6e4, 1e-4)), (128, 32, BF16, (1e12, 1e-3)), (64, 32, BF16, (1.0, 1e-7)), (256, 32, F16, (100.0, 1e-6))])
+def test_prompts_with_small_values_behind_or_beside_large_ones(head_dim, blocksize, dtype, sizes, heads, kv_heads, new):
+    """Where large values lie far before the small ones, among them (with a window, of rows that see the small ones alone), or in
+    another block of channels; sequences of ordinary ones beside them."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+
+    def change(k, v, b):
+        if b % 3 == 1:
+            return
+        v.clamp_(-1, 1).mul_(sizes[1])
+        if b % 3 == 0:
+            v[:60] *= sizes[0] / sizes[1]
+        else:
+            v[..., :blocksize] *= sizes[0] / sizes[1]
+        v.clamp_(-sizes[0], sizes[0])
+    cache, table, lens, starts, q = _prompts(head_dim, blocksize, dtype, heads, kv_heads, new, 70, gen, change)
+    got = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), max(new), window=16)
+    for b, n in enumerate(new):
+        rows = slice(starts[b], starts[b + 1])
+        close(got[rows], *reference(q[rows], cache, 0, table[b], lens[b], 16))
+    assert_device_ok()
+
+
+def test_a_graph_of_prompts_follows_magnitudes():
+    """Captured over ordinary values, replayed over others and back."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    cache, table, lens, starts, q = _prompts(128, 64, BF16, 32, 8, [150, 300, 129], 20, gen, lambda k, v, b: None)
+    args = (q, cache, 0, table, _i32(lens), _i32(starts), 300)
+    clean = bnb.attention_4bit(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = bnb.attention_4bit(*args)
+    before = cache.data.clone()
+    for large in (False, True, False, True):
+        cache.data.copy_(before)
+        if large:
+            page, place = table[1, 250 // 32], 250 % 32
+            cache.v_absmax[0, page, :, place // 16, place % 16] = 1e12
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        if not large:
+            assert torch.equal(out, clean)
+        else:
+            for b, n in enumerate([150, 300, 129]):
+                rows = slice(starts[b], starts[b + 1])
+                close(out[rows], *reference(q[rows], cache, 0, table[b], lens[b]))
+            assert torch.equal(out[:150], clean[:150]) and torch.equal(out[450:], clean[450:])
+    assert_device_ok()
