@@ -498,7 +498,7 @@ int mpsbnb_kv4_copy_pages(const mpsbnb_kv4_cache *cache, const int32_t *src, con
  * for keys: never on the lengths, so a captured graph follows them.
  * Keys and values of any magnitude may lie side by side: those that a row does not see, or sees with next to no weight, take nothing
  * from its precision.  (Where the magnitudes of blocks of keys, or of values, that some block of rows sees are more than 2^22
- * apart, the sequence's prompt is done again by the kernel for single tokens, some ten times slower.  An absmax of 1e-8 or less
+ * apart, or a score times log2(e) is 2^20 or more, the sequence's prompt is done again by the kernel for single tokens, some ten times slower.  An absmax of 1e-8 or less
  * counts as nothing beside a larger one.)
  * workspace: mpsbnb_attention_4bit_workspace_bytes() bytes, 16-byte aligned, used by this call only while it runs. */
 size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads);

@@ -32,7 +32,10 @@ struct Attn4Args {
 __host__ __device__ inline float attn4_code_scale(int quant_type) { return quant_type == MPSBNB_NF4 ? ATTN4_NF4_SCALE : 1.0f; }
 __device__ __forceinline__ float attn4_code_unscale(int quant_type) { return quant_type == MPSBNB_NF4 ? 1.0f / ATTN4_NF4_SCALE : 1.0f; }
 
-constexpr float ATTN4_NONE = -1e30f;             // running maximum before any key has been seen
+constexpr float ATTN4_NONE = -0x1p127f;          // running maximum before any key has been seen
+// From this reference on, the fused score * factor - reference is no longer the difference of two rounded products: for scores of 1e10
+// it leaves up to 2^9 of the reference's rounding, where the largest must leave 0.
+constexpr float ATTN4_FAR = 0x1p20f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

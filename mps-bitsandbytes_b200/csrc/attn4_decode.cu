@@ -420,6 +420,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) { m[nt][j] = ATTN4_NONE; l[nt][j] = 0.0f; }
+        bool far = false;                                            // some column's reference is
 
         int place0 = (sq.tlo + cur.a + warp) * S::TOK;
 #pragma unroll 1
@@ -543,7 +544,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
             };
             // p stays under 2^8 and absmax * up in [2^-4, 2^7]: their product is at home in fp16
             auto least = [&]() { return __int_as_float((250 << 23) - __float_as_int(up)); };   // 2^-4 / up
-            const bool high = top > 8.0f || sm * up > 128.0f;
+            const bool high = top > 8.0f || sm * up > 128.0f || far;
             if (__any_sync(0xffffffffu, high || sn < least())) {
                 uint32_t sl = 0xffffffffu;                           // the least above the floor, as bits from there on
 #pragma unroll
@@ -585,15 +586,17 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                             mx *= f[nt][j];
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                            const float mn = mx > m[nt][j] + 8.0f ? mx : m[nt][j], k = ex2(m[nt][j] - mn);
+                            const float mn = mx > m[nt][j] + (fabsf(m[nt][j]) < ATTN4_FAR ? 8.0f : 0.0f) ? mx : m[nt][j], k = ex2(m[nt][j] - mn);
+                            const bool off = fabsf(mn) >= ATTN4_FAR && mn != ATTN4_NONE;
+                            far = far || off;
                             m[nt][j] = mn;
                             l[nt][j] *= k;
 #pragma unroll
                             for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k * ku; o[i][nt][j + 2] *= k * ku; }
 #pragma unroll
                             for (int x = 0; x < G; ++x) {
-                                p[x][nt][j] = fmaf(s[x][nt][j], f[nt][j], -mn);
-                                p[x][nt][j + 2] = fmaf(s[x][nt][j + 2], f[nt][j], -mn);
+                                p[x][nt][j] = off ? __fmul_rn(s[x][nt][j], f[nt][j]) - mn : fmaf(s[x][nt][j], f[nt][j], -mn);
+                                p[x][nt][j + 2] = off ? __fmul_rn(s[x][nt][j + 2], f[nt][j]) - mn : fmaf(s[x][nt][j + 2], f[nt][j], -mn);
                             }
                         }
                     if (sm * up > 128.0f || low()) {

@@ -33,7 +33,7 @@
 // fp16 operands hold bf16 caches too: the absmax of a K tile (and, carried along, of the V tiles) is brought near 2^8 by
 // a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.  Blocks of elements that this
 // leaves under 2^-14, of which fp16 keeps too few bits, are noticed: their sequence is done again by attn4_decode_kernel, which
-// takes any magnitudes side by side.
+// takes any magnitudes side by side, and scores of any size.
 #include <type_traits>
 
 #include "attn4.cuh"
@@ -837,7 +837,11 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
                 a0 = fmaxf(a0, a1);
                 const float top = a0 == __int_as_float(0xff800000) ? ATTN4_NONE : a0 * fj;
                 float k = 1.0f;
-                if (top > m + 8.0f) { k = ex2(m - top); m = top; }
+                if (top > m + 8.0f) {
+                    k = ex2(m - top);
+                    m = top;
+                    if (fabsf(top) >= ATTN4_FAR) atomicOr(wide, 1u << (w.b & 31));
+                }
                 const uint64_t f2 = ap_pack2(__float_as_uint(fj), __float_as_uint(fj));
                 const uint64_t b2 = ap_pack2(__float_as_uint(AP_LIFT - m), __float_as_uint(AP_LIFT - m));
                 uint64_t add = 0;

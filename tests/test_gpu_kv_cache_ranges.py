@@ -238,3 +238,37 @@ def test_a_graph_of_prompts_follows_magnitudes():
                 close(out[rows], *reference(q[rows], cache, 0, table[b], lens[b]))
             assert torch.equal(out[:150], clean[:150]) and torch.equal(out[450:], clean[450:])
     assert_device_ok()
+
+
+@pytest.mark.parametrize("heads,kv_heads,new", [(4, 2, [1, 3])] + PROMPTS, ids=["tokens", "shared out", "whole", "mixed"])
+@pytest.mark.parametrize("head_dim,dtype,size", [(128, BF16, 2.0 ** 13), (128, BF16, 2.0 ** 30), (64, BF16, 2.0 ** 45), (256, BF16, 2.0 ** 7), (128, F16, 2.0 ** 10)])
+def test_scores_of_any_size(head_dim, dtype, size, heads, kv_heads, new):
+    """Every score is size^2 times +-2^(0 .. 3) times head_dim ** 0.5, many of them equal: the weights are shared by the largest that a row sees."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+
+    def change(k, v, b):
+        order = torch.randint(0, 4, (k.shape[0], 1, 1), generator=gen, device="cuda")
+        k.copy_(size * 2.0 ** order * torch.where(torch.arange(head_dim, device="cuda") % 3 == 0, -1.0, 1.0))
+    cache, table, lens, starts, q = _prompts(head_dim, 64, dtype, heads, kv_heads, new, 20, gen, change)
+    signs = torch.where(torch.arange(head_dim, device="cuda") % 3 == 0, -size, size).to(dtype)
+    q[:, ::2], q[:, 1::2] = signs, -signs
+    got, lse = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), max(new), return_lse=True)
+    import kv_util as U
+    for b, n in enumerate(new):
+        k, v = (U.rows_of(cache, 0, table[b], 0, lens[b], x) for x in "kv")
+        seen = torch.arange(lens[b], device="cuda")[None] <= torch.arange(lens[b] - n, lens[b], device="cuda")[:, None]
+        for h in range(heads):
+            g = h // (heads // kv_heads)
+            s = (q[starts[b]:starts[b + 1], h].double() @ k[:, g].T * head_dim ** -0.5).masked_fill(~seen, -math.inf)
+            top = s.amax(-1, keepdim=True)
+            p = (s == top).double()                                  # (the others are 2^13 at least below)
+            total = p.sum(-1, keepdim=True)
+            p /= total
+            size_v = p @ v[:, g].abs()
+            want, out = p @ v[:, g], got[starts[b]:starts[b + 1], h].double()
+            limit = size_v * (3 * 2.0 ** -11 + lens[b] * 2.0 ** -23 + 2.0 ** -18) + HALF_STEP[dtype] * size_v * 1.01 + 2.0 ** -25
+            worst = ((out - want).abs() / limit).max().item()
+            assert torch.isfinite(out).all() and worst <= 1.0, f"off by {worst:.3g} of the limit"
+            want_lse = top[:, 0] + torch.log(total[:, 0])
+            assert ((lse[starts[b]:starts[b + 1], h].double() - want_lse).abs() <= 2.0 ** -9 * want_lse.abs() + 1e-3).all()
+    assert_device_ok()
