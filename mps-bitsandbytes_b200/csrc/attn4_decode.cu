@@ -322,12 +322,14 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
         }
         const uint32_t full = bars + 8 * put, dst = ring + put * S::STAGE;
         if (in_bad >> (at * G) & ((1u << G) - 1u)) {
-            // a page outside the cache: its keys' absmax is NaN, and so is every row that sees them
+            // a page outside the cache: its keys' absmax is NaN, and so is every row that sees them; its values' is 0, not what lies there
 #pragma unroll
             for (int x = 0; x < G; ++x)
                 if (in_bad >> (at * G + x) & 1u)
-                    for (int i = lane; i < KV4_GROUP * NB; i += 32)
+                    for (int i = lane; i < KV4_GROUP * NB; i += 32) {
                         asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + x * S::GROUP + SOFF + 2 * i), "h"((uint16_t)0x7fff) : "memory");
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + x * S::GROUP + HALF + SOFF + 2 * i), "h"((uint16_t)0) : "memory");
+                    }
             if (lane == 0) atomicExch(&g_attn4_status, KV4_BAD_PAGE);
             __syncwarp();
         }
