@@ -131,7 +131,14 @@ template <int D, int RT, int ROWS, typename T> static int attn4_combine(const At
     return check_launch();
 }
 
-// attn4_prompt.cu.  split: its blocks share out the keys evenly and leave partial results.  grid: how many wrote their word of `wide`
+// Dynamic shared memory of a kernel without any other begins behind what the system keeps for itself, here at `address`?
+inline bool attn4_smem_at(int dev, int address) {
+    int kept = -1;
+    return cudaDeviceGetAttribute(&kept, cudaDevAttrReservedSharedMemoryPerBlock, dev) == cudaSuccess && kept == address;
+}
+
+// attn4_prompt.cu; MPSBNB_ERR_UNSUPPORTED, and nothing launched, where the compiler or the device does not meet what the kernel counts on.
+// split: its blocks share out the keys evenly and leave partial results.  grid: how many wrote their word of `wide`
 int attn4_prompt(const Attn4Args &a, int head_dim, int blocksize, int dtype, bool split, cudaStream_t st, int *grid);
 size_t attn4_prompt_ws(int head_dim);            // bytes of workspace when split
 

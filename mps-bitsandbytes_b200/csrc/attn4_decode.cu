@@ -232,7 +232,8 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
     extern __shared__ __align__(128) unsigned char smem[];
     if (A.redo) pdl_grid_dependency_wait();                          // (before any return: this kernel's end means the ends of those before)
     if (smem_u32(smem) != AD_BASE) {                                 // the layout counts on it
-        if (threadIdx.x == 0) atomicExch(&g_attn4_status, 403);
+        if (threadIdx.x == 0) atomicExch(&g_attn4_status, 403);      // (and nothing to join)
+        if (!A.redo && threadIdx.x < S::TEAMS) attn4_join<D, RT>(A.ws, gridDim.x * S::TEAMS)[threadIdx.x * gridDim.x + blockIdx.x].n = 0;
         return;
     }
     const int cta_warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -823,6 +824,7 @@ static int ad_launch(const Attn4Args &a, cudaStream_t st) {
     int dev = 0;
     MPSBNB_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
+        if (!attn4_smem_at(dev, AD_BASE)) return MPSBNB_ERR_UNSUPPORTED;   // the layout counts on it
         MPSBNB_CUDA_TRY(cudaFuncSetAttribute(attn4_decode_kernel<D, BS, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
@@ -938,11 +940,15 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
         nt = group > 8 ? 2 : 1;
         a.rows_lo = ad_few_rows(cache->head_dim);
         rc = ad_prompt(a, cache, ad_split(cache, seqs, group), st);
-        if (rc != MPSBNB_OK) return rc;
-        a.rows_hi = a.rows_lo; a.rows_lo = 0;
+        if (rc != MPSBNB_OK && rc != MPSBNB_ERR_UNSUPPORTED) return rc;
+        if (rc == MPSBNB_OK) a.rows_hi = a.rows_lo;                  // (else nothing has been launched: the kernel here takes all)
+        a.rows_lo = 0;
     } else {
         const AdKind kind = ad_kind(cache, seqs, group, window);
-        if (kind != AD_TOKENS) return ad_prompt(a, cache, kind == AD_PROMPTS_SPLIT, st);
+        if (kind != AD_TOKENS) {
+            rc = ad_prompt(a, cache, kind == AD_PROMPTS_SPLIT, st);
+            if (rc != MPSBNB_ERR_UNSUPPORTED) return rc;
+        }
     }
     return ad_run(a, cache, nt, st);
 }

@@ -288,7 +288,11 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t sb = smem_u32(smem), bar = sb + S::BAR;
     if ((sb & 1023u) != 0) {                                         // the swizzle counts on it
-        if (threadIdx.x == 0) atomicExch(&g_attn4_prompt_status, 410);
+        if (threadIdx.x == 0) {                                      // (nothing to join, everything to be done again)
+            atomicExch(&g_attn4_prompt_status, 410);
+            if (split) attn4_join<D, TILES * 128>(A.ws, gridDim.x)[blockIdx.x].n = 0;
+            A.wide[blockIdx.x] = 0xffffffffu;
+        }
         return;
     }
     auto buf_full = [&](int s) { return bar + 8u * s; };             // [3]
@@ -981,6 +985,7 @@ static int ap_launch(const Attn4Args &a, bool split, cudaStream_t st, int *grid_
     int dev = 0;
     MPSBNB_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
+        if (!attn4_smem_at(dev, 1024)) return MPSBNB_ERR_UNSUPPORTED;
         MPSBNB_CUDA_TRY(cudaFuncSetAttribute(attn4_prompt_kernel<D, BS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         cudaFuncAttributes at;
         MPSBNB_CUDA_TRY(cudaFuncGetAttributes(&at, attn4_prompt_kernel<D, BS, T>));
