@@ -449,8 +449,9 @@ typedef struct mpsbnb_kv4_cache {
 /* The sequences of a call.  Sequence b holds seq_lens[b] tokens (the call's new ones included; clamped to what its
  * row of the page table can hold) in the pages page_table[b * table_ld + 0 ...].  Its new tokens are rows
  * cu_seqlens[b] ... cu_seqlens[b + 1] - 1 of the call's [tokens, ...] tensors, or rows b * new_tokens ... with
- * cu_seqlens NULL; they take the last places of the sequence.  new_tokens is the largest number of new tokens of a
- * sequence (more are not looked at).  All tables are int32 on the device; they must not change while a call reads them. */
+ * cu_seqlens NULL; they take the last places of the sequence.  With cu_seqlens, new_tokens is the largest number of new
+ * tokens of a sequence as far as the caller knows it: the choice of kernels goes by it, not the result.  All tables are int32 on
+ * the device; they must not change while a call reads them. */
 typedef struct mpsbnb_kv4_seqs {
     const int32_t *page_table;
     int64_t table_ld;

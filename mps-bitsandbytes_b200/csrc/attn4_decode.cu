@@ -915,10 +915,11 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     if (rc != MPSBNB_OK) return rc;
     if (heads <= 0 || heads % cache->kv_heads != 0 || window < 0 || (window > 0 && !causal) || !(fabsf(scale) < INFINITY)) return MPSBNB_ERR_INVALID_ARG;
     if (q_token_stride < 0 || q_head_stride < 0) return MPSBNB_ERR_INVALID_ARG;
-    if (seqs->batch == 0 || seqs->tokens == 0 || seqs->new_tokens == 0) return MPSBNB_OK;
+    if (seqs->batch == 0 || seqs->tokens == 0) return MPSBNB_OK;
     if (q == nullptr || out == nullptr) return MPSBNB_ERR_INVALID_ARG;
     const int group = heads / cache->kv_heads;
-    if ((int64_t)seqs->new_tokens * group > 0x3fffffffll) return MPSBNB_ERR_TOO_LARGE;
+    // rows of a sequence and head are 32-bit numbers, with room for the tile behind the last (outputs of 2^31 rows: 256 GB and more)
+    if (seqs->tokens * group > 0x7ffff000ll) return MPSBNB_ERR_TOO_LARGE;
     if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < mpsbnb_attention_4bit_workspace_bytes(cache, seqs, heads)) return MPSBNB_ERR_WORKSPACE;
     // rows are fetched in 16-byte pieces
     if (!aligned16(q) || ((q_token_stride | q_head_stride) & 7) != 0 || !aligned16(out)) return MPSBNB_ERR_UNSUPPORTED;

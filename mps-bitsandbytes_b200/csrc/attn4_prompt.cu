@@ -279,7 +279,7 @@ template <int TILES, int KT> struct ApRun {
 
 template <int D, int BS, typename T>
 __global__ void __launch_bounds__(AP_THREADS, 1)
-attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) {
+attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int split) {
     using S = ApSmem<D, BS>;
     constexpr int TILES = S::TILES, KT = S::KT, NB = D / BS, SOFF = KV4_GROUP * (D / 2), HALF = kv4_half_bytes(D, BS);
     constexpr bool BF = !std::is_same<T, __half>::value;
@@ -451,6 +451,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int blocks, int split) 
             ApRun<TILES, KT> run;
             Attn4Join *join = attn4_join<D, TILES * 128>(A.ws, gridDim.x) + blockIdx.x;
             bool more = true;
+            const int blocks = (A.sq.longest() * A.group + TILES * 128 - 1) / (TILES * 128);   // of the longest sequence
             if (split) {
                 if (lane == 0) join->n = 0;
                 __syncwarp();
@@ -992,13 +993,12 @@ static int ap_launch(const Attn4Args &a, bool split, cudaStream_t st, int *grid_
         if (at.numRegs != AP_REGS) return MPSBNB_ERR_UNSUPPORTED;    // the warpgroups' shares are made for this number
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const int64_t blocks = ((int64_t)a.sq.new_tokens * a.group + S::TILES * 128 - 1) / (S::TILES * 128);
     // no more blocks than there can be items: a sequence's last block of rows may be partly filled
     const int64_t most = a.kv.kv_heads * (((int64_t)a.sq.tokens * a.group) / (S::TILES * 128) + a.sq.batch);
     const int sms = sm_count();
     const int grid = split || most > sms ? sms : (int)most;
     *grid_out = grid;
-    attn4_prompt_kernel<D, BS, T><<<grid, AP_THREADS, smem, st>>>(a, (int)blocks, split);
+    attn4_prompt_kernel<D, BS, T><<<grid, AP_THREADS, smem, st>>>(a, split);
     const int rc = check_launch();
     return rc != MPSBNB_OK || !split ? rc : attn4_combine<D, S::TILES * 128, ATTN4_JOIN_WARPS, T>(a, grid, st);
 }

@@ -32,19 +32,30 @@ struct Kv4Seqs {
     const int32_t *table, *lens, *cu;
     int64_t table_ld;
     int32_t capacity;                            // places that a row of the page table can hold
-    int32_t batch, new_tokens, tokens;
+    int32_t batch, new_tokens, tokens;           // new_tokens: of every sequence where cu is null, else not looked at
 
-    // first row of the call's tensors, number of new tokens (at most new_tokens) and length of sequence b
+    // first row of the call's tensors, number of new tokens and length of sequence b
     __device__ __forceinline__ void get(int b, int &row, int &n, int &len) const {
         if (cu != nullptr) {
             const int a = min(max(__ldg(cu + b), 0), tokens), e = min(max(__ldg(cu + b + 1), a), tokens);
             row = a;
-            n = min(e - a, new_tokens);
+            n = e - a;
         } else {
             row = b * new_tokens;
             n = new_tokens;
         }
         len = min(max(__ldg(lens + b), 0), capacity);
+    }
+    // the largest number of new tokens of a sequence; whole warp
+    __device__ __forceinline__ int longest() const {
+        if (cu == nullptr) return new_tokens;
+        int most = 0;
+        for (int b = threadIdx.x & 31; b < batch; b += 32) {
+            int row, n, len;
+            get(b, row, n, len);
+            most = max(most, n);
+        }
+        return __reduce_max_sync(0xffffffffu, most);
     }
 };
 

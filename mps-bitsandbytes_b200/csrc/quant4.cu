@@ -934,7 +934,7 @@ extern "C" int mpsbnb_kv4_append(const mpsbnb_kv4_cache *cache, int layer, const
     int rc = kv4_check_cache(cache, layer);
     if (rc == MPSBNB_OK) rc = kv4_check_seqs(seqs, cache);
     if (rc != MPSBNB_OK) return rc;
-    if (seqs->tokens == 0 || seqs->batch == 0 || seqs->new_tokens == 0) return MPSBNB_OK;
+    if (seqs->tokens == 0 || seqs->batch == 0) return MPSBNB_OK;
     if (k == nullptr || v == nullptr || k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0) return MPSBNB_ERR_INVALID_ARG;
     const Kv4Layer kv = kv4_layer(cache, layer);
     const Kv4Seqs sq = kv4_seqs(seqs, cache);

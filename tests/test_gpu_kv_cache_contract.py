@@ -47,3 +47,34 @@ def test_a_page_outside_the_cache_is_no_matter_of_the_rows_that_do_not_see_it(he
     for b in range(0, batch, 9):
         want, limit = reference(q[b], cache, 0, table[b], length, window)
         close(outs[2][b, 2:], want[2:, ::2], limit[2:, ::2])
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads,new,lens", [
+    (128, 8, 2, [3, 1, 9, 2], [40, 1, 77, 30]), (128, 32, 8, [300, 129, 1, 200], [400, 129, 30, 700]), (256, 16, 8, [257, 300], [500, 300]),
+    (64, 64, 16, [100, 33, 256, 64, 1, 17, 130] * 3, [177, 33, 400, 64, 5, 99, 131] * 3)])
+def test_max_seqlen_guides_the_choice_of_kernels_and_nothing_else(head_dim, heads, kv_heads, new, lens):
+    import kv_util as U
+    width = -(-max(lens) // 32)
+    cache = U.make_cache(len(new) * width, kv_heads, head_dim, 32, seed=3)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    narrow = U.random_table(len(new), width, len(new) * width)
+    q = torch.randn(starts[-1], heads, head_dim, device="cuda", dtype=F16)
+    want, _, bound = U.attention(q, cache, 0, narrow, lens, starts)
+    for table in (narrow, U.widen(narrow, 32)):
+        for longest in (0, 1, max(new) // 2, max(new), starts[-1], None):
+            U.check(bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), longest), want, bound, F16)
+    assert_device_ok()
+
+
+def test_append_stores_every_row_whatever_the_longest_is_said_to_be():
+    cache, other = (bnb.KVCache4bit(1, 8, 2, 64, page_size=16) for _ in range(2))
+    k, v = (torch.randn(20, 2, 64, device="cuda", dtype=F16) for _ in range(2))
+    table, lens, starts = _i32([[0, 1], [2, 3]]), _i32([17, 20]), _i32([0, 7, 20])
+    bnb.append_kv_4bit(other, 0, k, v, table, lens, starts)
+    for longest in (0, 3, 13, 20):
+        cache.data.zero_()
+        sq = N.Kv4Seqs(table.data_ptr(), 2, lens.data_ptr(), starts.data_ptr(), 20, 2, 2, longest)
+        assert N.lib().mpsbnb_kv4_append(cache._ref, 0, sq, k.data_ptr(), 128, 64, v.data_ptr(), 128, 64, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(cache.data, other.data) and cache.data.any()
