@@ -506,6 +506,11 @@ size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, cons
 int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,
                           int64_t q_token_stride, int64_t q_head_stride, int heads, int causal, int window, float scale,
                           void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+/* Which kernels that call runs: a sum of the following (0: nothing to do), or a negative status. */
+#define MPSBNB_ATTENTION_TOKENS 1      /* the kernel for single tokens */
+#define MPSBNB_ATTENTION_PROMPTS 2     /* the kernel for prompts; with the former, each for its sequences */
+#define MPSBNB_ATTENTION_SHARED_OUT 4  /* ... whose blocks share out the keys and whose partial results are joined */
+int mpsbnb_attention_4bit_kernels(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads, int window);
 
 #ifdef __cplusplus
 }

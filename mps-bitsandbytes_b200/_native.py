@@ -88,6 +88,7 @@ def lib():
         l.mpsbnb_kv4_dequantize.argtypes = [kv, int_, sq, i64_, ptr_, ptr_, ptr_]
         l.mpsbnb_kv4_copy_pages.argtypes = [kv, C.POINTER(C.c_int32), C.POINTER(C.c_int32), i64_, ptr_]
         l.mpsbnb_attention_4bit_workspace_bytes.argtypes = [kv, sq, int_]
+        l.mpsbnb_attention_4bit_kernels.argtypes = [kv, sq, int_, int_]
         l.mpsbnb_attention_4bit.argtypes = [kv, int_, sq, ptr_, i64_, i64_, int_, int_, int_, C.c_float, ptr_, ptr_, ptr_, C.c_size_t, ptr_]
         _lib = l
     return _lib

@@ -815,6 +815,13 @@ static bool ad_mixed(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int gr
 // rows a head up to which a sequence of a mixed call counts as single tokens: where the kernels' times per key meet
 static int ad_few_rows(int D) { return D == 64 ? 80 : D == 128 ? 48 : 32; }
 
+// what a call runs: both kernels (mixed) or one; how the prompt kernel does; 8-row tiles of single tokens
+struct AdPlan { bool mixed; AdKind prompts; int nt; };
+static AdPlan ad_plan(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group, int window) {
+    if (ad_mixed(c, s, group, window)) return {true, ad_split(c, s, group) ? AD_PROMPTS_SPLIT : AD_PROMPTS, group > 8 ? 2 : 1};
+    return {false, ad_kind(c, s, group, window), ad_nt(s, group)};
+}
+
 static int ad_teams(int D, int NT) { return sm_count() * ((D * NT <= 128 ? 12 : 8) / AD_WARPS); }
 
 template <int D, int BS, int NT, typename T>
@@ -936,20 +943,24 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.wide = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(workspace) + ad_tokens_ws(cache, seqs, group));
     a.wide_n = a.redo = 0;
     cudaStream_t st = (cudaStream_t)stream;
-    int nt = ad_nt(seqs, group);
-    if (ad_mixed(cache, seqs, group, window)) {
-        nt = group > 8 ? 2 : 1;
-        a.rows_lo = ad_few_rows(cache->head_dim);
-        rc = ad_prompt(a, cache, ad_split(cache, seqs, group), st);
-        if (rc != MPSBNB_OK && rc != MPSBNB_ERR_UNSUPPORTED) return rc;
+    const AdPlan plan = ad_plan(cache, seqs, group, window);
+    if (plan.prompts != AD_TOKENS) {
+        if (plan.mixed) a.rows_lo = ad_few_rows(cache->head_dim);
+        rc = ad_prompt(a, cache, plan.prompts == AD_PROMPTS_SPLIT, st);
+        if (rc != MPSBNB_ERR_UNSUPPORTED && (rc != MPSBNB_OK || !plan.mixed)) return rc;
         if (rc == MPSBNB_OK) a.rows_hi = a.rows_lo;                  // (else nothing has been launched: the kernel here takes all)
         a.rows_lo = 0;
-    } else {
-        const AdKind kind = ad_kind(cache, seqs, group, window);
-        if (kind != AD_TOKENS) {
-            rc = ad_prompt(a, cache, kind == AD_PROMPTS_SPLIT, st);
-            if (rc != MPSBNB_ERR_UNSUPPORTED) return rc;
-        }
     }
-    return ad_run(a, cache, nt, st);
+    return ad_run(a, cache, plan.nt, st);
+}
+
+extern "C" int mpsbnb_attention_4bit_kernels(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads, int window) {
+    int rc = kv4_check_cache(cache, 0);
+    if (rc == MPSBNB_OK) rc = kv4_check_seqs(seqs, cache);
+    if (rc != MPSBNB_OK) return rc;
+    if (heads <= 0 || heads % cache->kv_heads != 0 || window < 0) return MPSBNB_ERR_INVALID_ARG;
+    if (seqs->batch == 0 || seqs->tokens == 0) return 0;
+    const AdPlan plan = ad_plan(cache, seqs, heads / cache->kv_heads, window);
+    return (plan.mixed || plan.prompts == AD_TOKENS ? MPSBNB_ATTENTION_TOKENS : 0) | (plan.prompts != AD_TOKENS ? MPSBNB_ATTENTION_PROMPTS : 0) |
+           (plan.prompts == AD_PROMPTS_SPLIT ? MPSBNB_ATTENTION_SHARED_OUT : 0);
 }

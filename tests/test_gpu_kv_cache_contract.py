@@ -78,3 +78,37 @@ def test_append_stores_every_row_whatever_the_longest_is_said_to_be():
         sq = N.Kv4Seqs(table.data_ptr(), 2, lens.data_ptr(), starts.data_ptr(), 20, 2, 2, longest)
         assert N.lib().mpsbnb_kv4_append(cache._ref, 0, sq, k.data_ptr(), 128, 64, v.data_ptr(), 128, 64, torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(cache.data, other.data) and cache.data.any()
+
+
+def test_the_attention_tests_reach_all_kernels():
+    """By the library's own choice, over the cases of the attention test (with the table's own width and widened)."""
+    from test_gpu_kv_cache import CASES
+    kinds = set()
+    for head_dim, blocksize, page, _, dtype, heads, kv_heads, new, lens, _, window in CASES:
+        cache = bnb.KVCache4bit(1, 1, kv_heads, head_dim, page, blocksize, dtype=dtype)
+        for width in (max(-(-max(lens) // page), 1), (1 << 17) // page):
+            sq = N.Kv4Seqs(1 << 21, width, 1 << 22, 1 << 23, sum(new), width, len(new), max(new))
+            kinds.add((N.lib().mpsbnb_attention_4bit_kernels(cache._ref, sq, heads, window or 0), head_dim, blocksize))
+    assert kinds >= {(k, d, b) for k in (1, 2, 6) for d in (64, 128, 256) for b in (32, 64)}
+    assert {(3, d) for d in (64, 128)} <= {(k, d) for k, d, _ in kinds}   # single tokens and prompts in a call; the others below
+
+
+@pytest.mark.parametrize("head_dim,blocksize,dtype,window,heads,kv_heads,kinds", [
+    (64, 64, F16, None, 8, 2, 7), (128, 64, BF16, None, 8, 2, 7), (128, 32, F16, 150, 8, 2, 7), (256, 64, F16, None, 4, 1, 7), (256, 32, BF16, None, 32, 8, 3)])
+def test_prompts_among_single_tokens(head_dim, blocksize, dtype, window, heads, kv_heads, kinds):
+    import kv_util as U
+    new, lens = [1, 2, 1, 400, 1, 1, 0, 5], [30, 500, 1, 555, 90, 257, 9, 5]
+    cache = U.make_cache(8 * 18, kv_heads, head_dim, 32, blocksize, dtype=dtype, seed=5)
+    table = U.widen(U.random_table(8, 18, 8 * 18), 32)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    sq = N.Kv4Seqs(1 << 21, table.shape[1], 1 << 22, 1 << 23, sum(new), table.shape[1], 8, 400)
+    assert N.lib().mpsbnb_attention_4bit_kernels(cache._ref, sq, heads, 0) == kinds
+    q = torch.randn(starts[-1], heads, head_dim, device="cuda").to(dtype)
+    want, want_lse, bound = U.attention(q, cache, 0, table, lens, starts, window=window)
+    got, lse = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), 400, window=window, return_lse=True)
+    U.check(got, want, bound, dtype)
+    assert ((lse.double() - want_lse).abs() <= 2.0 ** -11 * 16 + 2.0 ** -20 * want_lse.abs()).all()
+    assert torch.equal(got, bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), 400, window=window))
+    assert_device_ok()
