@@ -772,8 +772,15 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
 // ------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------
+// The longest sequence's new tokens, for the choices below: what the caller says, but no more than is left when every other has one.
+// (A caller that does not know says the number of all rows; single tokens are still seen for what they are.)
+static int64_t ad_longest(const mpsbnb_kv4_seqs *s) {
+    if (s->cu_seqlens == nullptr) return s->new_tokens;
+    const int64_t most = s->tokens - (s->batch - 1) > 1 ? s->tokens - (s->batch - 1) : 1;
+    return s->new_tokens < most ? s->new_tokens : most;
+}
 // 16 rows per tile where 8 do not hold a sequence's rows: the keys are then expanded half as often
-static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return (int64_t)s->new_tokens * group > 8 ? 2 : 1; }
+static int ad_nt(const mpsbnb_kv4_seqs *s, int group) { return ad_longest(s) * group > 8 ? 2 : 1; }
 
 // The tensor-core kernel of attn4_prompt.cu instead?  A key tile costs it the same whether its rows are 16 or 256: 2.0, 2.4, 3.3 us
 // per 128 keys and block of rows on an SM (head_dim 64, 128, 256).  The kernel here spreads any amount of work over the whole card,
@@ -788,7 +795,7 @@ enum AdKind { AD_TOKENS, AD_PROMPTS, AD_PROMPTS_SPLIT };
 static bool ad_split(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group) {
     const int64_t block = c->head_dim == 256 ? 128 : 256;
     // (every block of the card looks through the (sequence, block of rows) pairs, 32 at a time)
-    return (int64_t)s->batch * c->kv_heads * (((int64_t)s->new_tokens * group + block - 1) / block) <= AD_SPLIT * (int64_t)sm_count();
+    return (int64_t)s->batch * c->kv_heads * ((ad_longest(s) * group + block - 1) / block) <= AD_SPLIT * (int64_t)sm_count();
 }
 static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group, int window) {
     const int64_t rows = (s->tokens * group + s->batch - 1) / s->batch;   // of a sequence and head, on average
@@ -796,7 +803,7 @@ static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int g
     const int64_t blocks = lists * ((rows + block - 1) / block), tiles = lists * ((rows + 15) / 16);
     const bool split = ad_split(c, s, group);
     double keys = (double)s->table_width * c->page_size;
-    if (window > 0 && keys > (double)window + s->new_tokens) keys = (double)window + s->new_tokens;
+    if (window > 0 && keys > (double)window + ad_longest(s)) keys = (double)window + ad_longest(s);
     const int at = c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2;
     const double meet[3] = {4.7, 2.9, 1.5}, sooner[3] = {570e3, 450e3, 50e3};
     if (rows <= 16 || keys * (tiles - meet[at] * (split ? blocks : (blocks + sms - 1) / sms * sms)) <= sooner[at]) return AD_TOKENS;
@@ -807,9 +814,9 @@ static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int g
 // four times the average's rows and alone would go to the prompt kernel.  (256 sequences over 4096 keys, one with 2048 new tokens, 32
 // heads on 8: 459 us; by the prompt kernel alone 1170, as two calls 156 and 276.)
 static bool ad_mixed(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group, int window) {
-    if (s->cu_seqlens == nullptr || 4 * s->tokens > (int64_t)s->batch * s->new_tokens) return false;
+    if (s->cu_seqlens == nullptr || 4 * s->tokens > (int64_t)s->batch * ad_longest(s)) return false;
     mpsbnb_kv4_seqs one = *s;
-    one.batch = 1; one.tokens = s->new_tokens;
+    one.batch = 1; one.new_tokens = (int)ad_longest(s); one.tokens = one.new_tokens;
     return ad_kind(c, &one, group, window) != AD_TOKENS;
 }
 // rows a head up to which a sequence of a mixed call counts as single tokens: where the kernels' times per key meet

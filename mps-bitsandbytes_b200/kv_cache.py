@@ -360,7 +360,8 @@ def attention_4bit(q: Tensor, cache: KVCache4bit, layer: int, page_table: Tensor
     ``q``: [tokens, heads, head_dim] or [batch, new, heads, head_dim] in the cache's dtype, the queries of each sequence's
     LAST tokens (the tokens that ``append_kv_4bit`` has just stored, one per sequence when decoding); ``page_table``,
     ``seq_lens`` and ``cu_seqlens`` as there, ``max_seqlen`` the largest number of rows of a sequence: with ``cu_seqlens`` the
-    choice of kernels goes by it, not the result.
+    choice of kernels goes by it, not the result.  Without it a call of prompts may launch the kernel for single tokens too,
+    which then finds nothing to do.
     heads / kv heads consecutive heads share a key/value head.  The query at place p sees the keys up to p - with ``window``
     only the last ``window`` of them - or all of its sequence when not ``causal``.  ``scale`` defaults to head_dim ** -0.5.
 

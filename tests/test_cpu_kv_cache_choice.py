@@ -29,3 +29,20 @@ def kernels(heads, kv_heads, new, places, head_dim=128, longest=None, window=0, 
     (-1, dict(heads=9, kv_heads=8, new=[1], places=64)), (-1, dict(heads=8, kv_heads=8, new=[1], places=64, window=-1))])
 def test_kernels_of_a_call(want, args):
     assert kernels(**args) == want
+
+
+@pytest.mark.parametrize("heads,kv_heads,batch,places", [(64, 8, 64, 16384), (64, 8, 32, 4096), (32, 8, 200, 2048), (8, 1, 512, 65536)])
+def test_single_tokens_are_seen_for_what_they_are_without_the_longest(heads, kv_heads, batch, places):
+    told = dict(heads=heads, kv_heads=kv_heads, new=[1] * batch, places=places)
+    assert kernels(**told) == kernels(**told, longest=batch) == TOKENS
+
+    def workspace(longest):
+        cache = N.Kv4Cache(1 << 20, 1 << 16, 1, kv_heads, 128, 64, 64, 0, 0)
+        seqs = N.Kv4Seqs(1 << 21, places // 64, 1 << 22, 1 << 23, batch, places // 64, batch, longest)
+        return N.lib().mpsbnb_attention_4bit_workspace_bytes(C.byref(cache), C.byref(seqs), heads)
+    assert workspace(batch) == workspace(1)                          # (the tiles are as wide, too)
+
+
+def test_prompts_without_the_longest_go_where_prompts_go():
+    for new in ([700, 300], [2048] * 8, [1] * 30 + [900]):
+        assert kernels(32, 8, new, 4096, longest=sum(new)) & PROMPTS
