@@ -446,7 +446,7 @@ typedef struct mpsbnb_kv4_cache {
     int num_layers, kv_heads, head_dim, page_size, blocksize, quant_type, dtype;
 } mpsbnb_kv4_cache;
 
-/* The sequences of a call.  Sequence b holds seq_lens[b] tokens (the call's new ones included; clamped to what its
+/* The sequences of a call.  Sequence b holds seq_lens[b] tokens (the call's new ones included; reading cuts it to what its
  * row of the page table can hold) in the pages page_table[b * table_ld + 0 ...].  Its new tokens are rows
  * cu_seqlens[b] ... cu_seqlens[b + 1] - 1 of the call's [tokens, ...] tensors, or rows b * new_tokens ... with
  * cu_seqlens NULL; they take the last places of the sequence.  With cu_seqlens, new_tokens is the largest number of new
@@ -467,7 +467,8 @@ size_t mpsbnb_kv4_cache_bytes(const mpsbnb_kv4_cache *cache);
 /* Quantises the new tokens' rows into their places.  k, v: [tokens, kv_heads, head_dim] in the cache's dtype with
  * strides (in elements) between tokens and heads, head_dim contiguous.  Rows past cu_seqlens[batch], and tokens
  * whose place is negative (a sequence shorter than its new tokens), are skipped; so are tokens whose page number is
- * outside the cache, which raise device status 401.  Pages that are written belong to one sequence only. */
+ * outside the cache, which raise device status 401, and tokens whose place the page table has no room for (a length
+ * beyond it is not cut here), which raise 430.  Pages that are written belong to one sequence only. */
 int mpsbnb_kv4_append(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *k,
                       int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
                       int64_t v_head_stride, void *stream);

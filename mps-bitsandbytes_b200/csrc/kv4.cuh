@@ -7,6 +7,7 @@ namespace mpsbnb {
 
 constexpr int KV4_GROUP = 16;                    // tokens per group: the unit a kernel fetches
 constexpr int KV4_BAD_PAGE = 401;                // device status: a page number outside the cache
+constexpr int KV4_NO_ROOM = 430;                 // ... a new token's place behind what the page table can hold
 
 // 16 tokens of one head: K codes, K absmax, V codes, V absmax
 __host__ __device__ constexpr int kv4_half_bytes(int head_dim, int blocksize) {

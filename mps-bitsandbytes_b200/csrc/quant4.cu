@@ -403,8 +403,12 @@ kv4_append_kernel(const Kv4Layer kv, const Kv4Seqs sq, const T *__restrict__ k, 
         }
         sq.get(b, row, n, len);
         const int i = t - row;
-        place = len - n + i;
+        place = max(__ldg(sq.lens + b), 0) - n + i;                // (not by the length cut to the table: other tokens are there)
         if (i < 0 || i >= n || place < 0) return -1;
+        if (place >= sq.capacity) {
+            if (lane == 0) atomicExch(&g_kv4_append_status, KV4_NO_ROOM);
+            return -1;
+        }
         const int page = __ldg(sq.table + (int64_t)b * sq.table_ld + (place >> kv.page_shift));
         if (page >= 0 && page < kv.num_pages) return page;
         if (lane == 0) atomicExch(&g_kv4_append_status, KV4_BAD_PAGE);

@@ -321,8 +321,8 @@ def append_kv_4bit(cache: KVCache4bit, layer: int, k: Tensor, v: Tensor, page_ta
     ``k``, ``v``: [tokens, kv heads, head_dim] (or [batch, new, kv heads, head_dim]) in the cache's dtype, any strides.
     ``page_table`` int32 [batch, pages] and ``seq_lens`` int32 [batch], the lengths WITH the new tokens; sequence b's
     rows are ``cu_seqlens[b]`` .. ``cu_seqlens[b + 1]`` (int32 [batch + 1]), or an equal share of all without it.  Rows
-    past ``cu_seqlens[-1]`` and tokens whose place would be negative are skipped.  The codes are those of
-    ``quantize_4bit``.  A page that is written must belong to one sequence only (``KVCache4bit.extend`` sees to it).
+    past ``cu_seqlens[-1]`` and tokens whose place would be negative, or behind what the page table can hold, are skipped.  The
+    codes are those of ``quantize_4bit``.  A page that is written must belong to one sequence only (``KVCache4bit.extend`` sees to it).
     """
     _check_cache(cache, layer, "append_kv_4bit")
     kr, tokens, _, k_token, k_head = _rows("k", k, cache.num_kv_heads, cache)

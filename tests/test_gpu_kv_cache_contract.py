@@ -112,3 +112,28 @@ def test_prompts_among_single_tokens(head_dim, blocksize, dtype, window, heads, 
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -11 * 16 + 2.0 ** -20 * want_lse.abs()).all()
     assert torch.equal(got, bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), 400, window=window))
     assert_device_ok()
+
+
+@pytest.mark.parametrize("new,length", [(10, 40), (10, 2 ** 31 - 1), (3, 33), (32, 64), (40, 40)])
+def test_append_leaves_the_tokens_alone_that_are_there_when_the_table_has_no_room(new, length):
+    cache = bnb.KVCache4bit(1, 4, 2, 64, page_size=16)
+    table = _i32([[3, 1], [0, 2]])
+    old = torch.randn(2, 32, 2, 64, device="cuda", dtype=F16)
+    bnb.append_kv_4bit(cache, 0, old, old * 2, table, _i32([32, 32]))
+    kept = bnb.dequantize_kv_4bit(cache, 0, table, _i32([32, 32]))
+    assert_device_ok()
+    k = torch.randn(2, new, 2, 64, device="cuda", dtype=F16)
+    bnb.append_kv_4bit(cache, 0, k, k * 3, table, _i32([length, 32]))
+    assert _status() == 430
+    got = bnb.dequantize_kv_4bit(cache, 0, table, _i32([32, 32]))
+    first = length - new                                             # the first new token's place
+    for x, was, now in zip((k, k * 3), kept, got):
+        room = max(0, 32 - first)
+        assert torch.equal(now[0, :min(first, 32)], was[0, :min(first, 32)])
+        if room:
+            want = bnb.dequantize_4bit(*bnb.quantize_4bit(x[0, :room].reshape(-1, 64))).view(room, 2, 64)
+            assert torch.equal(now[0, first:], want)
+    own = min(new, 32)
+    want = bnb.dequantize_4bit(*bnb.quantize_4bit(k[1, new - own:].reshape(-1, 64))).view(own, 2, 64)
+    assert torch.equal(got[0][1, 32 - own:], want)
+    assert_device_ok()
