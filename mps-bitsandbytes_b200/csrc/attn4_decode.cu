@@ -942,7 +942,7 @@ extern "C" int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, c
     a.sq = kv4_seqs(seqs, cache);
     a.q = q; a.q_ts = q_token_stride; a.q_hs = q_head_stride;
     a.out = out; a.lse = lse; a.ws = (float *)workspace;
-    a.heads = heads; a.group = group; a.causal = causal != 0; a.window = window; a.quant_type = cache->quant_type;
+    a.heads = heads; a.group = group; a.causal = causal != 0; a.window = window < (1 << 30) ? window : 1 << 30; a.quant_type = cache->quant_type;
     a.scale_log2 = scale * 1.4426950408889634f;
     static const float codes[2][16] = {MPSBNB_NF4_TABLE, MPSBNB_FP4_TABLE};
     for (int i = 0; i < 16; ++i) a.code[i] = codes[cache->quant_type][i] * attn4_code_scale(cache->quant_type);

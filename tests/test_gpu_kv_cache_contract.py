@@ -137,3 +137,22 @@ def test_append_leaves_the_tokens_alone_that_are_there_when_the_table_has_no_roo
     want = bnb.dequantize_4bit(*bnb.quantize_4bit(k[1, new - own:].reshape(-1, 64))).view(own, 2, 64)
     assert torch.equal(got[0][1, 32 - own:], want)
     assert_device_ok()
+
+
+@pytest.mark.parametrize("heads,kv_heads,new,length", [(8, 2, 10, 5), (32, 8, 300, 200), (32, 8, 300, 300)])
+def test_the_largest_window_is_none(heads, kv_heads, new, length):
+    """By the C entry point, for a sequence that is shorter than its new tokens too: places are negative there."""
+    import kv_util as U
+    cache = U.make_cache(10, kv_heads, 128, 32, seed=6)
+    table = U.widen(U.random_table(1, 10, 10), 32)
+    q = torch.randn(new, heads, 128, device="cuda", dtype=F16)
+    lens = _i32([length])
+    want = bnb.attention_4bit(q[None], cache, 0, table, lens)[0]
+    sq = N.Kv4Seqs(table.data_ptr(), table.shape[1], lens.data_ptr(), None, new, table.shape[1], 1, new)
+    nbytes = N.lib().mpsbnb_attention_4bit_workspace_bytes(cache._ref, sq, heads)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    for window in (1 << 30, (1 << 31) - 1):
+        got = torch.full_like(q, 7.0)
+        assert N.lib().mpsbnb_attention_4bit(cache._ref, 0, sq, q.data_ptr(), heads * 128, 128, heads, 1, window, 128 ** -0.5, got.data_ptr(), None,
+                                             ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(got, want) and want.any()
