@@ -69,7 +69,7 @@ class _PageBook:
     def extend(self, ids: Sequence[int], counts: Union[int, Sequence[int]]) -> None:
         """Makes room for ``counts`` more tokens in each sequence and raises its length.  A page that the new tokens
         share with another sequence is copied first (one launch for all sequences and layers, on the current stream).
-        Raises RuntimeError, with nothing changed, if the pages do not suffice."""
+        Raises RuntimeError if the pages do not suffice; nothing has changed after an error, that of a copy included."""
         ids = list(ids)
         counts = [counts] * len(ids) if isinstance(counts, int) else list(counts)
         if len(counts) != len(ids):
@@ -93,23 +93,29 @@ class _PageBook:
             plan.append((pages, fresh, copy))
         if need > len(self._free):
             raise RuntimeError(f"the cache is out of pages: {need} needed, {len(self._free)} free")
-        src, dst = [], []
+        taken = [heapq.heappop(self._free) for _ in range(need)]
+        src, dst, at = [], [], 0
         for pages, fresh, copy in plan:
             if copy:
-                page = heapq.heappop(self._free)
                 src.append(pages[-1])
-                dst.append(page)
-                self._users[pages[-1]] -= 1
-                self._users[page] = 1
-                pages[-1] = page
-            for _ in range(fresh):
-                page = heapq.heappop(self._free)
-                self._users[page] = 1
-                pages.append(page)
-        for seq_id, count in zip(ids, counts):
-            self._seqs[seq_id][1] += count
+                dst.append(taken[at])
+            at += fresh + copy
         if src:
-            self._copy_pages(src, dst)
+            try:
+                self._copy_pages(src, dst)
+            except BaseException:
+                for page in taken:
+                    heapq.heappush(self._free, page)
+                raise
+        at = 0
+        for (pages, fresh, copy), seq_id, count in zip(plan, ids, counts):
+            if copy:
+                self._users[pages.pop()] -= 1
+            pages += taken[at:at + fresh + copy]
+            at += fresh + copy
+            self._seqs[seq_id][1] += count
+        for page in taken:
+            self._users[page] = 1
 
     def fork(self, seq_id: int) -> int:
         """A sequence with the same tokens, sharing all pages; returns its number."""
