@@ -171,7 +171,7 @@ class KVCache4bit(_PageBook):
 
     ``data`` is uint8 [layers, pages, kv heads, page_size / 16, group bytes]; ``k_codes`` / ``v_codes`` (uint8 [..., 16,
     head_dim / 2], low nibble = even element) and ``k_absmax`` / ``v_absmax`` (``dtype`` [..., 16, head_dim /
-    blocksize]) are views of it.
+    blocksize]) are views of it.  Another tensor of its shape may be assigned to it.
 
     The book: ``new_sequence``, ``extend``, ``fork``, ``truncate``, ``free``, ``compact`` and ``batch``.  Forked
     sequences share their pages; a shared page is copied when one of them is about to write to it.  Pages are handed out
@@ -202,16 +202,33 @@ class KVCache4bit(_PageBook):
         super().__init__(num_pages, page_size)
         self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
         self.blocksize, self.quant_type, self.dtype, self.device = blocksize, quant_type, dtype, device
-        nb = head_dim // blocksize
-        codes, half = _GROUP * head_dim // 2, _GROUP * (head_dim // 2 + 2 * nb)
-        self.data = torch.zeros(num_layers, num_pages, num_kv_heads, page_size // _GROUP, 2 * half, dtype=torch.uint8, device=device)
-        self.k_codes = self.data[..., :codes].unflatten(-1, (_GROUP, head_dim // 2))
-        self.k_absmax = self.data[..., codes:half].view(dtype).unflatten(-1, (_GROUP, nb))
-        self.v_codes = self.data[..., half:half + codes].unflatten(-1, (_GROUP, head_dim // 2))
-        self.v_absmax = self.data[..., half + codes:].view(dtype).unflatten(-1, (_GROUP, nb))
-        self._desc = N.Kv4Cache(self.data.data_ptr(), num_pages, num_layers, num_kv_heads, head_dim, page_size, blocksize,
-                                N.qt(quant_type), N.dt(dtype))
+        self._desc = N.Kv4Cache(None, num_pages, num_layers, num_kv_heads, head_dim, page_size, blocksize, N.qt(quant_type), N.dt(dtype))
         self._ref, self._index = C.byref(self._desc), device.index
+        half = _GROUP * (head_dim // 2 + 2 * (head_dim // blocksize))
+        self._bind(torch.zeros(num_layers, num_pages, num_kv_heads, page_size // _GROUP, 2 * half, dtype=torch.uint8, device=device))
+
+    def _bind(self, data: Tensor) -> None:
+        """The storage, its views and the address that the kernels get."""
+        nb = self.head_dim // self.blocksize
+        codes, half = _GROUP * self.head_dim // 2, data.shape[-1] // 2
+        self._data = data
+        self.k_codes = data[..., :codes].unflatten(-1, (_GROUP, self.head_dim // 2))
+        self.k_absmax = data[..., codes:half].view(self.dtype).unflatten(-1, (_GROUP, nb))
+        self.v_codes = data[..., half:half + codes].unflatten(-1, (_GROUP, self.head_dim // 2))
+        self.v_absmax = data[..., half + codes:].view(self.dtype).unflatten(-1, (_GROUP, nb))
+        self._desc.data = data.data_ptr()
+
+    @property
+    def data(self) -> Tensor:
+        return self._data
+
+    @data.setter
+    def data(self, value: Tensor) -> None:
+        old = self._data
+        if (not isinstance(value, Tensor) or value.shape != old.shape or value.dtype != old.dtype or value.device != old.device
+                or not value.is_contiguous() or value.data_ptr() & 15):
+            raise ValueError(f"data must be a contiguous uint8 tensor of shape {tuple(old.shape)} on {old.device}, 16-byte aligned")
+        self._bind(value)
 
     def _copy_pages(self, src: List[int], dst: List[int]) -> None:
         copy_kv_pages_4bit(self, src, dst)
