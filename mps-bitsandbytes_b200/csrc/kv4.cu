@@ -37,7 +37,7 @@ kv4_dequantize_kernel(const Kv4Layer kv, const Kv4Seqs sq, int quant_type, int c
     for (int i = threadIdx.x; i < 512; i += 256) room[(tab - at) / 4 + i] = kCode[quant_type][i >> 5];
     __syncthreads();
     const int lane = threadIdx.x & 31;
-    const uint32_t tab_lane = tab + lane * 4u;
+    const uint32_t tab_lane = kv4_after_barrier(tab + lane * 4u);
     // a row is cpr chunks of 8 elements (8, 16 or 32 lanes); the warp goes on by `step` heads: 256 elements
     const int cpr = 1 << cpr_shift, step = 32 >> cpr_shift, kc = lane & (cpr - 1), rl = lane >> cpr_shift;
     const int64_t head_bytes = (int64_t)(1 << (kv.page_shift - 4)) * kv.group_bytes;

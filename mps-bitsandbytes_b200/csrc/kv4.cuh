@@ -60,6 +60,13 @@ struct Kv4Seqs {
     }
 };
 
+// A table's address that is known behind the barrier only: look-ups by it, which tell the compiler of no memory, stay there.
+__device__ __forceinline__ uint32_t kv4_after_barrier(uint32_t address) {
+    uint32_t same;
+    asm volatile("mov.b32 %0, %1;" : "=r"(same) : "r"(address) : "memory");
+    return same;
+}
+
 inline int kv4_check_cache(const mpsbnb_kv4_cache *c, int layer) {
     if (c == nullptr || c->data == nullptr || !aligned16(c->data)) return MPSBNB_ERR_INVALID_ARG;
     if (layer < 0 || layer >= c->num_layers || c->num_pages <= 0 || c->kv_heads <= 0) return MPSBNB_ERR_INVALID_ARG;

@@ -383,7 +383,7 @@ kv4_append_kernel(const Kv4Layer kv, const Kv4Seqs sq, const T *__restrict__ k, 
     kv4_bucket_fill<QT>(table, threadIdx.x, 256);
     __syncthreads();
     const int lane = threadIdx.x & 31;
-    const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(table) + (uint32_t)lane * 16u;
+    const uint32_t tab_lane = kv4_after_barrier((uint32_t)__cvta_generic_to_shared(table) + (uint32_t)lane * 16u);
     // a row is cpr chunks of 8 elements (8, 16 or 32 lanes); the warp goes on by `step` heads
     const int cpr = 1 << cpr_shift, half_dim = cpr * 4, step = 32 >> cpr_shift, kc = lane & (cpr - 1), rl = lane >> cpr_shift;
     const int64_t head_bytes = (int64_t)(1 << (kv.page_shift - 4)) * kv.group_bytes;
