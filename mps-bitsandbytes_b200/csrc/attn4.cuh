@@ -32,6 +32,8 @@ struct Attn4Args {
 __host__ __device__ inline float attn4_code_scale(int quant_type) { return quant_type == MPSBNB_NF4 ? ATTN4_NF4_SCALE : 1.0f; }
 __device__ __forceinline__ float attn4_code_unscale(int quant_type) { return quant_type == MPSBNB_NF4 ? 1.0f / ATTN4_NF4_SCALE : 1.0f; }
 
+// Sums of probability * value are joined times this: 2^16 values of the type's largest under weights of up to 2^8 stay finite.
+constexpr float ATTN4_SUM = 0x1p-24f;
 constexpr float ATTN4_NONE = -0x1p127f;          // running maximum before any key has been seen
 // From this reference on, the fused score * factor - reference is no longer the difference of two rounded products: for scores of 1e10
 // it leaves up to 2^9 of the reference's rounding, where the largest must leave 0.
@@ -44,7 +46,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Runs of work end inside a (sequence, kv head, tile of RT rows): what a run (a team's or a block's) then leaves in the workspace.
-// Partial result of run c, slot s (0: its first piece, 1: its last): RT x D sums, then RT (reference, sum) pairs
+// Partial result of run c, slot s (0: its first piece, 1: its last): RT x D sums times ATTN4_SUM, then RT (reference, sum) pairs
 template <int D, int RT> __device__ __forceinline__ float *attn4_partial(float *ws, int64_t c, int s) {
     return ws + (c * 2 + s) * (RT * (D + 2));
 }
@@ -101,7 +103,7 @@ attn4_combine_kernel(const __grid_constant__ Attn4Args A, int runs) {
         L = 0.0f;
 #pragma unroll
         for (int w = 0; w < ATTN4_JOIN_WARPS; ++w) { k[w] = ex2(red[w][D] - M); L = fmaf(red[w][D + 1], k[w], L); }
-        const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
+        const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f / ATTN4_SUM, L);
         for (int d = threadIdx.x; d < D; d += ATTN4_JOIN_WARPS * 32) {
             float y = 0.0f;
 #pragma unroll
@@ -109,7 +111,7 @@ attn4_combine_kernel(const __grid_constant__ Attn4Args A, int runs) {
             out[d] = from_f32<T>(y * inv);
         }
     } else {
-        const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
+        const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f / ATTN4_SUM, L);
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) out[j * 32 + lane] = from_f32<T>(v[j] * inv);
     }

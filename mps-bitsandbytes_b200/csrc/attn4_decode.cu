@@ -714,7 +714,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                 float M = m[nt][j];
 #pragma unroll
                 for (int w = 0; w < AD_WARPS; ++w) M = fmaxf(M, stat[w * RT + nt * 8 + 2 * c + j].x);
-                const float k = ex2(m[nt][j] - M) * __frcp_rn(up) * attn4_code_unscale(A.quant_type);
+                const float k = ex2(m[nt][j] - M) * (__frcp_rn(up) * (attn4_code_unscale(A.quant_type) * ATTN4_SUM));
 #pragma unroll
                 for (int i = 0; i < MT; ++i) { o[i][nt][j] *= k; o[i][nt][j + 2] *= k; }
             }
@@ -753,7 +753,7 @@ attn4_decode_kernel(const __grid_constant__ Attn4Args A) {
                     L = fmaf(z.y, ex2(z.x - M), L);
                 }
                 if (whole) {
-                    const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
+                    const float inv = L == 0.0f ? 0.0f : __fdividef(1.0f / ATTN4_SUM, L);
                     const int64_t orow = (int64_t)(sq.row0 + i) * A.heads + cur.h * A.group + (R - i * A.group);
                     T pr[2] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv)};
                     *reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(A.out) + orow * D + d0 + d) = *reinterpret_cast<const uint32_t *>(pr);

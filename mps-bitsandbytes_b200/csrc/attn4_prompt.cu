@@ -919,7 +919,7 @@ attn4_prompt_kernel(const __grid_constant__ Attn4Args A, int split) {
             const float l = la + lb;
             // a partial result: sums as they are, and the reference
             const float up = w.nk > 0 ? __int_as_float(max(1, ve - 8) << 23) * attn4_code_unscale(A.quant_type) : 0.0f;
-            const float inv = l == 0.0f ? 0.0f : w.slot < 0 ? __fdividef(1.0f, l) * up : up;
+            const float inv = l == 0.0f ? 0.0f : w.slot < 0 ? __fdividef(1.0f, l) * up : up * ATTN4_SUM;
             // Four lanes take 32 channels (64 bytes) of a row, eight rows at a time: with 16 bytes of 32 rows each, stores kept the
             // load and store unit busy 4 times as long.  (The order that V's channels have in O makes a lane's eight neighbours.)
             float *const part = attn4_partial<D, TILES * 128>(A.ws, blockIdx.x, max(w.slot, 0));

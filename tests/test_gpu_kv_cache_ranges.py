@@ -272,3 +272,20 @@ def test_scores_of_any_size(head_dim, dtype, size, heads, kv_heads, new):
             want_lse = top[:, 0] + torch.log(total[:, 0])
             assert ((lse[starts[b]:starts[b + 1], h].double() - want_lse).abs() <= 2.0 ** -9 * want_lse.abs() + 1e-3).all()
     assert_device_ok()
+
+
+@pytest.mark.parametrize("heads,kv_heads,new", [(4, 2, [1, 3, 1])] + PROMPTS, ids=["tokens", "shared out", "whole", "mixed"])
+@pytest.mark.parametrize("before,size", [(20, 3e38), (2000, 3e38), (300, 1e33)])
+def test_values_up_to_the_types_largest(heads, kv_heads, new, before, size):
+    """Their sum over the keys leaves fp32, their mean does not."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+
+    def change(k, v, b):
+        k.mul_(0.1)
+        v.copy_(size * torch.where(v > 1.0, 0.5, 1.0) * torch.where(v > 1.5, -1.0, 1.0))
+    cache, table, lens, starts, q = _prompts(128, 64, BF16, heads, kv_heads, new, before, gen, change)
+    got = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), max(new))
+    for b, n in enumerate(new):
+        rows = slice(starts[b], starts[b + 1])
+        close(got[rows], *reference(q[rows], cache, 0, table[b], lens[b]))
+    assert_device_ok()
