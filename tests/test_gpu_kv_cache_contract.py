@@ -156,3 +156,71 @@ def test_the_largest_window_is_none(heads, kv_heads, new, length):
         assert N.lib().mpsbnb_attention_4bit(cache._ref, 0, sq, q.data_ptr(), heads * 128, 128, heads, 1, window, 128 ** -0.5, got.data_ptr(), None,
                                              ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(got, want) and want.any()
+
+
+#  tokens of each sequence; what of them is new
+LARGE = [([5200], [5200]), ([1700, 0, 900, 3001, 64, 1], [1700, 0, 333, 3001, 1, 1]), ([3, 1, 2], [3, 1, 1])]
+
+
+@pytest.mark.parametrize("lens,new", LARGE, ids=["one of many tokens", "ragged", "few"])
+@pytest.mark.parametrize("head_dim,blocksize,kv_heads,dtype,quant", [
+    (256, 64, 8, BF16, "nf4"), (256, 32, 5, F16, "fp4"), (128, 64, 11, F16, "nf4"), (64, 32, 17, BF16, "fp4"), (128, 32, 1, BF16, "nf4"), (64, 64, 3, F16, "nf4")])
+def test_append_and_read_back_of_many_tokens_and_many_heads(lens, new, head_dim, blocksize, kv_heads, dtype, quant):
+    """More tokens than there are warps, so that each goes on from one to the next, and more heads than a warp takes at a time; few
+    tokens, whose heads several warps share."""
+    width = max(-(-max(lens) // 64), 1)
+    cache = bnb.KVCache4bit(1, len(lens) * width, kv_heads, head_dim, 64, blocksize, quant, dtype)
+    table = torch.randperm(cache.num_pages, generator=torch.Generator().manual_seed(2)).to(torch.int32).view(len(lens), width).cuda()
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    k, v = (torch.randn(starts[-1], kv_heads, head_dim, device="cuda").to(dtype) for _ in range(2))
+    cache.data.random_(0, 128)
+    before = bnb.dequantize_kv_4bit(cache, 0, table, _i32(lens))
+    bnb.append_kv_4bit(cache, 0, k, v, table, _i32(lens), _i32(starts))
+    after = bnb.dequantize_kv_4bit(cache, 0, table, _i32(lens))
+    for x, was, now in zip((k, v), before, after):
+        want = bnb.dequantize_4bit(*bnb.quantize_4bit(x.reshape(-1, head_dim), blocksize=blocksize, quant_type=quant)).view(x.shape)
+        for b, (n, length) in enumerate(zip(new, lens)):
+            assert torch.equal(now[b, length - n:length], want[starts[b]:starts[b + 1]])
+            same = now[b, :length - n].view(torch.int16) == was[b, :length - n].view(torch.int16)
+            assert same.all() and (now[b, length:] == 0).all()
+    assert_device_ok()
+
+
+def test_read_back_of_more_places_than_there_are_warps():
+    import kv_util as U
+    lens = [9000, 0, 12345, 700]
+    cache = U.make_cache(4 * 200, 5, 256, 64, 64, "nf4", BF16, seed=8)
+    table = U.random_table(4, 200, 800)
+    k, v = bnb.dequantize_kv_4bit(cache, 0, table, _i32(lens), 12400)
+    for x, name in ((k, "k"), (v, "v")):
+        for b, length in enumerate(lens):
+            for a in range(0, length, 4000):
+                e = min(length, a + 4000)
+                assert torch.equal(x[b, a:e], U.rows_of(cache, 0, table[b], a, e, name).float().to(BF16))
+            assert (x[b, length:] == 0).all()
+
+
+@pytest.mark.parametrize("head_dim,kv_heads", [(128, 3), (64, 2), (256, 2)])
+def test_append_takes_rows_on_uneven_addresses_from_the_c_entry_point(head_dim, kv_heads):
+    """Python copies such rows first; the kernel takes them as they are: odd addresses, odd strides, heads between which others lie."""
+    tokens, token, head = 37, (kv_heads + 1) * (head_dim + 3) + 5, head_dim + 3
+    cache, other = (bnb.KVCache4bit(1, 3, kv_heads, head_dim, page_size=16) for _ in range(2))
+    flat = torch.randn(2 * tokens * token + 9, device="cuda", dtype=F16)
+    rows = [flat[at:].as_strided((tokens, kv_heads, head_dim), (token, head, 1)) for at in (1, 7 + tokens * token)]
+    table, lens = _i32([[2, 0, 1]]), _i32([40])
+    bnb.append_kv_4bit(other, 0, *(x.contiguous() for x in rows), table, lens)
+    sq = N.Kv4Seqs(table.data_ptr(), 3, lens.data_ptr(), None, tokens, 3, 1, tokens)
+    assert N.lib().mpsbnb_kv4_append(cache._ref, 0, sq, rows[0].data_ptr(), token, head, rows[1].data_ptr(), token, head, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(cache.data, other.data) and cache.data.any()
+    assert_device_ok()
+
+
+def test_an_output_that_is_not_contiguous_is_refused():
+    cache = bnb.KVCache4bit(1, 4, 2, 128)
+    q = torch.zeros(2, 3, 8, 128, device="cuda", dtype=F16)
+    for out in (torch.zeros(2, 8, 3, 128, device="cuda", dtype=F16).transpose(1, 2), torch.zeros(2, 3, 8, 136, device="cuda", dtype=F16)[..., :128],
+                torch.zeros(2 * 3 * 8 * 128 + 1, device="cuda", dtype=F16)[1:].view(q.shape)):
+        with pytest.raises(ValueError, match="out must be"):
+            bnb.attention_4bit(q, cache, 0, _i32([[0, 1], [2, 3]]), _i32([3, 4]), out=out)

@@ -289,3 +289,19 @@ def test_values_up_to_the_types_largest(heads, kv_heads, new, before, size):
         rows = slice(starts[b], starts[b + 1])
         close(got[rows], *reference(q[rows], cache, 0, table[b], lens[b]))
     assert_device_ok()
+
+
+def test_one_sequence_of_many_with_magnitudes_far_apart():
+    """Forty prompts, two of which have a value that the others do not: theirs are done again, whichever else are with them."""
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    new = [40 + 7 * (b % 9) for b in range(40)]
+
+    def change(k, v, b):
+        if b in (2, 35):
+            v[-20] *= 1e12
+    cache, table, lens, starts, q = _prompts(64, 64, BF16, 16, 4, new, 5, gen, change)
+    got = bnb.attention_4bit(q, cache, 0, table, _i32(lens), _i32(starts), max(new))
+    for b, n in enumerate(new):
+        rows = slice(starts[b], starts[b + 1])
+        close(got[rows], *reference(q[rows], cache, 0, table[b], lens[b]))
+    assert_device_ok()
