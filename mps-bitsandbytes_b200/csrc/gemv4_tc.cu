@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) mpsbnb_decode4_tmem_kernel(cons
                 const TcPiece pc = piece_of(p);
                 const CUtensorMap *map = &lin_of(pc.lin)->map;
                 for (int s = pc.s_begin; s < pc.s_end; ++s) {
-                    if (!mbar_wait_sleep(empty_bar(slot), ph ^ 1u, abort_flag, kSleepSlow)) { atomicExch(&g_tc_status, 401); *abort_flag = 1; ok = false; break; }
+                    if (!mbar_wait_sleep(empty_bar(slot), ph ^ 1u, abort_flag, kSleepSlow)) { atomicExch(&g_tc_status, 451); *abort_flag = 1; ok = false; break; }
                     mbar_arrive_expect_tx(full_bar(slot), TG_W_BYTES);
                     tma_load_2d(sm.addr(slot), map, full_bar(slot), s * 128, pc.row0);
                     if (++slot == nslots) { slot = 0; ph ^= 1u; }
@@ -257,11 +257,11 @@ __global__ void __launch_bounds__(TG_THREADS, 1) mpsbnb_decode4_tmem_kernel(cons
             for (int p = p_first; p < p_last && ok && !*abort_flag; p += p_step, ++dcount) {
                 const TcPiece pc = piece_of(p);
                 const int d = dcount & 1;
-                if (!mbar_wait_sleep(dempty_bar(d), (((uint32_t)dcount >> 1) & 1u) ^ 1u, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 402); *abort_flag = 1; break; }
+                if (!mbar_wait_sleep(dempty_bar(d), (((uint32_t)dcount >> 1) & 1u) ^ 1u, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 452); *abort_flag = 1; break; }
                 const uint32_t tmem_d = tmem_base + TG_D_COL0 + D_STRIDE * (uint32_t)d;
                 for (int s = pc.s_begin; s < pc.s_end; ++s) {
-                    if (!mbar_wait_sleep(xfull_bar(xslot), xph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 403); *abort_flag = 1; ok = false; break; }
-                    if (!mbar_wait_sleep(afull_bar(abuf), aph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 404); *abort_flag = 1; ok = false; break; }
+                    if (!mbar_wait_sleep(xfull_bar(xslot), xph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 453); *abort_flag = 1; ok = false; break; }
+                    if (!mbar_wait_sleep(afull_bar(abuf), aph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 454); *abort_flag = 1; ok = false; break; }
                     tc_fence_after();
                     fence_proxy_async_smem();                            // the x tile was written through the generic proxy
                     const uint64_t xdesc = umma_desc_k_sw128(s_xs + (uint32_t)(xslot * XS_BYTES));
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) mpsbnb_decode4_tmem_kernel(cons
             float *acc = L->acc, *ws = L->ws;
             void *y = L->y;
             const int d = dcount & 1;
-            if (!mbar_wait_sleep(dfull_bar(d), ((uint32_t)dcount >> 1) & 1u, abort_flag, kSleepSlow)) { atomicExch(&g_tc_status, 405); *abort_flag = 1; break; }
+            if (!mbar_wait_sleep(dfull_bar(d), ((uint32_t)dcount >> 1) & 1u, abort_flag, kSleepSlow)) { atomicExch(&g_tc_status, 455); *abort_flag = 1; break; }
             tc_fence_after();
             float v[NB];
 #pragma unroll
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) mpsbnb_decode4_tmem_kernel(cons
             float nxt[16];
             more = advance_to_mine();
             if (more && !L->scale_async) read_scales(L, pc.row0, s, nxt);
-            if (!mbar_wait_sleep(xempty_bar(my_x), my_ph ^ 1u, abort_flag, kSleepSlow)) { atomicExch(&g_tc_status, 406); *abort_flag = 1; break; }
+            if (!mbar_wait_sleep(xempty_bar(my_x), my_ph ^ 1u, abort_flag, kSleepSlow)) { atomicExch(&g_tc_status, 456); *abort_flag = 1; break; }
             const uint32_t xb = s_xs + (uint32_t)(my_x * XS_BYTES);
             const uint32_t ab = xb + X_BYTES;
             if (my_async) {
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) mpsbnb_decode4_tmem_kernel(cons
         for (int p = p_first; p < p_last; p += p_step) { const TcPiece pc = piece_of(p); total += pc.s_end - pc.s_begin; }
         for (int q = g; q < total && ok && !*abort_flag; q += TG_EGROUPS) {
             // the stage's packed bytes: this lane's 64 bytes, then the slot is free for the producer
-            if (!mbar_wait_sleep(full_bar(slot), ph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 407); *abort_flag = 1; ok = false; break; }
+            if (!mbar_wait_sleep(full_bar(slot), ph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 457); *abort_flag = 1; ok = false; break; }
             const uint32_t sb = sm.addr(slot);
             uint4 w4[4];
 #pragma unroll
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) mpsbnb_decode4_tmem_kernel(cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty_bar(slot) + dep);
             }
-            if (!mbar_wait_sleep(xfull_bar(xslot), xph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 408); *abort_flag = 1; ok = false; break; }
+            if (!mbar_wait_sleep(xfull_bar(xslot), xph, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 458); *abort_flag = 1; ok = false; break; }
             const uint32_t ab = s_xs + (uint32_t)(xslot * XS_BYTES) + X_BYTES;
             const bool coded = tg_lds_u32(s_mode + 4u * xslot) != 0u;   // int8 codes [row] + second-level maximum [row], or fp32 [row][4]
             const uint32_t codes = coded ? tg_lds_u32(ab + (uint32_t)(row * 4)) : 0u;
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(TG_THREADS, 1) mpsbnb_decode4_tmem_kernel(cons
                 }
                 if (bb == 0) {
                     // the A tile is free once the MMAs that read it three stages ago have completed
-                    if (!mbar_wait_sleep(aempty_bar(abuf), aph ^ 1u, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 409); *abort_flag = 1; ok = false; break; }
+                    if (!mbar_wait_sleep(aempty_bar(abuf), aph ^ 1u, abort_flag, kSleepFast)) { atomicExch(&g_tc_status, 459); *abort_flag = 1; ok = false; break; }
                     tc_fence_after();
                 }
                 tmem_st_32x32(tmem_mine + (uint32_t)(abuf * 128 + 32 * bb), out);

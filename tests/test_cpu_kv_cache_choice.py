@@ -46,3 +46,20 @@ def test_single_tokens_are_seen_for_what_they_are_without_the_longest(heads, kv_
 def test_prompts_without_the_longest_go_where_prompts_go():
     for new in ([700, 300], [2048] * 8, [1] * 30 + [900]):
         assert kernels(32, 8, new, 4096, longest=sum(new)) & PROMPTS
+
+
+def test_device_status_codes_say_which_kernel_they_are_from():
+    """Page numbers (401) and places without room (430) are the caller's business: no other kernel's code may look like them."""
+    import glob
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(N.LIB_PATH), "..", "csrc")
+    owners = {}
+    for path in glob.glob(os.path.join(csrc, "*.cu")):
+        text = open(path).read()
+        codes = set(map(int, re.findall(r"_status, (\d+)\)", text))) | set(map(int, re.findall(r"AP_WAIT\([^;]*?, (\d+)\)", text)))
+        for code in codes:
+            owners.setdefault(code, set()).add(os.path.basename(path))
+    assert len(owners) > 30
+    assert not {c: f for c, f in owners.items() if len(f) > 1}
+    assert not {401, 430} & set(owners)
