@@ -495,13 +495,13 @@ int mpsbnb_kv4_copy_pages(const mpsbnb_kv4_cache *cache, const int32_t *src, con
  * Scores, softmax statistics and sums are fp32.  fp16 products: single tokens round the 16 code values and the weights
  * probability * absmax, prompts code * absmax (keys and values) and the probabilities.
  * A key whose absmax is not finite makes the rows that see it NaN; a value's makes NaN of its block's channels in those rows
- * (single tokens) or of the rows (prompts).  Which of two kernels runs (both, where prompts and single tokens are mixed) -
+ * (single tokens, and what is done again, below) or of the rows (prompts).  Which of two kernels runs (both, where prompts and single tokens are mixed) -
  * and with it the rounding - depends on the numbers of rows, heads and sequences, on the window and on table_width, the room
  * for keys: never on the lengths, so a captured graph follows them.
- * Keys and values of any magnitude may lie side by side: those that a row does not see, or sees with next to no weight, take nothing
- * from its precision.  (Where the magnitudes of blocks of keys, or of values, that some block of rows sees are more than 2^22
- * apart, or a score times log2(e) is 2^20 or more, the sequence's prompt is done again by the kernel for single tokens, some ten times slower.  An absmax of 1e-8 or less
- * counts as nothing beside a larger one.)
+ * Keys and values of any magnitude may lie side by side: those that a row does not see, or sees with next to no weight, take
+ * nothing from its precision.  (Where the magnitudes of blocks of keys, or of values, that some block of rows sees are more
+ * than 2^22 apart, or a score times log2(e) is 2^20 or more, a sequence of the prompt kernel is done again by the one for single
+ * tokens, some ten times slower.  An absmax of 1e-8 or less counts as nothing beside a larger one.)
  * workspace: mpsbnb_attention_4bit_workspace_bytes() bytes, 16-byte aligned, used by this call only while it runs. */
 size_t mpsbnb_attention_4bit_workspace_bytes(const mpsbnb_kv4_cache *cache, const mpsbnb_kv4_seqs *seqs, int heads);
 int mpsbnb_attention_4bit(const mpsbnb_kv4_cache *cache, int layer, const mpsbnb_kv4_seqs *seqs, const void *q,

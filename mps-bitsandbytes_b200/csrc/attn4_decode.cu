@@ -3,10 +3,12 @@
 //
 // Floor: HBM, for the cached bytes (head_dim / 2 + 2 head_dim / blocksize per token, head and side) are read once and
 // the arithmetic per byte is small.  Bound: turning 4-bit codes into operands at that rate.  64 sequences of up to 16384 places
-// (8 kv heads of 128, 8 query heads each: 545 MB) take 151 us, 3.6 TB/s, 0.55 of what a copy reaches; 57 % of the issue slots and 61 %
-// of the load pipe are then in use (326 instructions and 128 look-ups a lane for 16 tokens), the tensor pipe at 22 %.  Tried for it:
-// 8 warps a block (+20 %) and 16 (=) for 12; codes straight from global memory instead of the ring (+10 %); the next tile's
-// scores under this one's values (=); all look-ups of a block before its products (=).
+// (8 kv heads of 128, 8 query heads each: 545 MB) take 152 us, 3.6 TB/s, 0.55 of what a copy reaches; 57 % of the issue slots and 60 %
+// of the load pipe are then in use (331 instructions and 64 look-ups a lane for 16 tokens; of 108 wavefronts of shared memory 18 are
+// conflicts of the loads of codes, 64 bytes a row: tokens four apart for K, two for V), the tensor pipe at 22 %.  No unit is at its
+// limit: most stalls are fixed latencies, with three warps a scheduler to hide them.  Tried for it: 8 warps a block (+20 %) and 16 (=) for
+// 12; codes straight from global memory instead of the ring (+10 %); the next tile's scores under this one's values (=); all look-ups of
+// a block before its products (=).  head_dim 256 with 16-row tiles spills 420 - 520 bytes a thread, the others next to nothing.
 // Little work is bound by latency: 14 us for two launches, however short the sequences are (32 heads of 200 keys).
 //
 //  * Work is a list of (sequence, kv head, row tile, key tile), cut into equal runs, one per team of four warps,
@@ -28,7 +30,8 @@
 //    more products and conversions): an output is off by 2.9e-4 - 3.6e-4 of its size, where its own rounding to fp16 makes 2.1e-4;
 //    in bf16 nothing is to be seen of it.  absmax is taken times a power of two that brings a tile's to [2^-4, 2^7]; the same
 //    vote sees when they leave that.  A tile that has more between its smallest and its largest takes a power of two for each row
-//    and block, after that row's largest weight: what other rows see, or what has next to no weight, costs a row no bits.
+//    and block, after that row's largest weight: what other rows see, or what has next to no weight, costs a row no bits.  (The
+//    vote and the room in the instruction cache cost 1.5 - 3 %; a cache all of whose tiles are like that takes half as long again.)
 //    bf16 queries are brought to fp16 by a power of two per row: exact, but for parts below 2^-24 of the row's largest.
 #include <cmath>
 #include <type_traits>
@@ -812,14 +815,15 @@ static AdKind ad_kind(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int g
 
 // Prompts among single tokens, as a server batches them: both kernels, each for its sequences.  It may be so where the longest has
 // four times the average's rows and alone would go to the prompt kernel.  (256 sequences over 4096 keys, one with 2048 new tokens, 32
-// heads on 8: 459 us; by the prompt kernel alone 1170, as two calls 156 and 276.)
+// heads on 8: 463 us; by the prompt kernel alone 1170, as two calls 156 and 276: one after the other, nothing overlaps.)
 static bool ad_mixed(const mpsbnb_kv4_cache *c, const mpsbnb_kv4_seqs *s, int group, int window) {
     if (s->cu_seqlens == nullptr || 4 * s->tokens > (int64_t)s->batch * ad_longest(s)) return false;
     mpsbnb_kv4_seqs one = *s;
     one.batch = 1; one.new_tokens = (int)ad_longest(s); one.tokens = one.new_tokens;
     return ad_kind(c, &one, group, window) != AD_TOKENS;
 }
-// rows a head up to which a sequence of a mixed call counts as single tokens: where the kernels' times per key meet
+// rows a head up to which a sequence of a mixed call counts as single tokens: the kernels' times per key meet at 4.7, 2.9, 1.5 tiles of
+// 16 rows (above), taken up to whole tiles
 static int ad_few_rows(int D) { return D == 64 ? 80 : D == 128 ? 48 : 32; }
 
 // what a call runs: both kernels (mixed) or one; how the prompt kernel does; 8-row tiles of single tokens

@@ -3,11 +3,12 @@
 //
 // Floor: the tensor pipe (4 rows keys head_dim operations) and, level with it at head_dim 128, the exponentials (16 a clock
 // and SM).  A tile of 256 rows and 128 keys: 2050 clocks for the products, 2050 for the powers, 3200 of shared memory (look-ups of
-// codes 1000, expanded operands written 500 and read by the products 1500 - 1700); it takes about 4400.  64 heads on 8 of 128,
-// 4096 tokens, causal: 344 us, 0.8 PFLOP/s of what the mask leaves, tensor pipe 40 - 44 % busy.
-// Without the expanders' arithmetic it takes 303 us, without the softmax's 231, without both 198: what is left is products and
-// hand-overs, and each of the two adds to them through shared memory and issue slots rather than by being waited for - P announced by
-// halves, so that its first products begin early, changed nothing (344 us).
+// codes 1000, expanded operands written 500 and read by the products 1500 - 1700); it takes about 4500.  64 heads on 8 of 128,
+// 4096 tokens, causal: 366 us, 0.75 PFLOP/s of what the mask leaves, tensor pipe 39 - 44 % busy; of 64, 303 us, 0.45 (powers and
+// expanding cost the same, products half).  When it took 344 us it took 303 without the expanders' arithmetic, 231 without the softmax's,
+// 198 without both: what is left is products and hand-overs, and each of the two adds to them through shared memory and issue slots rather
+// than by being waited for - P announced by halves, so that its first products begin early, changed nothing.  The roles' code does not
+// fit the instruction cache together (1 of 9 stalled warps waits for it): 20 instructions more in a role cost 2 - 3 %.
 //
 // A block takes 256 rows (or the last 128) of one (sequence, kv head) at a time, long ones first; a row is a (new token,
 // head of the group) pair, so all heads of a group share each expanded tile.  Two 128-row tiles A and B alternate: while
@@ -28,12 +29,14 @@
 // Where few blocks of rows would leave SMs idle, a block takes an equal run of all their key tiles instead, and partial results are
 // joined (attn4.cuh): 8 heads of 1024 rows over 8192 keys 71 us, of 4096 rows over 32768 keys 583.
 // Rounding: code * absmax of K and of V and the powers P go to fp16 once each, 2.1e-4 in the root mean square; an fp16 output is then
-// off by 4.8e-4 of its size, half a step of its type (its own rounding: 2.1e-4 on average); a bf16 output shows nothing of it.
+// off by 4.8e-4 of its size, half a step of its type (its own rounding: 2.1e-4 on average), a bf16 output by 1.76e-3 where its own
+// rounding makes 1.66e-3 (24 000 keys).
 // Products in TF32 would halve the rate and double the operands.
 // fp16 operands hold bf16 caches too: the absmax of a K tile (and, carried along, of the V tiles) is brought near 2^8 by
 // a power of two that the scores' factor (and the end of the row, or a rescale of O) takes back.  Blocks of elements that this
 // leaves under 2^-14, of which fp16 keeps too few bits, are noticed: their sequence is done again by attn4_decode_kernel, which
-// takes any magnitudes side by side, and scores of any size.
+// takes any magnitudes side by side, and scores of any size: its launch costs 5 us where it finds nothing to do, the look at the
+// magnitudes 0 - 3 %; a prompt of 4096 that is done again takes 4.0 ms.
 #include <type_traits>
 
 #include "attn4.cuh"
@@ -50,7 +53,8 @@ constexpr float AP_LIFT = 7.0f;
 constexpr int AP_EXPAND = 8, AP_EXPANDERS = 8;                       // first expander warp, their number
 constexpr int AP_MMA = 16, AP_LOAD = 17, AP_Q = 18, AP_THREADS = 20 * 32;
 // Registers: launched with 96 a thread (640 threads); the warpgroups then share them out anew.  (A spilled register costs a
-// trip to L2 here: shared memory leaves next to nothing of L1.)
+// trip to L2 here: shared memory leaves next to nothing of L1.  head_dim 64 and 128 spill 80 - 116 bytes a thread of the softmax: 1.5 % of
+// all instructions.)
 constexpr int AP_REGS = 96, AP_REGS_SOFTMAX = 128, AP_REGS_EXPAND = 72, AP_REGS_OTHER = 80;
 static_assert(2 * AP_REGS_SOFTMAX + 2 * AP_REGS_EXPAND + AP_REGS_OTHER <= 5 * AP_REGS, "a raise beyond the launch's registers would wait for ever");
 template <int N> __device__ __forceinline__ void ap_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }

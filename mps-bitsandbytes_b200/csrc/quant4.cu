@@ -337,7 +337,7 @@ quantize4_stream_kernel(const T *__restrict__ A, IDX total, uint8_t *__restrict_
 // The codes are quantize_4bit's without its division.  x and the block's a are 16-bit numbers, so there are few quotients x / a near a
 // threshold: x * fl(1 / a) lies on the side of it that x / a lies on, with NF4's thresholds as they are and with FP4's, which
 // x / a can equal, taken 2^-16 larger in magnitude.  oracle/oracle.c:o_prove_kv4_thresholds tries every x and a.
-// Floor: the rows' bytes.  Bound: instruction issue, 76 % of the slots.  28 900 tokens of 8 heads of 128, FP4 from bf16: 62 us for
+// Floor: the rows' bytes.  Bound: instruction issue, 76 % of the slots, some 20 instructions an element.  28 900 tokens of 8 heads of 128, FP4 from bf16: 62 us for
 // 150 MB in and out, 2.4 TB/s.  64 registers a thread: with 80 or 48 it takes 70 and 75.
 // ------------------------------------------------------------------------------------------
 static __device__ int g_kv4_append_status = 0;
