@@ -224,3 +224,42 @@ def test_an_output_that_is_not_contiguous_is_refused():
                 torch.zeros(2 * 3 * 8 * 128 + 1, device="cuda", dtype=F16)[1:].view(q.shape)):
         with pytest.raises(ValueError, match="out must be"):
             bnb.attention_4bit(q, cache, 0, _i32([[0, 1], [2, 3]]), _i32([3, 4]), out=out)
+
+
+def test_calls_without_tokens_or_sequences():
+    cache = bnb.KVCache4bit(1, 4, 2, 64)
+    before = cache.data.clone()
+    table, lens = _i32([[0, 1], [2, 3]]), _i32([5, 0])
+    for q, args in ((torch.zeros(0, 8, 64, device="cuda", dtype=F16), (table, lens, _i32([0, 0, 0]))), (torch.zeros(2, 0, 8, 64, device="cuda", dtype=F16), (table, lens)),
+                    (torch.zeros(0, 8, 64, device="cuda", dtype=F16), (table[:0], lens[:0], _i32([0]))), (torch.zeros(0, 1, 8, 64, device="cuda", dtype=F16), (table[:0], lens[:0]))):
+        out, lse = bnb.attention_4bit(q, cache, 0, *args, return_lse=True)
+        assert out.shape == q.shape and lse.shape == q.shape[:-1]
+        bnb.append_kv_4bit(cache, 0, q[..., :2, :], q[..., :2, :], *args)
+    # rows that belong to no sequence, for the kernels of either kind
+    for rows in (5, 3000):
+        q = torch.randn(rows, 8, 64, device="cuda", dtype=F16)
+        out, lse = bnb.attention_4bit(q, cache, 0, table, lens, _i32([0, 0, 0]), return_lse=True)
+        assert (out == 0).all() and torch.isinf(lse).all()
+        bnb.append_kv_4bit(cache, 0, q[:, :2], q[:, :2], table, lens, _i32([0, 0, 0]))
+    assert torch.equal(cache.data, before)
+    assert_device_ok()
+
+
+def test_prompts_done_again_on_two_streams_at_once():
+    """Each call has its own list of what is to be done again."""
+    import kv_util as U
+    cache = U.make_cache(40, 8, 128, 64, dtype=BF16, seed=9)
+    plain, wide = U.widen(_i32([list(range(20))]), 64), U.widen(_i32([list(range(20, 40))]), 64)
+    cache.v_absmax[0, 25, :, 1, 3] = 1e14
+    qs = [torch.randn(1, 1100, 32, 128, device="cuda").to(BF16) for _ in range(2)]
+    lens = _i32([1200])
+    want = [bnb.attention_4bit(q, cache, 0, t, lens) for q, t in zip(qs, (plain, wide))]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i, t in enumerate((plain, wide)):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(bnb.attention_4bit(qs[i], cache, 0, t, lens))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])
+    assert_device_ok()
